@@ -30,6 +30,16 @@ from .core import (
     set_packing_bitwidth,
 )
 from .dtypes import DTYPE_TO_TORCH, TORCH_TO_DTYPE, DType, is_mx_dtype
+from .experts import (
+    ExpertPlan,
+    GemLiteExperts,
+    GemLiteMoE,
+    experts_combined_functional,
+    experts_functional,
+    experts_gated_functional,
+    plan_experts,
+    route_experts,
+)
 from .quant_utils import (
     WeightQuantizerMXFP,
     quantize_weights_per_channel,

@@ -5,6 +5,7 @@ The library is built in-tree by ``gemlite_amd/csrc/Makefile`` (or
 object is missing, or a call returns a non-zero status, the caller gets an
 exception.
 """
+import contextlib
 import ctypes
 import os
 import threading
@@ -80,6 +81,47 @@ class MatmulArgs(ctypes.Structure):
     ]
 
 
+class ExpertsArgs(ctypes.Structure):
+    """Mirror of ``gla_experts_args``; field order and types must match the header."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("mode", ctypes.c_int32),
+        ("x", ctypes.c_void_p),
+        ("w", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("zeros", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_uint64),
+        ("offsets", ctypes.c_void_p),
+        ("order", ctypes.c_void_p),
+        ("places", ctypes.c_void_p),
+        ("weights", ctypes.c_void_p),
+        ("w_stride_e", ctypes.c_int64),
+        ("meta_stride_e", ctypes.c_int64),
+        ("x_stride_m", ctypes.c_int64),
+        ("out_stride_m", ctypes.c_int64),
+        ("R", ctypes.c_int32),
+        ("T", ctypes.c_int32),
+        ("top_k", ctypes.c_int32),
+        ("E", ctypes.c_int32),
+        ("N", ctypes.c_int32),
+        ("K", ctypes.c_int32),
+        ("W_nbits", ctypes.c_int32),
+        ("group_size", ctypes.c_int32),
+        ("elements_per_sample", ctypes.c_int32),
+        ("input_dtype", ctypes.c_int32),
+        ("output_dtype", ctypes.c_int32),
+        ("meta_dtype", ctypes.c_int32),
+        ("x_dtype", ctypes.c_int32),
+        ("channel_scale_mode", ctypes.c_int32),
+        ("W_group_mode", ctypes.c_int32),
+        ("tile_config", ctypes.c_int32),
+    ]
+
+
 _lib = None
 _lib_lock = threading.Lock()
 
@@ -129,6 +171,18 @@ SYMBOLS = {
         ctypes.c_int,
         [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_void_p],
     ),
+    "gla_route_workspace_bytes": (ctypes.c_int64, [ctypes.c_int, ctypes.c_int]),
+    "gla_route_experts": (
+        ctypes.c_int,
+        [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+         ctypes.c_float] + [ctypes.c_void_p] * 6 + [ctypes.c_int64, ctypes.c_void_p],
+    ),
+    "gla_plan_experts": (
+        ctypes.c_int,
+        [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int] + [ctypes.c_void_p] * 4 + [ctypes.c_int64, ctypes.c_void_p],
+    ),
+    "gla_experts_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(ExpertsArgs)]),
+    "gla_experts_matmul": (ctypes.c_int, [ctypes.POINTER(ExpertsArgs), ctypes.c_void_p]),
 }
 
 
@@ -513,3 +567,65 @@ def unpack_over_cols(packed: torch.Tensor, out: torch.Tensor, rows: int, pcols: 
         ),
         "gla_unpack_over_cols",
     )
+
+
+# ---------------------------------------------------------------------------
+# mixture of experts
+# ---------------------------------------------------------------------------
+def _on_device(device: torch.device):
+    """Makes ``device`` the current one for a launch (nothing to do where it is already)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def route_experts(logits, top_k, scoring, renormalize, scale, weights, ids, offsets, order, places):
+    _require_cuda(logits, weights, ids, offsets, order, places)
+    lib = load_library()
+    T, E = logits.shape
+    need = lib.gla_route_workspace_bytes(T, E)
+    if need < 0:
+        _check(int(need), "gla_route_workspace_bytes")
+    with _on_device(logits.device):
+        counts = torch.empty(need, dtype=torch.uint8, device=logits.device)
+        _check(
+            lib.gla_route_experts(
+                logits.data_ptr(), TORCH_TO_DTYPE[logits.dtype].value if logits.dtype in TORCH_TO_DTYPE else -1, logits.stride(0),
+                T, E, int(top_k), int(scoring), int(bool(renormalize)), float(scale), weights.data_ptr(), ids.data_ptr(),
+                offsets.data_ptr(), order.data_ptr(), places.data_ptr(), counts.data_ptr(), need, _stream_ptr(logits.device),
+            ),
+            "gla_route_experts",
+        )
+
+
+def plan_experts(ids, num_experts, offsets, order, places):
+    _require_cuda(ids, offsets, order, places)
+    lib = load_library()
+    T, k = ids.shape
+    need = lib.gla_route_workspace_bytes(T, int(num_experts))
+    if need < 0:
+        _check(int(need), "gla_route_workspace_bytes")
+    with _on_device(ids.device):
+        counts = torch.empty(need, dtype=torch.uint8, device=ids.device)
+        _check(
+            lib.gla_plan_experts(ids.data_ptr(), T, int(num_experts), k, offsets.data_ptr(), order.data_ptr(), places.data_ptr(),
+                                 counts.data_ptr(), need, _stream_ptr(ids.device)),
+            "gla_plan_experts",
+        )
+
+
+def experts_matmul(args: ExpertsArgs, device: torch.device):
+    """Launch ``gla_experts_matmul`` on the current stream of ``device``.  Its workspace (fp32 rows, contents arbitrary)
+    comes from torch's allocator for this call, so calls on several streams or in several captured graphs share none."""
+    lib = load_library()
+    args.struct_size = ctypes.sizeof(ExpertsArgs)
+    ref = ctypes.byref(args)
+    need = lib.gla_experts_workspace_bytes(ref)
+    if need < 0:
+        _check(int(need), "gla_experts_workspace_bytes")
+    with _on_device(device):
+        if need > 0:
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+            args.workspace = workspace.data_ptr()
+            args.workspace_bytes = need
+        _check(lib.gla_experts_matmul(ref, _stream_ptr(device)), "gla_experts_matmul")

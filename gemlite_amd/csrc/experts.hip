@@ -1,0 +1,338 @@
+// C entry points of the mixture-of-experts operators: argument checks, the choice between the streaming kernel and the
+// tiled GEMM, and the finishing kernel that joins K splits and the experts of a token.
+#include "common.hpp"
+#include "experts.hpp"
+
+namespace gla {
+
+namespace {
+
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+
+struct FinishArgs {
+    const float* partials;   // [S][R][N]
+    const int32_t* offsets;
+    const int32_t* places;   // combined: [T][k]
+    const float* weights;    // combined: [T][k]
+    void* out;
+    int64_t osm;
+    int R, E, N, S, k, half;
+};
+
+// out[r] = sum of the splits (gated: silu(gate) * up of it), or zeros where the row has no expert; combined: out[t] =
+// sum over the token's slots of weight * sum of the splits of its row.  All sums in fp32, in a fixed order; bound by the
+// fp32 rows it reads.  A thread takes 4 columns of one row.
+template <bool BF16, bool COMBINED>
+__global__ __launch_bounds__(256) void experts_finish_kernel(FinishArgs a) {
+    const int64_t row = blockIdx.x;
+    const int width = a.half ? a.half : a.N;
+    const int c = (blockIdx.y * 256 + threadIdx.x) * 4;
+    if (c >= width) return;
+    int limit = a.offsets[a.E];
+    if (limit > a.R) limit = a.R;
+    const int64_t slab = (int64_t)a.R * a.N;
+    auto sum_at = [&](int64_t r, int col) __attribute__((always_inline)) {
+        const float* p = a.partials + r * a.N + col;
+        float4_t v = *(const float4_t*)p;
+        for (int s = 1; s < a.S; ++s) v += *(const float4_t*)(p + s * slab);
+        return v;
+    };
+    float4_t v = float4_t{0.f, 0.f, 0.f, 0.f};
+    if constexpr (COMBINED) {
+        for (int j = 0; j < a.k; ++j) {
+            const int p = a.places[row * a.k + j];
+            if (p < 0 || p >= limit) continue;
+            const float w = a.weights[row * a.k + j];
+            const float4_t y = sum_at(p, c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = __builtin_fmaf(w, y[i], v[i]);
+        }
+    } else if (row < limit) {
+        v = sum_at(row, c);
+        if (a.half) {
+            const float4_t up = sum_at(row, c + a.half);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = silu_mul(v[i], up[i]);
+        }
+    }
+    *(u32x2*)((uint16_t*)a.out + row * a.osm + c) = u32x2{pack16<BF16>(v[0], v[1]), pack16<BF16>(v[2], v[3])};
+}
+
+int format_of(const gla_experts_args& p) {
+    if (p.W_nbits == 4 && p.elements_per_sample == 8 && p.channel_scale_mode == GLA_CSM_NONE &&
+        (p.input_dtype == GLA_DT_FP16 || p.input_dtype == GLA_DT_BF16))
+        return kEW4;
+    if (p.W_nbits == 8 && p.elements_per_sample == 1 && p.channel_scale_mode == GLA_CSM_BLOCK && p.input_dtype == GLA_DT_FP8 &&
+        p.W_group_mode == GLA_WGM_NONE)
+        return kEF8;
+    if (p.W_nbits == 16 && p.elements_per_sample == 1 && p.channel_scale_mode == GLA_CSM_NONE && p.W_group_mode == GLA_WGM_NONE &&
+        (p.input_dtype == GLA_DT_FP16 || p.input_dtype == GLA_DT_BF16))
+        return kE16;
+    return -1;
+}
+
+bool aligned(const void* p, int64_t bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
+
+int validate(const gla_experts_args* p) {
+    if (p == nullptr || p->struct_size != sizeof(gla_experts_args)) {
+        set_error("experts: struct_size does not match this library");
+        return GLA_ERR_INVALID_ARGUMENT;
+    }
+    if (p->mode < GLA_EXPERTS_ROWS || p->mode > GLA_EXPERTS_COMBINED) {
+        set_error("experts: mode %d", p->mode);
+        return GLA_ERR_UNSUPPORTED_MODE;
+    }
+    const bool combined = p->mode == GLA_EXPERTS_COMBINED, gated = p->mode == GLA_EXPERTS_GATED;
+    if (p->R < 0 || p->T < 0 || p->E <= 0 || p->E > GLA_EXPERTS_MAX || p->N <= 0 || p->K <= 0) {
+        set_error("experts: R=%d T=%d E=%d (1..%d) N=%d K=%d", p->R, p->T, p->E, GLA_EXPERTS_MAX, p->N, p->K);
+        return GLA_ERR_INVALID_ARGUMENT;
+    }
+    if (p->output_dtype != GLA_DT_FP16 && p->output_dtype != GLA_DT_BF16) {
+        set_error("experts: output type %d (fp16 and bf16 are built)", p->output_dtype);
+        return GLA_ERR_UNSUPPORTED_DTYPE;
+    }
+    const int fmt = format_of(*p);
+    if (fmt < 0) {
+        set_error("experts: W_nbits=%d elements_per_sample=%d input_dtype=%d output_dtype=%d channel_scale_mode=%d W_group_mode=%d is not built "
+                  "(4-bit codes in 32-bit words with group scales, fp8 with 128 x 128 block scales, 16-bit weights)",
+                  p->W_nbits, p->elements_per_sample, p->input_dtype, p->output_dtype, p->channel_scale_mode, p->W_group_mode);
+        return GLA_ERR_UNSUPPORTED_MODE;
+    }
+    if (p->x_dtype != p->output_dtype || (fmt != kEF8 && p->input_dtype != p->x_dtype)) {
+        set_error("experts: activations of type %d (input type %d) with output type %d", p->x_dtype, p->input_dtype, p->output_dtype);
+        return GLA_ERR_UNSUPPORTED_DTYPE;
+    }
+    if (p->tile_config != -1) {
+        const int rows = p->tile_config % 1000, splits = p->tile_config / 1000;
+        if (p->tile_config < 0 || splits > 64 || (rows != 16 && rows != 32)) {
+            set_error("experts: tile_config %d", p->tile_config);
+            return GLA_ERR_INVALID_ARGUMENT;
+        }
+    }
+    const int kstep = fmt == kEF8 ? 128 : 32;
+    if (p->K % kstep != 0 || p->N % (gated ? 16 : 8) != 0) {
+        set_error("experts: K=%d has to be a multiple of %d, N=%d of %d", p->K, kstep, p->N, gated ? 16 : 8);
+        return GLA_ERR_MISALIGNED_SHAPE;
+    }
+    const int64_t expert_bytes = fmt == kEW4 ? (int64_t)p->K / 2 * p->N : (int64_t)p->K * p->N * (fmt == kE16 ? 2 : 1);
+    if (expert_bytes >= (int64_t)1 << 31) {
+        set_error("experts: one expert's weights take %lld bytes (2^31 or more)", (long long)expert_bytes);
+        return GLA_ERR_UNSUPPORTED_MODE;
+    }
+    if (p->R > 0) {
+        if (!p->x || !p->w || !p->out || !p->offsets || (gated && !p->order) || (combined && (!p->places || !p->weights))) {
+            set_error("experts: NULL pointer");
+            return GLA_ERR_INVALID_ARGUMENT;
+        }
+        if (p->x_stride_m < p->K || p->out_stride_m < (gated ? p->N / 2 : p->N)) {
+            set_error("experts: row strides %lld / %lld are shorter than the rows", (long long)p->x_stride_m, (long long)p->out_stride_m);
+            return GLA_ERR_INVALID_ARGUMENT;
+        }
+        if (!aligned(p->x, 16) || p->x_stride_m % 8 || !aligned(p->w, 16) || p->w_stride_e % 16 || !aligned(p->out, 8) || p->out_stride_m % 4 ||
+            !aligned(p->scales, fmt == kEF8 ? 4 : 16) || !aligned(p->zeros, 16) || p->meta_stride_e % (fmt == kEF8 ? 4 : 16) ||
+            !aligned(p->bias, 16)) {
+            set_error("experts: x and its rows, w, scales, zeros and bias have to be 16-byte aligned (fp8: scales 4-byte), out and its rows 8-byte");
+            return GLA_ERR_INVALID_ARGUMENT;
+        }
+        if (p->w_stride_e < expert_bytes) {
+            set_error("experts: w_stride_e=%lld bytes is shorter than an expert's %lld", (long long)p->w_stride_e, (long long)expert_bytes);
+            return GLA_ERR_INVALID_ARGUMENT;
+        }
+        if (gated || combined) {
+            if (p->top_k <= 0 || (int64_t)p->T * p->top_k != p->R) {
+                set_error("experts: T=%d tokens of %d slots are not the plan's R=%d rows", p->T, p->top_k, p->R);
+                return GLA_ERR_INVALID_ARGUMENT;
+            }
+        }
+        if (fmt == kEF8 && (!p->scales || p->meta_dtype != GLA_DT_FP32)) {
+            set_error("experts: fp8 experts need fp32 block scales");
+            return GLA_ERR_INVALID_ARGUMENT;
+        }
+    }
+    if (fmt == kEW4) {
+        if (p->group_size <= 0 || p->group_size % 32 != 0 || p->K % p->group_size != 0) {
+            set_error("experts: groups of %d K-values (multiples of 32 that divide K=%d)", p->group_size, p->K);
+            return GLA_ERR_MISALIGNED_SHAPE;
+        }
+        if (p->W_group_mode != GLA_WGM_SCALE && p->W_group_mode != GLA_WGM_SHIFT_SCALE && p->W_group_mode != GLA_WGM_FMA) {
+            set_error("experts: W_group_mode %d of 4-bit codes (scale, shift and scale, fma are built)", p->W_group_mode);
+            return GLA_ERR_UNSUPPORTED_MODE;
+        }
+        if (p->meta_dtype != GLA_DT_FP16 && p->meta_dtype != GLA_DT_BF16) {
+            set_error("experts: scales of type %d (fp16 and bf16 are built)", p->meta_dtype);
+            return GLA_ERR_UNSUPPORTED_DTYPE;
+        }
+        if (p->R > 0 && (!p->scales || (p->W_group_mode != GLA_WGM_SCALE && !p->zeros))) {
+            set_error("experts: NULL scales or zeros");
+            return GLA_ERR_INVALID_ARGUMENT;
+        }
+    }
+    return GLA_OK;
+}
+
+struct ExpertPlanHost {
+    int format;
+    int bm;      // 0: streaming kernel
+    int row_tiles;
+    int S;
+    bool to_partials;
+    bool quantise;                       // F8: a launch in front writes codes and scales to the workspace
+    int64_t partial_bytes, code_bytes, total_bytes;  // of the workspace: fp32 rows, codes, scales
+};
+
+ExpertPlanHost plan_of(const gla_experts_args& p) {
+    ExpertPlanHost h;
+    h.format = format_of(p);
+    h.bm = 0;
+    const int want_rows = p.tile_config < 0 ? 0 : p.tile_config % 1000, want_s = p.tile_config < 0 ? 0 : p.tile_config / 1000;
+    const int active = p.R < p.E ? p.R : p.E;
+    const int per = active > 0 ? p.R / active : 0;
+    h.row_tiles = want_rows == 16 ? 1 : (want_rows == 32 || per > 8 ? 2 : 1);
+    h.S = want_s > 0 ? want_s : 1;
+    h.to_partials = p.mode == GLA_EXPERTS_COMBINED || h.S > 1;
+    h.partial_bytes = h.to_partials ? (int64_t)h.S * p.R * p.N * 4 : 0;
+    const int64_t rows = p.mode == GLA_EXPERTS_GATED ? p.T : p.R;
+    h.quantise = h.format == kEF8 && (h.bm > 0 || h.row_tiles > 1);
+    h.code_bytes = h.quantise ? rows * p.K : 0;
+    h.total_bytes = h.partial_bytes + h.code_bytes + (h.quantise ? rows * (p.K / 128) * 4 : 0);
+    return h;
+}
+
+}  // namespace
+
+}  // namespace gla
+
+using namespace gla;
+
+extern "C" {
+
+int64_t gla_experts_workspace_bytes(const gla_experts_args* p) {
+    const int rc = validate(p);
+    if (rc != GLA_OK) return rc;
+    return plan_of(*p).total_bytes;
+}
+
+int gla_experts_matmul(const gla_experts_args* p, void* stream) {
+    const int rc = validate(p);
+    if (rc != GLA_OK) return rc;
+    if (p->R == 0) return GLA_OK;
+    const ExpertPlanHost h = plan_of(*p);
+    if (h.total_bytes > 0 && (p->workspace == nullptr || (int64_t)p->workspace_bytes < h.total_bytes || !aligned(p->workspace, 16))) {
+        set_error("experts: a 16-byte aligned workspace of %lld bytes required, %llu given", (long long)h.total_bytes,
+                  (unsigned long long)p->workspace_bytes);
+        return GLA_ERR_WORKSPACE_TOO_SMALL;
+    }
+    const bool bf16 = p->output_dtype == GLA_DT_BF16;
+    ExpertArgs a{};
+    a.x = (const unsigned char*)p->x;
+    a.w = (const unsigned char*)p->w;
+    a.scales = (const unsigned char*)(p->scales != nullptr ? p->scales : p->w);
+    a.zeros = p->W_group_mode == GLA_WGM_SCALE ? nullptr : (const unsigned char*)p->zeros;
+    a.bias = p->bias;
+    a.out = p->out;
+    a.partials = (float*)p->workspace;
+    a.offsets = p->offsets;
+    a.order = p->mode == GLA_EXPERTS_GATED ? p->order : nullptr;
+    a.w_stride_e = p->w_stride_e;
+    a.meta_stride_e = p->meta_stride_e;
+    a.xsm = p->x_stride_m * 2;
+    a.osm = p->out_stride_m;
+    a.R = p->R;
+    a.E = p->E;
+    a.N = p->N;
+    a.K = p->K;
+    a.top_k = p->top_k;
+    a.half = p->mode == GLA_EXPERTS_GATED ? p->N / 2 : 0;
+    a.S = h.S;
+    a.to_partials = h.to_partials;
+    a.group = p->group_size;
+    a.meta_bf16 = p->meta_dtype == GLA_DT_BF16;
+    a.c1 = p->W_group_mode == GLA_WGM_FMA ? 1.0f : 0.0f;
+    a.c2 = p->W_group_mode == GLA_WGM_SHIFT_SCALE ? -1.0f : 0.0f;
+    hipStream_t s = (hipStream_t)stream;
+    if (h.quantise) {
+        unsigned char* codes = (unsigned char*)p->workspace + h.partial_bytes;
+        float* scales_x = (float*)(codes + h.code_bytes);  // (K is a multiple of 128: aligned)
+        const int rcq = launch_experts_quantise(p->x, bf16, a.xsm, p->mode == GLA_EXPERTS_GATED ? p->T : p->R, p->K, codes, scales_x, s);
+        if (rcq != GLA_OK) return rcq;
+        a.x = codes;
+        a.xsm = p->K;
+        a.scales_x = scales_x;
+    }
+    const int rc2 = launch_experts_stream(a, h.format, bf16, h.row_tiles, s);
+    if (rc2 != GLA_OK || !h.to_partials) return rc2;
+    const bool combined = p->mode == GLA_EXPERTS_COMBINED;
+    FinishArgs f{a.partials, p->offsets, p->places, p->weights, p->out, p->out_stride_m, p->R, p->E, p->N, h.S, p->top_k, a.half};
+    const int width = a.half ? a.half : p->N;
+    const dim3 grid(combined ? p->T : p->R, (width + 1023) / 1024);
+    if (combined) {
+        if (bf16) experts_finish_kernel<true, true><<<grid, 256, 0, s>>>(f);
+        else experts_finish_kernel<false, true><<<grid, 256, 0, s>>>(f);
+    } else {
+        if (bf16) experts_finish_kernel<true, false><<<grid, 256, 0, s>>>(f);
+        else experts_finish_kernel<false, false><<<grid, 256, 0, s>>>(f);
+    }
+    return check_hip(hipGetLastError(), "experts_finish");
+}
+
+static int check_route(int64_t T, int E, int top_k, const void* ids, const void* offsets, const void* order, const void* places) {
+    if (T < 0 || E <= 0 || E > GLA_EXPERTS_MAX || top_k <= 0 || top_k > 64 || T * top_k >= ((int64_t)1 << 31)) {
+        set_error("route: T=%lld E=%d (1..%d) top_k=%d (1..64)", (long long)T, E, GLA_EXPERTS_MAX, top_k);
+        return GLA_ERR_INVALID_ARGUMENT;
+    }
+    if (offsets == nullptr || (T > 0 && (ids == nullptr || order == nullptr || places == nullptr))) {
+        set_error("route: NULL pointer");
+        return GLA_ERR_INVALID_ARGUMENT;
+    }
+    return GLA_OK;
+}
+
+int64_t gla_route_workspace_bytes(int T, int E) {
+    if (T < 0 || E <= 0 || E > GLA_EXPERTS_MAX) {
+        set_error("route: T=%d E=%d (1..%d)", T, E, GLA_EXPERTS_MAX);
+        return GLA_ERR_INVALID_ARGUMENT;
+    }
+    return (int64_t)(E + 1) * route_blocks(T) * 4;
+}
+
+static int check_counts(int T, int E, const void* workspace, int64_t bytes) {
+    const int64_t need = gla_route_workspace_bytes(T, E);
+    if (workspace == nullptr || bytes < need || !aligned(workspace, 16)) {
+        set_error("route: a 16-byte aligned workspace of %lld bytes required, %lld given", (long long)need, (long long)bytes);
+        return GLA_ERR_WORKSPACE_TOO_SMALL;
+    }
+    return GLA_OK;
+}
+
+int gla_route_experts(const void* logits, int dtype, int64_t stride, int T, int E, int top_k, int scoring, int renormalize, float scale,
+                      float* weights, int32_t* ids, int32_t* offsets, int32_t* order, int32_t* places, void* workspace,
+                      int64_t workspace_bytes, void* stream) {
+    int rc = check_route(T, E, top_k, ids, offsets, order, places);
+    if (rc != GLA_OK) return rc;
+    if (dtype != GLA_DT_FP32 && dtype != GLA_DT_FP16 && dtype != GLA_DT_BF16) {
+        set_error("route: logits of type %d (fp32, fp16 and bf16 are built)", dtype);
+        return GLA_ERR_UNSUPPORTED_DTYPE;
+    }
+    if (top_k > E || (scoring != GLA_SCORING_SOFTMAX && scoring != GLA_SCORING_SIGMOID)) {
+        set_error("route: top_k=%d of %d experts, scoring %d", top_k, E, scoring);
+        return GLA_ERR_INVALID_ARGUMENT;
+    }
+    if (T > 0 && (logits == nullptr || weights == nullptr || stride < E)) {
+        set_error("route: NULL pointer, or rows %lld apart with %d logits", (long long)stride, E);
+        return GLA_ERR_INVALID_ARGUMENT;
+    }
+    if ((rc = check_counts(T, E, workspace, workspace_bytes)) != GLA_OK) return rc;
+    return launch_route(logits, T > 0 ? dtype : GLA_DT_FP32, stride, T, E, top_k, scoring == GLA_SCORING_SIGMOID, renormalize, scale, weights, ids,
+                        offsets, order, places, (int32_t*)workspace, (hipStream_t)stream);
+}
+
+int gla_plan_experts(const int32_t* ids, int T, int E, int top_k, int32_t* offsets, int32_t* order, int32_t* places, void* workspace,
+                     int64_t workspace_bytes, void* stream) {
+    int rc = check_route(T, E, top_k, ids, offsets, order, places);
+    if (rc != GLA_OK) return rc;
+    if ((rc = check_counts(T, E, workspace, workspace_bytes)) != GLA_OK) return rc;
+    return launch_route(nullptr, 0, 0, T, E, top_k, 0, 0, 1.0f, nullptr, const_cast<int32_t*>(ids), offsets, order, places, (int32_t*)workspace,
+                        (hipStream_t)stream);
+}
+
+}  // extern "C"

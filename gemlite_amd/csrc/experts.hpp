@@ -1,0 +1,179 @@
+// Products grouped by expert: what the streaming kernel (experts_stream.hip), the tiled GEMM (experts_gemm.hip), the
+// finishing kernel and the host side (experts.hip) share.
+//
+// The R rows of a call are sorted by expert: rows offsets[e] .. offsets[e + 1] - 1 meet the weights of expert e, rows from
+// offsets[E] on meet none.  offsets lives on the device, so the host knows only R and E: a launch has as many row tiles
+// as any distribution can need, and a workgroup finds its tile (expert, first row, last row) from offsets itself.
+#pragma once
+
+#include "common.hpp"
+
+namespace gla {
+
+// weight formats
+enum ExpertFormat { kEW4 = 0, kEF8 = 1, kE16 = 2 };
+
+struct ExpertArgs {
+    const unsigned char* x;         // activation rows: fp16 / bf16, or e4m3 bytes (F8 with scales_x)
+    const unsigned char* w;         // expert 0's weights
+    const unsigned char* scales;    // W4: [E][G][N] 16-bit; F8: [E][K/128][ceil(N/128)] fp32
+    const unsigned char* zeros;     // W4: as scales, or NULL
+    const float* scales_x;          // F8: [rows of x][K/128]; NULL: x holds 16-bit rows and the kernel quantises them
+    const float* bias;              // [E][N] fp32 or NULL
+    void* out;                      // 16-bit rows (rows / gated)
+    float* partials;                // [S][R][N] fp32 (combined, or S > 1)
+    const int32_t* offsets;         // [E + 1]
+    const int32_t* order;           // gated: sorted row -> flat (token, slot) index
+    int64_t w_stride_e, meta_stride_e;  // bytes per expert of w / of scales (and zeros)
+    int64_t xsm;                    // bytes per row of x
+    int64_t osm;                    // elements per row of out
+    int R, E, N, K;
+    int top_k;                      // gated: flat index / top_k = row of x
+    int half;                       // gated: N / 2 (gate columns 0 .. half - 1, up columns half ..), else 0
+    int S;                          // K splits
+    int to_partials;                // raw fp32 sums to `partials` instead of finished rows to `out`
+    int group;                      // W4: K-values per group
+    int meta_bf16;                  // W4: type of scales and zeros
+    float c1, c2;                   // W4: zero-point term of a weight = zero * (c1 + c2 * scale)
+};
+
+// Sum of the row tiles of all experts for BM-row tiles, at most (host): a experts with rows need a + floor((R - a) / BM).
+inline int64_t max_row_tiles(int64_t R, int E, int BM) {
+    const int64_t a = R < (int64_t)E + 1 ? R : (int64_t)E + 1;  // rows without an expert count as one more
+    return a + (R - a) / BM;
+}
+
+// Inclusive sum over the wave's lanes (row shifts inside 16 lanes, then the two row broadcasts; lanes outside a shift add 0).
+__device__ __forceinline__ int wave_inclusive_sum(int v) {
+#define GLA_DPP0(ctrl, rm) __builtin_amdgcn_update_dpp(0, v, (ctrl), (rm), 0xf, false)
+    v += GLA_DPP0(0x111, 0xf);  // row_shr:1
+    v += GLA_DPP0(0x112, 0xf);  // row_shr:2
+    v += GLA_DPP0(0x114, 0xf);  // row_shr:4
+    v += GLA_DPP0(0x118, 0xf);  // row_shr:8
+    v += GLA_DPP0(0x142, 0xa);  // row_bcast:15 into rows 1 and 3
+    v += GLA_DPP0(0x143, 0xc);  // row_bcast:31 into rows 2 and 3
+#undef GLA_DPP0
+    return v;
+}
+
+struct ExpertTile {
+    int expert;   // E: the rows without an expert (they become zeros); -1: no such tile
+    int row0, row_end;
+    int total;    // row tiles in all
+};
+
+// Row tile t of the call, computed by every wave for itself: lane l counts the tiles of experts l C .. l C + C - 1
+// (C = 1 up to 63 experts), an inclusive sum over the lanes finds the lane, that lane the expert.  Offsets are clamped
+// to 0 .. R and to rising order, so no tile leaves the R rows whatever they hold.  One round trip to memory and about a
+// hundred vector instructions; a table written by the routing kernel would cost the same round trip.
+template <int BM>
+__device__ __forceinline__ ExpertTile find_tile(const int32_t* offsets, int E, int R, int t, bool with_rest) {
+    const int lane = threadIdx.x & 63;
+    const int C = (E + 1 + 63) / 64;
+    auto at = [&](int e) __attribute__((always_inline)) {
+        const int v = e > E ? R : offsets[e];
+        return v < 0 ? 0 : (v > R ? R : v);
+    };
+    auto tiles_of = [&](int e, int lo, int hi) __attribute__((always_inline)) {
+        return e > E || (e == E && !with_rest) || hi <= lo ? 0 : (hi - lo + BM - 1) / BM;
+    };
+    int mine = 0;
+    {
+        int lo = at(lane * C);
+        for (int c = 0; c < C; ++c) {
+            const int e = lane * C + c;
+            const int hi = at(e + 1);
+            mine += tiles_of(e, lo, hi);
+            lo = hi;
+        }
+    }
+    const int upto = wave_inclusive_sum(mine);
+    ExpertTile r;
+    r.total = __builtin_amdgcn_readlane(upto, 63);
+    if (t >= r.total) {
+        r.expert = -1;
+        r.row0 = r.row_end = 0;
+        return r;
+    }
+    const int owner = __builtin_ctzll(__ballot(upto > t));
+    int left = t - (upto - mine), found = -1, row0 = 0, row_end = 0;
+    int lo = at(lane * C);
+    for (int c = 0; c < C; ++c) {
+        const int e = lane * C + c;
+        const int hi = at(e + 1);
+        const int n = tiles_of(e, lo, hi);
+        if (found < 0 && left < n) {
+            found = e;
+            row0 = lo + left * BM;
+            row_end = hi;
+        }
+        left -= n;
+        lo = hi;
+    }
+    r.expert = __builtin_amdgcn_readlane(found, owner);
+    r.row0 = __builtin_amdgcn_readlane(row0, owner);
+    r.row_end = __builtin_amdgcn_readlane(row_end, owner);
+    if (r.row_end > r.row0 + BM) r.row_end = r.row0 + BM;
+    return r;
+}
+
+// Row of x that sorted row r reads.
+__device__ __forceinline__ int64_t source_row(const ExpertArgs& a, int r) {
+    if (a.order == nullptr) return r;
+    int v = a.order[r];
+    v = v < 0 ? 0 : (v > a.R - 1 ? a.R - 1 : v);
+    return v / a.top_k;
+}
+
+// Column of the weights that column c of a 64-column tile stands for: the tile's own, or (gated) 32 gate columns followed
+// by the same 32 up columns.
+__device__ __forceinline__ int tile_column(int half, int tile, int c) {
+    if (half == 0) return tile * 64 + c;
+    return tile * 32 + (c & 31) + (c < 32 ? 0 : half);
+}
+
+__device__ __forceinline__ float silu_mul(float gate, float up) { return gate / (1.0f + __expf(-gate)) * up; }
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+    if constexpr (BF16) return pack_bf16x2(lo, hi);
+    else return pack_half2(lo, hi);
+}
+
+// The scale and the reciprocal that a block of 128 activations of amax is quantised with.  (The constant's reciprocal, not
+// a division: the codes of values that lie on a border between two depend on it.)
+__device__ __forceinline__ void block_scale(float amax, float& s, float& inv) {
+    s = fmaxf(amax * (1.0f / 448.0f), 1e-6f);
+    inv = 1.0f / s;
+}
+
+// Four values of such a block -> four e4m3 codes.
+__device__ __forceinline__ uint32_t quantise4(float a, float b, float c, float d, float inv) {
+    auto lim = [](float v) __attribute__((always_inline)) { return __builtin_amdgcn_fmed3f(v, -448.0f, 448.0f); };
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(lim(a * inv), lim(b * inv), 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(lim(c * inv), lim(d * inv), r, true);
+}
+
+template <bool BF16>
+__device__ __forceinline__ float low16(uint32_t v) {
+    if constexpr (BF16) return __builtin_bit_cast(float, v << 16);
+    else return half_bits_to_float((uint16_t)v);
+}
+template <bool BF16>
+__device__ __forceinline__ float high16(uint32_t v) {
+    if constexpr (BF16) return __builtin_bit_cast(float, v & 0xffff0000u);
+    else return half_bits_to_float((uint16_t)(v >> 16));
+}
+
+// 16-bit rows -> e4m3 codes [rows][K] and scales [rows][K/128] (experts_quant.hip)
+int launch_experts_quantise(const void* x, bool bf16, int64_t xsm, int rows, int K, unsigned char* codes, float* scales, hipStream_t stream);
+
+int launch_experts_stream(const ExpertArgs& a, int format, bool bf16, int row_tiles, hipStream_t stream);
+int launch_experts_gemm(const ExpertArgs& a, int format, bool bf16, int bm, hipStream_t stream);
+
+// logits NULL: the ids are given and only sorted.  counts: (E + 1) * route_blocks(T) integers of scratch.
+int route_blocks(int T);
+int launch_route(const void* logits, int dtype, int64_t stride, int T, int E, int top_k, int sigmoid, int renormalize, float scale,
+                 float* weights, int32_t* ids, int32_t* offsets, int32_t* order, int32_t* places, int32_t* counts, hipStream_t stream);
+
+}  // namespace gla

@@ -308,6 +308,81 @@ int gla_pack_over_cols(const uint8_t* codes, void* out, int64_t rows, int64_t co
 int gla_unpack_over_cols(const void* packed, uint8_t* out, int64_t rows, int64_t packed_cols,
                          int W_nbits, int packing_bitwidth, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Mixture of experts (no counterpart in the reference): routing, and quantised products grouped by expert.
+ *
+ * A plan sorts the R = T * top_k (token, slot) pairs by expert: order[p] is the flat index token * top_k + slot of
+ * sorted row p (within an expert in rising order), places[token * top_k + slot] the sorted row of a pair, and rows
+ * offsets[e] .. offsets[e + 1] - 1 belong to expert e.  Pairs without an expert (id < 0 or >= E) come last, from
+ * offsets[E] on.  offsets, order and places are device memory; the kernels keep whatever they hold inside the R rows. */
+#define GLA_EXPERTS_MAX 1024
+
+#define GLA_SCORING_SOFTMAX 0
+#define GLA_SCORING_SIGMOID 1
+
+/* ids[T, top_k] / weights[T, top_k]: the top_k largest of each row of logits [T, E] (fp32, fp16 or bf16, rows
+ * stride_t elements apart), largest first, ties to the lower expert; NaN and -inf are never chosen (id -1, weight 0).
+ * weights: softmax or sigmoid in fp32, divided by their sum over the chosen ones if `renormalize`, times `scale`.
+ * Then the plan of these ids: offsets [E + 1], order [T * top_k], places [T * top_k].  top_k <= 64.
+ * workspace: gla_route_workspace_bytes(T, E) bytes, 16-byte aligned, contents arbitrary. */
+int64_t gla_route_workspace_bytes(int T, int E);
+int gla_route_experts(const void* logits, int dtype, int64_t stride_t, int T, int E, int top_k, int scoring, int renormalize, float scale,
+                      float* weights, int32_t* ids, int32_t* offsets, int32_t* order, int32_t* places, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+/* The plan alone, of ids [T, top_k] that another router chose. */
+int gla_plan_experts(const int32_t* ids, int T, int E, int top_k, int32_t* offsets, int32_t* order, int32_t* places, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
+/* What gla_experts_matmul computes, with W[e] = dequant(weights of expert e) [K, N] and e(r) the expert of sorted row r:
+ *   ROWS      out[r, :]   = x[r, :] W[e(r)] (+ bias[e(r)])                              out [R, N]
+ *   GATED     y[r, :]     = x[order[r] / top_k, :] W[e(r)] (+ bias[e(r)]), out[r, :] = silu(y[r, : N / 2]) * y[r, N / 2 :]
+ *                                                                                       out [R, N / 2]
+ *   COMBINED  out[t, :]   = sum over slots j of weights[t, j] * (x[places[t, j], :] W[e] (+ bias[e]))   out [T, N]
+ * With fp8 experts every row of x is quantised per 128 values, s = max(amax * fp32(1/448), 1e-6), code = e4m3(x * (1/s)),
+ * by the call itself.
+ * Rows without an expert are zeros in ROWS and GATED and add nothing in COMBINED.  Sums and the combination are fp32,
+ * rounded once to the output type, and do not depend on the order of execution. */
+#define GLA_EXPERTS_ROWS 0
+#define GLA_EXPERTS_GATED 1
+#define GLA_EXPERTS_COMBINED 2
+
+typedef struct gla_experts_args {
+    uint32_t struct_size; /* sizeof(gla_experts_args) */
+    int32_t mode;         /* GLA_EXPERTS_* */
+
+    const void* x;         /* ROWS, COMBINED: [R, K] sorted by expert; GATED: [T, K].  fp16 / bf16 */
+    const void* w;         /* [E] experts, w_stride_e bytes apart, each laid out as gla_matmul takes it: packed words
+                              [K/8, N], or K-contiguous bytes / 16-bit values [N, K] */
+    const void* scales;    /* 4-bit: [E][K/group_size, N] fp16 / bf16; fp8: [E][K/128, ceil(N/128)] fp32; 16-bit: NULL */
+    const void* zeros;     /* 4-bit: as scales (group modes 3 and 4), else NULL */
+    const float* bias;     /* [E, N] or NULL */
+    void* out;
+    void* workspace;       /* gla_experts_workspace_bytes() bytes, 16-byte aligned, contents arbitrary */
+    uint64_t workspace_bytes;
+
+    const int32_t* offsets;
+    const int32_t* order;  /* GATED */
+    const int32_t* places; /* COMBINED */
+    const float* weights;  /* COMBINED */
+
+    int64_t w_stride_e;    /* bytes */
+    int64_t meta_stride_e; /* bytes, of scales and of zeros */
+    int64_t x_stride_m;    /* elements; rows are 16-byte aligned */
+    int64_t out_stride_m;  /* elements; rows are 8-byte aligned */
+
+    int32_t R, T, top_k;   /* ROWS: T and top_k are not read */
+    int32_t E, N, K;       /* K a multiple of 32 (fp8: 128), N of 8 (GATED: 16); an expert's weights below 2^31 bytes */
+    int32_t W_nbits, group_size, elements_per_sample;
+    int32_t input_dtype, output_dtype, meta_dtype; /* input_dtype FP8: x is quantised first, see below */
+    int32_t x_dtype;       /* of x, fp16 or bf16: the output type */
+    int32_t channel_scale_mode, W_group_mode;
+    int32_t tile_config;   /* -1: the library chooses; else rows per tile (16, 32: streaming kernel; 64, 128, 256: tiled
+                              GEMM) + 1000 * K splits (0: the library's number; streaming kernel only) */
+} gla_experts_args;
+
+int64_t gla_experts_workspace_bytes(const gla_experts_args* args);
+int gla_experts_matmul(const gla_experts_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,304 @@
+"""Mixture-of-experts operators on the GPU against plain 64-bit computations of the same definitions.
+
+Tolerances.  u = eps / 2 of the output type is the largest relative error of the one final rounding.  Around it an
+element may be off by what the sum itself loses:
+  * fp32 accumulation of K products: at most K 2^-24 of the sum of their magnitudes.  4-bit codes may enter the matrix
+    unit with an offset of 128 (bf16) or 1024 (fp16) that is taken off again, so the magnitudes count with
+    (offset + 15) * scale + |zero|;
+  * 4-bit weights that are rounded to the activation type in front of the matrix unit: u of the sum of |x w|.
+The gated output multiplies two such sums: |d(silu(g) u)| <= 1.1 |u| dg + |silu(g)| du + 1.1 dg du (the slope of silu is below 1.1).
+Independent errors hardly ever add up to these bounds, so the whole output's 2-norm error has to stay below u as well:
+the roundings (one of the result and, in the worst case, one of every weight) are uniform, with a root mean square of
+u / sqrt(3) or less each, so 2-norm errors of 0.58 u for the result, 0.82 u with the weights' and 1.05 u for the gated product of
+two such sums: bounds of u, and 1.5 u for gated 4-bit experts."""
+import numpy as np
+import pytest
+import torch
+
+import gemlite_amd
+from gemlite_amd import DType, ExpertPlan, GemLiteExperts, GemLiteLinear, GemLiteMoE
+from gemlite_amd.helper import A16W4_HQQ_INT, A8W8_fp8_dynamic
+
+pytestmark = pytest.mark.gpu
+
+DT = {"bf16": (torch.bfloat16, DType.BF16), "fp16": (torch.float16, DType.FP16)}
+
+
+def _gen(seed):
+    return torch.Generator(device="cpu").manual_seed(seed)
+
+
+def make_layers(fmt, dtype, E, K, N, gs=64, seed=0, bias=False, device="cuda"):
+    """E packed layers of one kind and their dequantised weights [E, K, N] in float64 (on the CPU)."""
+    g = _gen(seed)
+    dt, gdt = DT[dtype]
+    layers, weights = [], []
+    for _ in range(E):
+        b = (torch.randn(N, generator=g)).to(dt) if bias else None
+        if fmt == "w4":
+            q = torch.randint(0, 16, (N, K), generator=g, dtype=torch.int32).to(torch.uint8)
+            s = ((0.5 + torch.rand((N * K // gs, 1), generator=g)) / (4.6 * K ** 0.5)).to(dt)
+            z = (torch.rand((N * K // gs, 1), generator=g) * 3 + 6).to(dt)
+            layer = A16W4_HQQ_INT(device=device, dtype=dt).from_weights(q.to(device), s.to(device), z.to(device), bias=b)
+            sc, zp = layer.scales.data.cpu().double(), layer.zeros.data.cpu().double()    # [K / gs, N], fma form
+            q = q.t().double().view(K // gs, gs, N)
+            if layer.channel_scale_mode == 1:   # one group for the whole of K: (q - z) s
+                w = (q - zp[:, None, :]) * sc[:, None, :]
+            else:
+                w = q * sc[:, None, :] + zp[:, None, :]
+            weights.append(w.reshape(K, N))
+        elif fmt == "fp8":
+            w = torch.randn((N, K), generator=g) / K ** 0.5
+            layer = A8W8_fp8_dynamic(device=device, dtype=dt, block_quant=True)
+            layer.fp8 = torch.float8_e4m3fn
+            layer = layer.from_weights(w.to(device), bias=b)
+            sc = layer.scales.data.cpu().double()
+            full = sc.repeat_interleave(128, 0)[:K].repeat_interleave(128, 1)[:, :N]
+            weights.append(layer.W_q.data.cpu().float().double() * full)
+        else:
+            w = (torch.randn((N, K), generator=g) / K ** 0.5).to(dt)
+            layer = GemLiteLinear(16, None, K, N, gdt, gdt).pack(w.to(device), None, None, b.to(device) if bias else None)
+            weights.append(w.t().double())
+        layers.append(layer)
+    return layers, torch.stack(weights)
+
+
+def make_x(rows, K, dtype, seed=1):
+    return torch.randn((rows, K), generator=_gen(seed)).to(DT[dtype][0])
+
+
+def make_ids(T, E, k, seed=2, drop=0.0, only=None):
+    g = _gen(seed)
+    score = torch.rand((T, E), generator=g)
+    if only is not None:
+        score[:, only] += 10.0
+    ids = torch.argsort(score, dim=1, descending=True)[:, :k].to(torch.int32)
+    if drop:
+        ids[torch.rand((T, k), generator=g) < drop] = -1
+    return ids, torch.rand((T, k), generator=g) + 0.1
+
+
+def ref_plan(ids, E):
+    flat = ids.reshape(-1).long()
+    key = torch.where((flat < 0) | (flat >= E), torch.full_like(flat, E), flat)
+    order = torch.sort(key, stable=True).indices
+    places = torch.empty_like(order)
+    places[order] = torch.arange(order.numel())
+    offsets = torch.tensor([0] + [int((key == e).sum()) for e in range(E)]).cumsum(0)
+    return offsets, order, places.view(ids.shape)
+
+
+def quantised(x):
+    """Rows as fp8 codes with a scale per 128 values, by the definition's fp32 steps; as float64."""
+    b = x.float().view(x.shape[0], -1, 128)
+    s = (b.abs().amax(2, keepdim=True) * torch.tensor(1 / 448, dtype=torch.float32)).clamp_min(1e-6)
+    q = (b * (1.0 / s)).clamp(-448, 448).to(torch.float8_e4m3fn)
+    return (q.float().double() * s.double()).view(x.shape)
+
+
+def ref_rows(fmt, x, W, offsets, bias=None):
+    """[R, N] products of rows sorted by expert and the sums of their magnitudes, in float64 (zeros without an expert)."""
+    R, (E, K, N) = x.shape[0], W.shape
+    xd = quantised(x) if fmt == "fp8" and R else x.double()
+    y, mag = torch.zeros(R, N, dtype=torch.float64), torch.zeros(R, N, dtype=torch.float64)
+    for e in range(E):
+        lo, hi = int(offsets[e]), int(offsets[e + 1])
+        y[lo:hi] = xd[lo:hi] @ W[e]
+        mag[lo:hi] = xd[lo:hi].abs() @ W[e].abs()
+        if bias is not None:
+            y[lo:hi] += bias[e]
+    return y, mag
+
+
+def sum_slack(fmt, dtype, x, layers, mag, u):
+    """How far an fp32 sum may be from the exact one (see the module's comment); per element or broadcast."""
+    K = x.shape[1]
+    slack = K * 2.0 ** -24 * mag
+    if fmt == "w4":
+        s = max(float(layer.scales.data.abs().max()) for layer in layers)
+        z = max(float(layer.zeros.data.abs().max()) for layer in layers) * (s if layers[0].channel_scale_mode == 1 else 1.0)
+        off = 128 if dtype == "bf16" else 1024
+        slack = u * mag + K * 2.0 ** -24 * x.double().abs().sum(1, keepdim=True) * ((off + 15) * s + z)
+    return slack
+
+
+def silu(v):
+    return v / (1 + torch.exp(-v))
+
+
+def check(y, ref, slack, u, norm):
+    y = y.cpu().double()
+    assert y.shape == ref.shape
+    err = (y - ref).abs()
+    bound = u * ref.abs() + (1 + u) * slack + 1e-30
+    worst = float((err / bound).max()) if err.numel() else 0.0
+    assert worst <= 1.0, f"element off by {worst} of its bound"
+    total = float(ref.norm())
+    if total > 0:
+        assert float(err.norm()) / total <= norm, f"norm error {float(err.norm()) / total} of {norm}"
+
+
+def run_case(fmt, dtype, E, T, k, K, N, gs=64, drop=0.0, only=None, bias=False, tile_config=-1, seed=0, modes=("rows", "gated", "combined")):
+    layers, W = make_layers(fmt, dtype, E, K, N, gs, seed, bias)
+    experts = GemLiteExperts.from_layers(layers)
+    B = None if not bias else torch.stack([layer.bias.data.cpu().double() for layer in layers])
+    u = torch.finfo(DT[dtype][0]).eps / 2
+    ids, w = make_ids(T, E, k, seed + 2, drop, only)
+    offsets, order, places = ref_plan(ids, E)
+    plan = gemlite_amd.plan_experts(ids.cuda(), w.cuda(), E)
+    assert torch.equal(plan.offsets.cpu().long(), offsets) and torch.equal(plan.order.cpu().long(), order)
+    assert torch.equal(plan.places.cpu().long(), places)
+    x = make_x(T, K, dtype, seed + 1)
+    targs, meta = experts.get_tensor_args(), experts.get_meta_args()
+    xs = x[order // k]
+    y, mag = ref_rows(fmt, xs, W, offsets, B)
+    slack = sum_slack(fmt, dtype, xs, layers, mag, u)
+    if "rows" in modes:
+        out = gemlite_amd.experts_functional(xs.cuda(), experts.bias, targs, meta, plan.offsets, tile_config=tile_config)
+        check(out, y, slack, u, u)
+        assert not out[int(offsets[E]):].any()
+    if "gated" in modes:
+        out = gemlite_amd.experts_gated_functional(x.cuda(), experts.bias, targs, meta, plan, tile_config=tile_config)
+        g, up, half = y[:, : N // 2], y[:, N // 2:], slack.expand(y.shape)
+        dg, du = half[:, : N // 2], half[:, N // 2:]
+        # (and the fp32 arithmetic of silu: a handful of roundings of 2^-24, the exponential's argument up to 2^-18)
+        s = 1.1 * up.abs() * dg + silu(g).abs() * du + 1.1 * dg * du + 2.0 ** -16 * (silu(g) * up).abs()
+        check(out, silu(g) * up, s, u, 1.5 * u if fmt == "w4" else u)
+        assert not out[int(offsets[E]):].any()
+    if "combined" in modes:
+        out = gemlite_amd.experts_combined_functional(xs.cuda(), experts.bias, targs, meta, plan, tile_config=tile_config)
+        live = (ids >= 0).double() * w.double()
+        take = lambda t: (t.expand(y.shape)[places.reshape(-1)].view(T, k, -1) * live[:, :, None])   # noqa: E731
+        ref = take(y).sum(1)
+        check(out, ref, take(slack).sum(1) + (k + 1) * 2.0 ** -24 * take(y.abs()).sum(1), u, u)
+    return experts
+
+
+# ---------------------------------------------------------------------------
+# routing
+# ---------------------------------------------------------------------------
+def ref_route(logits, k, scoring, renormalize, scale):
+    x = logits.double().clone()
+    T, E = x.shape
+    x[torch.isnan(x)] = float("-inf")
+    order = torch.sort(x, dim=1, descending=True, stable=True)
+    best, ids = order.values[:, :k], order.indices[:, :k].clone()
+    none = best == float("-inf")
+    if scoring == "sigmoid":
+        p = 1 / (1 + torch.exp(-best))
+        total = p.masked_fill(none, 0).sum(1, keepdim=True)
+    else:
+        top = best[:, :1]
+        e = torch.where(best == top, torch.ones_like(best), torch.exp(best - top)).masked_fill(none, 0)
+        every = torch.where(x == top, torch.ones_like(x), torch.exp(x - top)).masked_fill(x == float("-inf"), 0)
+        p, total = e, (e if renormalize else every).sum(1, keepdim=True)
+    p = p.masked_fill(none, 0)
+    if renormalize or scoring == "softmax":
+        p = torch.where(total > 0, p / total, torch.zeros_like(p))
+    return p * scale, ids.masked_fill(none, -1)
+
+
+@pytest.mark.parametrize("T,E,k", [(1, 8, 2), (1, 1, 1), (3, 60, 6), (64, 64, 8), (128, 128, 8), (129, 128, 8), (1024, 1, 1), (1025, 2, 1),
+                                    (17, 1024, 64), (500, 256, 8), (2000, 160, 6), (4097, 100, 3), (9001, 128, 8), (40000, 8, 2)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_route(T, E, k, dtype):
+    g = _gen(T + E)
+    logits = (2 * torch.randn((T, E), generator=g)).to(dtype)   # 16-bit logits: many ties
+    logits[torch.rand((T, E), generator=g) < 0.1] = float("-inf")
+    for scoring, renormalize, scale in (("softmax", True, 1.0), ("softmax", False, 2.5), ("sigmoid", True, 1.0), ("sigmoid", False, 1.0)):
+        plan = gemlite_amd.route_experts(logits.cuda(), k, scoring, renormalize, scale)
+        w, ids = ref_route(logits, k, scoring, renormalize, scale)
+        assert torch.equal(plan.expert_ids.cpu().long(), ids)
+        # exp of a difference below 32 (2^-19 off), a sum of up to E of them, one division
+        np.testing.assert_allclose(plan.weights.cpu().double().numpy(), w.numpy(), rtol=2.0 ** -18 + E * 2.0 ** -24, atol=1e-37)
+        offsets, order, places = ref_plan(ids, E)
+        assert torch.equal(plan.offsets.cpu().long(), offsets)
+        assert torch.equal(plan.order.cpu().long(), order)
+        assert torch.equal(plan.places.cpu().long(), places)
+
+
+def test_route_special_values():
+    inf, nan = float("inf"), float("nan")
+    logits = torch.tensor([[nan, 1.0, -inf, 1.0], [-inf] * 4, [nan] * 4, [inf, 0.0, inf, 5.0], [0.0, -0.0, 0.0, -0.0],
+                           [-3e38, 3e38, -3e38, 1.0], [-inf, -inf, 2.0, -inf]])
+    for scoring in ("softmax", "sigmoid"):
+        for renormalize in (True, False):
+            plan = gemlite_amd.route_experts(logits.cuda(), 3, scoring, renormalize)
+            w, ids = ref_route(logits, 3, scoring, renormalize, 1.0)
+            assert torch.equal(plan.expert_ids.cpu().long(), ids)
+            np.testing.assert_allclose(plan.weights.cpu().double().numpy(), w.numpy(), rtol=1e-6, atol=1e-37)
+
+
+def test_route_strided_logits_and_no_tokens():
+    wide = torch.randn((50, 40), generator=_gen(3))
+    for view in (wide[:, 3:19], wide[::2, :16], wide.t()[:16].t(), wide[:, :16].t().contiguous().t()):
+        plan = gemlite_amd.route_experts(view.cuda() if view.is_contiguous() else view.cuda(), 2)
+        assert torch.equal(plan.expert_ids.cpu().long(), ref_route(view, 2, "softmax", True, 1.0)[1])
+    on_gpu = wide.cuda()
+    for view, cpu in ((on_gpu[:, 3:19], wide[:, 3:19]), (on_gpu[::2, :16], wide[::2, :16]), (on_gpu.t()[:16].t(), wide[:, :16])):
+        assert torch.equal(gemlite_amd.route_experts(view, 2).expert_ids.cpu().long(), ref_route(cpu, 2, "softmax", True, 1.0)[1])
+    plan = gemlite_amd.route_experts(torch.empty((0, 16), device="cuda"), 2)
+    assert plan.weights.shape == (0, 2) and plan.order.shape == (0,) and not plan.offsets.any() and plan.offsets.shape == (17,)
+
+
+@pytest.mark.parametrize("T,k", [(5, 2), (700, 4)])
+def test_plan_of_foreign_ids(T, k):
+    """Ids of another rank's experts, repeated ids and ids that 32 bits cannot hold."""
+    g = _gen(T)
+    ids = torch.randint(-3, 12, (T, k), generator=g)
+    ids[0, 0], ids[T - 1, k - 1], ids[T // 2, 0] = 2 ** 40, -2 ** 40, 2 ** 32 + 1
+    plan = gemlite_amd.plan_experts(ids.cuda(), torch.ones((T, k), device="cuda"), 8)
+    offsets, order, places = ref_plan(ids, 8)
+    assert torch.equal(plan.offsets.cpu().long(), offsets) and torch.equal(plan.order.cpu().long(), order)
+    assert torch.equal(plan.places.cpu().long(), places)
+
+
+# ---------------------------------------------------------------------------
+# products
+# ---------------------------------------------------------------------------
+FORMATS = ["w4", "fp8", "h16"]
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("E,T,k,K,N,gs", [(4, 1, 2, 256, 64, 64), (8, 5, 3, 384, 208, 128), (3, 70, 2, 640, 144, 32), (130, 40, 4, 128, 32, 64),
+                                          (16, 300, 4, 256, 272, 128), (2, 600, 1, 512, 96, 64), (1, 33, 1, 1152, 112, 64)])
+def test_products(fmt, dtype, E, T, k, K, N, gs):
+    run_case(fmt, dtype, E, T, k, K, N, gs, drop=0.1 if T > 4 else 0.0)
+
+
+@pytest.mark.parametrize("fmt", ["w4", "h16"])
+@pytest.mark.parametrize("K,gs", [(32, 32), (96, 32), (160, 32), (192, 192), (320, 64), (480, 96), (416, 416)])
+def test_ragged_k(fmt, K, gs):
+    """K that ends inside a pipeline stage, groups that are no power of two, one group for the whole of K."""
+    for T, k in ((2, 1), (90, 2)):
+        run_case(fmt, "bf16", 3, T, k, K, 80, gs)
+        run_case(fmt, "fp16", 3, T, k, K, 80, gs)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_one_expert_gets_everything(fmt):
+    run_case(fmt, "bf16", 6, 150, 1, 256, 96, only=4)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_no_slot_has_an_expert(fmt):
+    run_case(fmt, "bf16", 6, 20, 2, 256, 96, drop=2.0)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_bias(fmt, dtype):
+    for T in (3, 200):
+        run_case(fmt, dtype, 4, T, 2, 256, 160, drop=0.2, bias=True)
+
+
+TILES = [16, 32, 2016, 3032]
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("tile_config", TILES)
+def test_every_kernel_variant(fmt, dtype, tile_config):
+    for T, K, N, gs in ((1, 512, 144, 128), (77, 1024, 272, 64), (330, 384, 528, 32)):
+        run_case(fmt, dtype, 5, T, 2, K, N, gs, drop=0.05, tile_config=tile_config, bias=T == 77)
