@@ -104,7 +104,7 @@ int validate(const gla_experts_args* p) {
     }
     if (p->tile_config != -1) {
         const int rows = p->tile_config % 1000, splits = p->tile_config / 1000;
-        if (p->tile_config < 0 || splits > 64 || (rows != 16 && rows != 32)) {
+        if (p->tile_config < 0 || splits > 64 || (rows != 16 && rows != 32 && rows != 64 && rows != 128 && rows != 256) || (rows > 32 && splits > 1)) {
             set_error("experts: tile_config %d", p->tile_config);
             return GLA_ERR_INVALID_ARGUMENT;
         }
@@ -187,6 +187,7 @@ ExpertPlanHost plan_of(const gla_experts_args& p) {
     const int want_rows = p.tile_config < 0 ? 0 : p.tile_config % 1000, want_s = p.tile_config < 0 ? 0 : p.tile_config / 1000;
     const int active = p.R < p.E ? p.R : p.E;
     const int per = active > 0 ? p.R / active : 0;
+    if (want_rows ? want_rows > 32 : per > 24) h.bm = want_rows ? want_rows : (per > 160 ? 256 : (per > 64 ? 128 : 64));
     h.row_tiles = want_rows == 16 ? 1 : (want_rows == 32 || per > 8 ? 2 : 1);
     h.S = want_s > 0 ? want_s : 1;
     h.to_partials = p.mode == GLA_EXPERTS_COMBINED || h.S > 1;
@@ -259,7 +260,7 @@ int gla_experts_matmul(const gla_experts_args* p, void* stream) {
         a.xsm = p->K;
         a.scales_x = scales_x;
     }
-    const int rc2 = launch_experts_stream(a, h.format, bf16, h.row_tiles, s);
+    const int rc2 = h.bm > 0 ? launch_experts_gemm(a, h.format, bf16, h.bm, s) : launch_experts_stream(a, h.format, bf16, h.row_tiles, s);
     if (rc2 != GLA_OK || !h.to_partials) return rc2;
     const bool combined = p->mode == GLA_EXPERTS_COMBINED;
     FinishArgs f{a.partials, p->offsets, p->places, p->weights, p->out, p->out_stride_m, p->R, p->E, p->N, h.S, p->top_k, a.half};

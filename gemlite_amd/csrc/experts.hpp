@@ -62,12 +62,13 @@ struct ExpertTile {
     int total;    // row tiles in all
 };
 
-// Row tile t of the call, computed by every wave for itself: lane l counts the tiles of experts l C .. l C + C - 1
-// (C = 1 up to 63 experts), an inclusive sum over the lanes finds the lane, that lane the expert.  Offsets are clamped
-// to 0 .. R and to rising order, so no tile leaves the R rows whatever they hold.  One round trip to memory and about a
-// hundred vector instructions; a table written by the routing kernel would cost the same round trip.
-template <int BM>
-__device__ __forceinline__ ExpertTile find_tile(const int32_t* offsets, int E, int R, int t, bool with_rest) {
+// The row tile `pick(total)` of the call's `total` ones, computed by every wave for itself: lane l counts the tiles of
+// experts l C .. l C + C - 1 (C = 1 up to 63 experts), an inclusive sum over the lanes finds the lane, that lane the
+// expert.  Offsets are clamped to 0 .. R and to rising order, so no tile leaves the R rows whatever they hold.  One round
+// trip to memory and about a hundred vector instructions; a table written by the routing kernel would cost the same round
+// trip.
+template <int BM, typename Pick>
+__device__ __forceinline__ ExpertTile find_tile(const int32_t* offsets, int E, int R, bool with_rest, Pick pick) {
     const int lane = threadIdx.x & 63;
     const int C = (E + 1 + 63) / 64;
     auto at = [&](int e) __attribute__((always_inline)) {
@@ -90,7 +91,8 @@ __device__ __forceinline__ ExpertTile find_tile(const int32_t* offsets, int E, i
     const int upto = wave_inclusive_sum(mine);
     ExpertTile r;
     r.total = __builtin_amdgcn_readlane(upto, 63);
-    if (t >= r.total) {
+    const int t = pick(r.total);
+    if (t < 0 || t >= r.total) {
         r.expert = -1;
         r.row0 = r.row_end = 0;
         return r;
@@ -102,7 +104,7 @@ __device__ __forceinline__ ExpertTile find_tile(const int32_t* offsets, int E, i
         const int e = lane * C + c;
         const int hi = at(e + 1);
         const int n = tiles_of(e, lo, hi);
-        if (found < 0 && left < n) {
+        if (found < 0 && left >= 0 && left < n) {
             found = e;
             row0 = lo + left * BM;
             row_end = hi;
@@ -125,11 +127,20 @@ __device__ __forceinline__ int64_t source_row(const ExpertArgs& a, int r) {
     return v / a.top_k;
 }
 
-// Column of the weights that column c of a 64-column tile stands for: the tile's own, or (gated) 32 gate columns followed
-// by the same 32 up columns.
-__device__ __forceinline__ int tile_column(int half, int tile, int c) {
-    if (half == 0) return tile * 64 + c;
-    return tile * 32 + (c & 31) + (c < 32 ? 0 : half);
+// Column of the weights that column c of the W columns of unit u stands for: u W + c, or (gated) W / 2 gate columns
+// followed by the same up columns, so that whoever computes the unit holds both factors of an output.
+template <int W>
+__device__ __forceinline__ int unit_column(int half, int u, int c) {
+    if (half == 0) return u * W + c;
+    return u * (W / 2) + (c % (W / 2)) + (c < W / 2 ? 0 : half);
+}
+// The same for a run of 4 columns that starts at c, moved back inside its half where it would begin past the end (N and
+// half are multiples of 8).
+template <int W>
+__device__ __forceinline__ int unit_column_inside(int half, int N, int u, int c) {
+    const int in = half == 0 ? u * W + c : u * (W / 2) + (c % (W / 2));
+    const int top = (half == 0 ? N : half) - 4;
+    return (in > top + 3 ? top : in) + (half != 0 && c >= W / 2 ? half : 0);
 }
 
 __device__ __forceinline__ float silu_mul(float gate, float up) { return gate / (1.0f + __expf(-gate)) * up; }

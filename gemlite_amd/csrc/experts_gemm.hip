@@ -1,0 +1,481 @@
+// Products grouped by expert, many rows per expert: a tiled MFMA GEMM over ragged row blocks.
+//
+//  * Workgroup tile BM rows of one expert x 256 columns, 8 waves; pipeline stage of 128 bytes of K per activation row (64
+//    16-bit values or 128 e4m3 codes).  Operand tiles, scales and zeros are copied global -> LDS by the load unit
+//    (global_load_lds) into a ring of stages, all of them in flight; gated calls gather their activation rows on the
+//    way.  16-byte chunk c of a 128-byte row r lies at position c ^ ((r >> 1) & 7), chosen on the global side of the copy,
+//    so that the 16 lanes of an LDS read phase hit 16 different bank groups.
+//  * The weights are the row operand of every MFMA: a lane holds 4 adjacent output columns of one row.
+//  * 16-bit weights and W4: v_mfma_f32_32x32x16, four K-steps per stage, fragments of a K-step read during the one in
+//    front of it.  The barrier of a stage stands before its last K-step, whose fragments are in registers by then: the
+//    matrix pipe has work while the waves meet and the first fragments of the next stage arrive.
+//  * W4: the packed words lie in LDS as they are in memory (a word = 8 K-values of a column = a lane's share of a
+//    K-step's operand) and are dequantised into the operand registers between the MFMAs, w = s q + z in fp32 for bf16,
+//    in packed fp16 for fp16, rounded once to the activation type.
+//  * F8: v_mfma_f32_16x16x128 starts from zero on every 128-block and its result joins the fp32 sum times the block's two
+//    scales.
+//  * A workgroup's tile is found from the offsets on the device; the tiles that exist are dealt to the 8 XCDs in
+//    contiguous bands, and a band is walked in groups of 1024 rows x all columns, so that the L2 of an XCD keeps a
+//    weight panel for all row tiles of the group.
+#include <type_traits>
+
+#include "common.hpp"
+#include "experts.hpp"
+#include "wn_dequant.hpp"
+
+namespace gla {
+
+namespace {
+
+__device__ __align__(16) unsigned char g_zero_chunk[16];  // what activations past the end of K are read from
+
+constexpr int kBN = 256;
+
+template <int N>
+__device__ __forceinline__ void wait_vmcnt_e() {
+    static_assert(N >= 0 && N < 64, "vmcnt is a 6-bit counter");
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+}
+
+__device__ __forceinline__ void bare_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+template <int FMT, int BM>
+struct GemmShape {
+    static constexpr int WN = FMT == kEW4 && BM <= 128 ? 8 : 4;  // wave columns (W4: no weight dequantised twice, if LDS allows)
+    static constexpr int WMW = 8 / WN;                            // wave rows
+    static constexpr int WM = BM / WMW, WC = kBN / WN;            // wave tile
+    static constexpr int A_BYTES = BM * 128;
+    static constexpr int B_BYTES = FMT == kEW4 ? 8 * 1024 : kBN * 128;
+    static constexpr int M_BYTES = FMT == kEW4 ? 2048 : (FMT == kEF8 ? (BM + kBN) * 4 : 0);  // W4: [32-half][scale, zero][256]; F8: rows, columns
+    static constexpr int STAGE = A_BYTES + B_BYTES + M_BYTES;
+    static constexpr int RING = FMT == kEW4 ? (BM == 256 ? 3 : 4) : (BM == 256 ? 2 : 3);
+    static constexpr int A_JOBS = BM / 64;                        // copies per wave and stage
+    static constexpr int B_JOBS = FMT == kEW4 ? 1 : 4;
+    static constexpr int M_JOBS = FMT == kE16 ? 0 : 1;
+    static constexpr int LPS = A_JOBS + B_JOBS + M_JOBS;
+    static constexpr int LDS = RING * STAGE;
+};
+
+template <int FMT, bool BF16, int BM>
+__global__ __launch_bounds__(512) void experts_gemm_kernel(ExpertArgs a, int tiles_n) {
+    using SH = GemmShape<FMT, BM>;
+    constexpr int RING = SH::RING, LPS = SH::LPS, WC = SH::WC, WM = SH::WM;
+    constexpr bool F8 = FMT == kEF8, W4 = FMT == kEW4;
+    constexpr int MT = F8 ? 16 : 32;                   // MFMA tile edge
+    constexpr int TI = WM / MT, TJ = WC / MT;
+    constexpr int KS = F8 ? 128 : 64;                  // K-values per stage
+    constexpr int ES = F8 ? 1 : 2;                     // bytes per activation
+    constexpr int B_OFF = SH::A_BYTES, M_OFF = SH::A_BYTES + SH::B_BYTES;
+
+    extern __shared__ __align__(16) unsigned char smem[];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / SH::WN, wn = wave % SH::WN;
+
+    // ---- which tile
+    int ct = 0;
+    const ExpertTile tile = find_tile<BM>(a.offsets, a.E, a.R, !a.to_partials, [&](int total_m) {
+        const int total = total_m * tiles_n, pid = blockIdx.x;
+        if (pid >= total) return -1;
+        const int xcd = pid & 7, q = total >> 3, r = total & 7;
+        const int t = xcd * q + (xcd < r ? xcd : r) + (pid >> 3);
+        constexpr int GROUP = 1024 / BM;
+        const int width = GROUP * tiles_n, group = t / width, first = group * GROUP;
+        const int rows = total_m - first < GROUP ? total_m - first : GROUP;
+        ct = (t - group * width) / rows;
+        return first + (t - group * width) % rows;
+    });
+    if (tile.expert < 0) return;
+    const int expert = tile.expert;
+    const int width = a.half ? a.half : a.N;
+    if (expert >= a.E) {  // rows without an expert
+        const int c0 = a.half ? ct * (kBN / 2) : ct * kBN, cols = a.half ? kBN / 2 : kBN;
+        for (int i = tid; i < (tile.row_end - tile.row0) * (cols / 4); i += 512) {
+            const int r = tile.row0 + i / (cols / 4), c = c0 + (i % (cols / 4)) * 4;
+            if (c < width) *(u32x2*)((uint16_t*)a.out + (int64_t)r * a.osm + c) = u32x2{0, 0};
+        }
+        return;
+    }
+
+    // ---- copies
+    const int Kb = a.K * ES;                                     // bytes of an activation row
+    const int stages = (a.K + KS - 1) / KS;
+    const unsigned char* a_src[SH::A_JOBS];
+    int a_dst[SH::A_JOBS], a_chunk[SH::A_JOBS];
+    const float* sx_src = nullptr;
+#pragma unroll
+    for (int i = 0; i < SH::A_JOBS; ++i) {
+        const int row = (wave + 8 * i) * 8 + (lane >> 3);
+        int r = tile.row0 + row;
+        if (r > tile.row_end - 1) r = tile.row_end - 1;          // multiplied, never stored
+        a_chunk[i] = ((lane & 7) ^ ((row >> 1) & 7)) * 16;
+        a_src[i] = a.x + source_row(a, r) * a.xsm + a_chunk[i];
+        a_dst[i] = (wave + 8 * i) * 1024;
+    }
+    const unsigned char* we = a.w + (int64_t)expert * a.w_stride_e;
+    const unsigned char* se = a.scales + (int64_t)expert * a.meta_stride_e;
+    const unsigned char* ze = a.zeros == nullptr ? se : a.zeros + (int64_t)expert * a.meta_stride_e;
+    uint32_t b_off[SH::B_JOBS];
+    int b_chunk = 0;
+    if constexpr (W4) {
+        const int c = 4 * lane;                                  // of the tile: 4 columns per lane, word row `wave`
+        b_off[0] = ((uint32_t)unit_column_inside<WC>(a.half, a.N, ct * SH::WN + c / WC, c % WC) + (uint32_t)wave * (uint32_t)a.N) * 4u;
+    } else {
+#pragma unroll
+        for (int i = 0; i < SH::B_JOBS; ++i) {
+            const int c = (wave + 8 * i) * 8 + (lane >> 3);
+            b_chunk = ((lane & 7) ^ ((c >> 1) & 7)) * 16;        // the same for all i (c advances by 64)
+            b_off[i] = (uint32_t)unit_column_inside<WC>(a.half, a.N, ct * SH::WN + c / WC, c % WC) * (uint32_t)(a.K * ES);
+        }
+    }
+    // one 4-byte copy per wave and stage: W4: scales (even waves) / zeros (odd) of 128 columns and one 32-half of the
+    // stage; F8: the activation scales of 64 rows, or the block scale of each of 64 columns
+    uint32_t m_off = 0;
+    int m_dst = 0, m_half = 0;
+    const unsigned char* m_src = se;
+    if constexpr (W4) {
+        const int c = ((wave >> 1) & 1) * 128 + 2 * lane;
+        m_half = wave >> 2;
+        // (a pair lies inside the run of 4 it belongs to)
+        m_off = (uint32_t)(unit_column_inside<WC>(a.half, a.N, ct * SH::WN + (c & ~3) / WC, (c & ~3) % WC) + (c & 3)) * 2u;
+        m_src = wave & 1 ? ze : se;
+        m_dst = M_OFF + m_half * 1024 + (wave & 1) * 512 + ((wave >> 1) & 1) * 256;
+    } else if constexpr (F8) {
+        constexpr int JOBS = BM / 64 + 4;
+        const int q = wave < JOBS ? wave : JOBS - 1;
+        if (q < BM / 64) {
+            int r = tile.row0 + q * 64 + lane;
+            if (r > tile.row_end - 1) r = tile.row_end - 1;
+            sx_src = a.scales_x + source_row(a, r) * (a.K / 128);
+        } else {
+            const int c = (q - BM / 64) * 64 + lane;
+            m_off = (uint32_t)(unit_column_inside<WC>(a.half, a.N, ct * SH::WN + (c & ~3) / WC, (c & ~3) % WC) >> 7) * 4u;
+        }
+        m_dst = M_OFF + q * 256;
+    }
+    const int nblk = (a.N + 127) / 128;
+    const int groups = W4 ? a.K / a.group : 0;
+    typedef const __attribute__((address_space(1))) void* gptr;
+    typedef __attribute__((address_space(3))) void* lptr;
+    auto issue_one = [&](int k, int slot, int c) __attribute__((always_inline)) {
+        unsigned char* base = smem + slot * SH::STAGE;
+        if (c < SH::A_JOBS) {
+            const unsigned char* p = a_src[c] + (int64_t)k * 128;
+            if constexpr (!F8) p = k * 128 + a_chunk[c] < Kb ? p : (const unsigned char*)g_zero_chunk;
+            __builtin_amdgcn_global_load_lds((gptr)p, (lptr)(base + a_dst[c]), 16, 0, 0);
+        } else if (c < SH::A_JOBS + SH::B_JOBS) {
+            const int i = c - SH::A_JOBS;
+            if constexpr (W4) {
+                // word rows past the end of K: the stage's first ones again (they meet zeros)
+                const int row0 = k * 8 + wave < a.K / 8 ? k * 8 : k * 8 - 4;
+                __builtin_amdgcn_global_load_lds((gptr)(we + (int64_t)row0 * a.N * 4 + b_off[0]), (lptr)(base + B_OFF + wave * 1024), 16, 0, 0);
+            } else {
+                const uint32_t chunk = F8 || k * 128 + b_chunk < Kb ? (uint32_t)b_chunk : 0u;
+                __builtin_amdgcn_global_load_lds((gptr)(we + (int64_t)k * 128 + (b_off[i] + chunk)), (lptr)(base + B_OFF + (wave + 8 * i) * 1024), 16, 0, 0);
+            }
+        } else if constexpr (W4) {
+            int g = (k * 64 + m_half * 32) / a.group;
+            if (g > groups - 1) g = groups - 1;
+            __builtin_amdgcn_global_load_lds((gptr)(m_src + (int64_t)g * a.N * 2 + m_off), (lptr)(base + m_dst), 4, 0, 0);
+        } else if constexpr (F8) {
+            const unsigned char* p = sx_src != nullptr ? (const unsigned char*)(sx_src + k) : se + (int64_t)k * nblk * 4 + m_off;
+            __builtin_amdgcn_global_load_lds((gptr)p, (lptr)(base + m_dst), 4, 0, 0);
+        }
+    };
+
+    // ---- accumulators and fragment addresses
+    typedef typename std::conditional<F8, float4_t, float16_t>::type acc_t;
+    constexpr int AE = F8 ? 4 : 16;
+    acc_t acc[TI][TJ];
+#pragma unroll
+    for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int j = 0; j < TJ; ++j)
+#pragma unroll
+            for (int e = 0; e < AE; ++e) acc[i][j][e] = 0.0f;
+    const int fr = lane & (MT - 1), fk = lane / MT;  // row of a fragment, K part
+    const int swz = (fr >> 1) & 7;                   // (tile offsets are multiples of 16 rows)
+    const int a_row = (wm * WM + fr) * 128, b_row = B_OFF + (wn * WC + fr) * 128;
+
+    auto wait_stage = [&](int k) __attribute__((always_inline)) {
+        // the copies of stage k have landed (they are the oldest; up to RING - 2 younger stages may be in flight)
+        if (k + RING - 2 < stages) wait_vmcnt_e<(RING - 2) * LPS>();
+        else wait_vmcnt_e<0>();
+    };
+
+#pragma unroll
+    for (int u = 0; u < RING; ++u)
+        if (u < stages) {
+#pragma unroll
+            for (int c = 0; c < LPS; ++c) issue_one(u, u, c);
+        }
+    if (stages >= RING) wait_vmcnt_e<(RING - 1) * LPS>();
+    else wait_vmcnt_e<0>();
+    bare_barrier();
+
+    if constexpr (F8) {
+        typedef union {
+            int8_t_v v;
+            u32x4 c[2];
+        } op_t;
+        const int c0 = ((2 * fk) ^ swz) * 16, c1 = ((2 * fk + 1) ^ swz) * 16;
+        int slot = 0;
+#pragma unroll 1
+        for (int k = 0; k < stages; ++k) {
+            const unsigned char* base = smem + slot * SH::STAGE;
+            op_t fb[TJ];
+            float sw[TJ];
+#pragma unroll
+            for (int j = 0; j < TJ; ++j) {
+                fb[j].c[0] = *(const u32x4*)(base + b_row + j * 2048 + c0);
+                fb[j].c[1] = *(const u32x4*)(base + b_row + j * 2048 + c1);
+                sw[j] = *(const float*)(base + M_OFF + (BM + wn * WC + j * 16 + 4 * fk) * 4);
+            }
+            const float4_t zero4 = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < TI; ++i) {
+                op_t fa;
+                fa.c[0] = *(const u32x4*)(base + a_row + i * 2048 + c0);
+                fa.c[1] = *(const u32x4*)(base + a_row + i * 2048 + c1);
+                const float sx = *(const float*)(base + M_OFF + (wm * WM + i * 16 + fr) * 4);
+#pragma unroll
+                for (int j = 0; j < TJ; ++j) {
+                    const float4_t d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j].v, fa.v, zero4, 0, 0, 0, 127, 0, 127);
+                    const float sc = sx * sw[j];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(d[e], sc, acc[i][j][e]);
+                }
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            bare_barrier();  // everybody has read the slot
+            if (k + RING < stages) {
+#pragma unroll
+                for (int c = 0; c < LPS; ++c) issue_one(k + RING, slot, c);
+                wait_vmcnt_e<(RING - 1) * LPS>();
+            } else {
+                wait_vmcnt_e<0>();
+            }
+            bare_barrier();
+            slot = slot == RING - 1 ? 0 : slot + 1;
+        }
+    } else {
+        u32x4 fa[2][TI], fb[2][TJ];
+        auto read_a = [&](const unsigned char* base, int s, int buf, int i) __attribute__((always_inline)) {
+            fa[buf][i] = *(const u32x4*)(base + a_row + i * 32 * 128 + (((2 * s + fk) ^ swz) * 16));
+        };
+        auto read_b = [&](const unsigned char* base, int s, int buf, int j) __attribute__((always_inline)) {
+            fb[buf][j] = *(const u32x4*)(base + b_row + j * 32 * 128 + (((2 * s + fk) ^ swz) * 16));
+        };
+        auto mfma = [&](int i, int j, int buf, const u32x4& b) __attribute__((always_inline)) {
+            if constexpr (BF16)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, b), __builtin_bit_cast(bf16x8_t, fa[buf][i]), acc[i][j], 0, 0, 0);
+            else
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, b), __builtin_bit_cast(half8_t, fa[buf][i]), acc[i][j], 0, 0, 0);
+        };
+        // W4: words of the K-step at hand and the next one, constants of the stage's two 32-halves
+        uint32_t words[2][TJ];
+        ColMeta<BF16> meta[2][TJ];
+        uint32_t raw_s[2][TJ], raw_z[2][TJ];
+        auto read_words = [&](const unsigned char* base, int s, int buf) __attribute__((always_inline)) {
+#pragma unroll
+            for (int j = 0; j < TJ; ++j) words[buf][j] = *(const uint32_t*)(base + B_OFF + (2 * s + fk) * 1024 + (wn * WC + j * 32 + fr) * 4);
+        };
+        auto read_meta = [&](const unsigned char* base) __attribute__((always_inline)) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < TJ; ++j) {
+                    raw_s[h][j] = *(const uint16_t*)(base + M_OFF + h * 1024 + (wn * WC + j * 32 + fr) * 2);
+                    raw_z[h][j] = *(const uint16_t*)(base + M_OFF + h * 1024 + 512 + (wn * WC + j * 32 + fr) * 2);
+                }
+        };
+        auto convert_meta = [&](int h) __attribute__((always_inline)) {
+#pragma unroll
+            for (int j = 0; j < TJ; ++j) {
+                const float s = a.meta_bf16 ? bf16_bits_to_float((uint16_t)raw_s[h][j]) : half_bits_to_float((uint16_t)raw_s[h][j]);
+                float z = a.meta_bf16 ? bf16_bits_to_float((uint16_t)raw_z[h][j]) : half_bits_to_float((uint16_t)raw_z[h][j]);
+                z = a.zeros == nullptr ? 0.0f : z * __builtin_fmaf(a.c2, s, a.c1);
+                meta[h][j] = make_meta<BF16, 0>(s, z);
+            }
+        };
+        uint32_t nat_mask = 0x00F0000Fu, nat_magic = 0x54006400u;
+        asm volatile("" : "+s"(nat_mask), "+v"(nat_magic));
+        // register q (codes 2q, 2q + 1) of the operand of column set j
+        auto dequant = [&](uint32_t w, const ColMeta<BF16>& m, int q) __attribute__((always_inline)) -> uint32_t {
+            if constexpr (BF16) {
+                const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
+                return pack_bf16x2(__builtin_fmaf((float)((lo >> (8 * q)) & 0xffu), m.s, m.z), __builtin_fmaf((float)((hi >> (8 * q)) & 0xffu), m.s, m.z));
+            } else {
+                return dequant_pair<BF16>((__builtin_amdgcn_perm(w, w, 0x0c000c00u | (q << 16) | q) & nat_mask) | nat_magic, m, 1024.0f, 64.0f);
+            }
+        };
+
+        // ---- prologue: fragments of K-step 0
+        const unsigned char* base = smem;
+#pragma unroll
+        for (int i = 0; i < TI; ++i) read_a(base, 0, 0, i);
+        if constexpr (W4) {
+            read_meta(base);
+            read_words(base, 0, 0);
+            convert_meta(0);
+            convert_meta(1);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) fb[0][0][q] = dequant(words[0][0], meta[0][0], q);
+        } else {
+#pragma unroll
+            for (int j = 0; j < TJ; ++j) read_b(base, 0, 0, j);
+        }
+        int slot = 0;
+#pragma unroll 1
+        for (int k = 0; k < stages; ++k) {
+            const int next_slot = slot == RING - 1 ? 0 : slot + 1;
+            const unsigned char* next = smem + next_slot * SH::STAGE;
+            const bool refill = k + RING < stages;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const int cur = s & 1, nxt = cur ^ 1;
+                if (s == 3) {
+                    // the fragments of this K-step are in registers; the next stage's copies have landed, here and (behind the
+                    // barrier) everywhere, and nobody reads this stage's slot any more
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    if (k + 1 < stages) wait_stage(k + 1);
+                    bare_barrier();
+                    if (refill) {
+#pragma unroll
+                        for (int c = 0; c < LPS; ++c) issue_one(k + RING, slot, c);
+                    }
+                }
+                const unsigned char* from = s == 3 ? next : base;
+                const int s1 = (s + 1) & 3;
+                if constexpr (W4) {
+                    // MFMAs of column set 0 with the dequantisation of set 1, then set 1 with set 0 of the next K-step
+                    read_words(from, s1, nxt);
+                    if (s == 3) read_meta(next);
+#pragma unroll
+                    for (int j = 0; j < TJ; ++j) {
+#pragma unroll
+                        for (int i = 0; i < TI; ++i) {
+                            mfma(i, j, cur, fb[0][j]);
+                            if (j == 0) read_a(from, s1, nxt, i);
+                            if (j + 1 < TJ) {
+#pragma unroll
+                                for (int q = i * 4 / TI; q < (i + 1) * 4 / TI; ++q) fb[0][j + 1][q] = dequant(words[cur][j + 1], meta[s / 2][j + 1], q);
+                            } else if (TJ > 1) {
+                                if (i == 0 && s == 3) convert_meta(0);
+#pragma unroll
+                                for (int q = i * 4 / TI; q < (i + 1) * 4 / TI; ++q) fb[0][0][q] = dequant(words[nxt][0], meta[s == 3 ? 0 : s1 / 2][0], q);
+                            } else {
+                                // one column set: its registers for the next K-step are the other buffer
+                                if (i == 0 && s == 3) convert_meta(0);
+#pragma unroll
+                                for (int q = i * 4 / TI; q < (i + 1) * 4 / TI; ++q) fb[1][0][q] = dequant(words[nxt][0], meta[s == 3 ? 0 : s1 / 2][0], q);
+                            }
+                        }
+                    }
+                    if constexpr (TJ == 1) fb[0][0] = fb[1][0];
+                    if (s == 3) convert_meta(1);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < TJ; ++j) read_b(from, s1, nxt, j);
+#pragma unroll
+                    for (int i = 0; i < TI; ++i) {
+                        read_a(from, s1, nxt, i);
+#pragma unroll
+                        for (int j = 0; j < TJ; ++j) mfma(i, j, cur, fb[cur][j]);
+                    }
+                }
+            }
+            slot = next_slot;
+            base = next;
+        }
+    }
+
+    // ---- epilogue: the lane holds row fr of an MFMA tile and runs of 4 columns
+    constexpr int RUNS = AE / 4;
+    auto run_col = [&](int j, int g) __attribute__((always_inline)) { return F8 ? j * 16 + 4 * fk : j * 32 + 8 * g + 4 * fk; };  // of the wave tile
+    auto get = [&](int i, int j, int g) __attribute__((always_inline)) {
+        float4_t v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * g + e];
+        if (a.bias != nullptr) {
+            const float4_t b = *(const float4_t*)(a.bias + (int64_t)expert * a.N + unit_column_inside<WC>(a.half, a.N, ct * SH::WN + wn, run_col(j, g)));
+            v += b;
+        }
+        return v;
+    };
+    const bool pairs = a.half != 0 && !a.to_partials;
+#pragma unroll
+    for (int i = 0; i < TI; ++i) {
+        const int r = tile.row0 + wm * WM + i * MT + fr;
+        if (r >= tile.row_end) continue;
+#pragma unroll
+        for (int j = 0; j < TJ; ++j)
+#pragma unroll
+            for (int g = 0; g < RUNS; ++g) {
+                const int c = run_col(j, g);
+                const bool second = c >= WC / 2;
+                const int in = a.half ? (ct * SH::WN + wn) * (WC / 2) + (c % (WC / 2)) : (ct * SH::WN + wn) * WC + c;
+                if (in >= width) continue;
+                if (a.to_partials) {
+                    *(float4_t*)(a.partials + (int64_t)r * a.N + in + (a.half && second ? a.half : 0)) = get(i, j, g);
+                } else if (!pairs) {
+                    const float4_t v = get(i, j, g);
+                    *(u32x2*)((uint16_t*)a.out + (int64_t)r * a.osm + in) = u32x2{pack16<BF16>(v[0], v[1]), pack16<BF16>(v[2], v[3])};
+                } else if (!second) {
+                    // the up columns: WC / 2 further on, in the same lane
+                    constexpr int HALF = WC / 2;
+                    constexpr int DJ = F8 ? HALF / 16 : HALF / 32, DG = F8 || HALF >= 32 ? 0 : HALF / 8;
+                    const int j2 = j + DJ < TJ ? j + DJ : j, g2 = g + DG < RUNS ? g + DG : g;
+                    const float4_t v = get(i, j, g), up = get(i, j2, g2);
+                    float h[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) h[e] = silu_mul(v[e], up[e]);
+                    *(u32x2*)((uint16_t*)a.out + (int64_t)r * a.osm + in) = u32x2{pack16<BF16>(h[0], h[1]), pack16<BF16>(h[2], h[3])};
+                }
+            }
+    }
+}
+
+template <int FMT, bool BF16, int BM>
+int launch_one(const ExpertArgs& a, hipStream_t stream) {
+    using SH = GemmShape<FMT, BM>;
+    static_assert(SH::LDS <= 160 * 1024, "ring does not fit LDS");
+    const int cols = a.half ? kBN / 2 : kBN, width = a.half ? a.half : a.N;
+    const int tiles_n = (width + cols - 1) / cols;
+    const int64_t grid = max_row_tiles(a.R, a.E, BM) * tiles_n;
+    if (grid >= (int64_t)1 << 31) {
+        set_error("experts: %lld tiles exceed the grid", (long long)grid);
+        return GLA_ERR_INVALID_ARGUMENT;
+    }
+    const auto kernel = experts_gemm_kernel<FMT, BF16, BM>;
+    static DeviceOnce once;
+    if (once.first()) {
+        const int rc = check_hip(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, SH::LDS), "hipFuncSetAttribute");
+        if (rc != GLA_OK) return rc;
+    }
+    kernel<<<(unsigned)grid, 512, SH::LDS, stream>>>(a, tiles_n);
+    return check_hip(hipGetLastError(), "experts_gemm");
+}
+
+template <int FMT, bool BF16>
+int launch_bm(const ExpertArgs& a, int bm, hipStream_t stream) {
+    if (bm >= 256) return launch_one<FMT, BF16, 256>(a, stream);
+    if (bm >= 128) return launch_one<FMT, BF16, 128>(a, stream);
+    return launch_one<FMT, BF16, 64>(a, stream);
+}
+
+}  // namespace
+
+int launch_experts_gemm(const ExpertArgs& a, int format, bool bf16, int bm, hipStream_t stream) {
+    switch (format) {
+        case kEW4: return bf16 ? launch_bm<kEW4, true>(a, bm, stream) : launch_bm<kEW4, false>(a, bm, stream);
+        case kEF8: return bf16 ? launch_bm<kEF8, true>(a, bm, stream) : launch_bm<kEF8, false>(a, bm, stream);
+        default: return bf16 ? launch_bm<kE16, true>(a, bm, stream) : launch_bm<kE16, false>(a, bm, stream);
+    }
+}
+
+}  // namespace gla

@@ -59,7 +59,7 @@ __global__ __launch_bounds__(NW * 64) void experts_stream_kernel(ExpertArgs a) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int cg = lane & 15, kb = lane >> 4;
-    const ExpertTile tile = find_tile<16 * RT>(a.offsets, a.E, a.R, blockIdx.y, !a.to_partials);
+    const ExpertTile tile = find_tile<16 * RT>(a.offsets, a.E, a.R, !a.to_partials, [](int) { return (int)blockIdx.y; });
     if (tile.expert < 0) return;
     const int ct = blockIdx.x, split = blockIdx.z;
     extern __shared__ __align__(16) float red[];  // [NW][16 RT][64]
@@ -85,12 +85,7 @@ __global__ __launch_bounds__(NW * 64) void experts_stream_kernel(ExpertArgs a) {
         }
         uint32_t w_off[FMT == kEW4 ? 1 : NT];
         uint32_t m_off[NT];
-        auto column = [&](int c) __attribute__((always_inline)) {  // column c of the tile, kept inside its half
-            const int base = a.half ? ct * 32 + (c & 31) : ct * 64 + c;
-            const int top = (a.half ? a.half : a.N) - 4;           // a multiple of 4
-            const int in = base > top + 3 ? top : base;
-            return in + (a.half && c >= 32 ? a.half : 0);
-        };
+        auto column = [&](int c) __attribute__((always_inline)) { return unit_column_inside<64>(a.half, a.N, ct, c); };
         if constexpr (FMT == kEW4) {
             w_off[0] = (uint32_t)column(4 * cg) * 4u + (uint32_t)kb * (uint32_t)a.N * 4u;
             m_off[0] = (uint32_t)column(4 * cg) * 2u;
@@ -305,7 +300,7 @@ __global__ __launch_bounds__(NW * 64) void experts_stream_kernel(ExpertArgs a) {
 #pragma unroll
         for (int w = 0; w < NW; ++w) v += *(const float4_t*)(red + w * (16 * RT * 64) + row * 64 + c);
         if (a.bias != nullptr && split == 0) {
-            const float* b = a.bias + (int64_t)tile.expert * a.N + tile_column(a.half, ct, c);
+            const float* b = a.bias + (int64_t)tile.expert * a.N + unit_column<64>(a.half, ct, c);
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] += b[i];
         }
@@ -320,7 +315,7 @@ __global__ __launch_bounds__(NW * 64) void experts_stream_kernel(ExpertArgs a) {
         if (r >= tile.row_end || in_half >= width) continue;  // N (half) is a multiple of 8: whole vectors
         float4_t v = total(row, c);
         if (a.to_partials) {
-            *(float4_t*)(a.partials + ((int64_t)split * a.R + r) * a.N + tile_column(a.half, ct, c)) = v;
+            *(float4_t*)(a.partials + ((int64_t)split * a.R + r) * a.N + unit_column<64>(a.half, ct, c)) = v;
             continue;
         }
         if (pairs) {
