@@ -106,7 +106,6 @@ __global__ __launch_bounds__(512) void experts_gemm_kernel(ExpertArgs a, int til
     const int stages = (a.K + KS - 1) / KS;
     const unsigned char* a_src[SH::A_JOBS];
     int a_dst[SH::A_JOBS], a_chunk[SH::A_JOBS];
-    const float* sx_src = nullptr;
 #pragma unroll
     for (int i = 0; i < SH::A_JOBS; ++i) {
         const int row = (wave + 8 * i) * 8 + (lane >> 3);
@@ -135,7 +134,8 @@ __global__ __launch_bounds__(512) void experts_gemm_kernel(ExpertArgs a, int til
     // one 4-byte copy per wave and stage: W4: scales (even waves) / zeros (odd) of 128 columns and one 32-half of the
     // stage; F8: the activation scales of 64 rows, or the block scale of each of 64 columns
     uint32_t m_off = 0;
-    int m_dst = 0, m_half = 0;
+    int64_t m_row = 0;
+    int m_dst = 0, m_half = 0, m_step = (a.N + 127) / 128 * 4;
     const unsigned char* m_src = se;
     if constexpr (W4) {
         const int c = ((wave >> 1) & 1) * 128 + 2 * lane;
@@ -150,40 +150,51 @@ __global__ __launch_bounds__(512) void experts_gemm_kernel(ExpertArgs a, int til
         if (q < BM / 64) {
             int r = tile.row0 + q * 64 + lane;
             if (r > tile.row_end - 1) r = tile.row_end - 1;
-            sx_src = a.scales_x + source_row(a, r) * (a.K / 128);
+            m_row = source_row(a, r) * (a.K / 128) * 4;
+            m_src = (const unsigned char*)a.scales_x;
+            m_step = 4;
         } else {
             const int c = (q - BM / 64) * 64 + lane;
-            m_off = (uint32_t)(unit_column_inside<WC>(a.half, a.N, ct * SH::WN + (c & ~3) / WC, (c & ~3) % WC) >> 7) * 4u;
+            m_row = (unit_column_inside<WC>(a.half, a.N, ct * SH::WN + (c & ~3) / WC, (c & ~3) % WC) >> 7) * 4;
         }
         m_dst = M_OFF + q * 256;
     }
-    const int nblk = (a.N + 127) / 128;
     const int groups = W4 ? a.K / a.group : 0;
+    const unsigned char* zero_chunk = g_zero_chunk;
+    asm volatile("" : "+s"(zero_chunk));  // its address stays in registers
     typedef const __attribute__((address_space(1))) void* gptr;
     typedef __attribute__((address_space(3))) void* lptr;
+    // The weights' address of a stage is a wave-uniform base that advances per stage plus a 32-bit lane offset; the base
+    // is made opaque, or the compiler keeps one 64-bit address per copy in vector registers, which the accumulators need.
+    const unsigned char* b_base = we;
+    const int64_t b_step = W4 ? (int64_t)a.N * 32 : 128;
     auto issue_one = [&](int k, int slot, int c) __attribute__((always_inline)) {
         unsigned char* base = smem + slot * SH::STAGE;
         if (c < SH::A_JOBS) {
             const unsigned char* p = a_src[c] + (int64_t)k * 128;
-            if constexpr (!F8) p = k * 128 + a_chunk[c] < Kb ? p : (const unsigned char*)g_zero_chunk;
+            if constexpr (!F8) p = k * 128 + a_chunk[c] < Kb ? p : zero_chunk;
             __builtin_amdgcn_global_load_lds((gptr)p, (lptr)(base + a_dst[c]), 16, 0, 0);
         } else if (c < SH::A_JOBS + SH::B_JOBS) {
             const int i = c - SH::A_JOBS;
             if constexpr (W4) {
                 // word rows past the end of K: the stage's first ones again (they meet zeros)
-                const int row0 = k * 8 + wave < a.K / 8 ? k * 8 : k * 8 - 4;
-                __builtin_amdgcn_global_load_lds((gptr)(we + (int64_t)row0 * a.N * 4 + b_off[0]), (lptr)(base + B_OFF + wave * 1024), 16, 0, 0);
+                const int64_t back = k * 8 + wave < a.K / 8 ? 0 : (int64_t)a.N * 16;
+                __builtin_amdgcn_global_load_lds((gptr)(b_base - back + b_off[0]), (lptr)(base + B_OFF + wave * 1024), 16, 0, 0);
             } else {
                 const uint32_t chunk = F8 || k * 128 + b_chunk < Kb ? (uint32_t)b_chunk : 0u;
-                __builtin_amdgcn_global_load_lds((gptr)(we + (int64_t)k * 128 + (b_off[i] + chunk)), (lptr)(base + B_OFF + (wave + 8 * i) * 1024), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((gptr)(b_base + (b_off[i] + chunk)), (lptr)(base + B_OFF + (wave + 8 * i) * 1024), 16, 0, 0);
             }
         } else if constexpr (W4) {
             int g = (k * 64 + m_half * 32) / a.group;
             if (g > groups - 1) g = groups - 1;
             __builtin_amdgcn_global_load_lds((gptr)(m_src + (int64_t)g * a.N * 2 + m_off), (lptr)(base + m_dst), 4, 0, 0);
         } else if constexpr (F8) {
-            const unsigned char* p = sx_src != nullptr ? (const unsigned char*)(sx_src + k) : se + (int64_t)k * nblk * 4 + m_off;
+            const unsigned char* p = m_src + (int64_t)k * m_step + m_row;
             __builtin_amdgcn_global_load_lds((gptr)p, (lptr)(base + m_dst), 4, 0, 0);
+        }
+        if (c == LPS - 1) {
+            b_base += b_step;
+            asm volatile("" : "+s"(b_base));
         }
     };
 
@@ -201,12 +212,6 @@ __global__ __launch_bounds__(512) void experts_gemm_kernel(ExpertArgs a, int til
     const int swz = (fr >> 1) & 7;                   // (tile offsets are multiples of 16 rows)
     const int a_row = (wm * WM + fr) * 128, b_row = B_OFF + (wn * WC + fr) * 128;
 
-    auto wait_stage = [&](int k) __attribute__((always_inline)) {
-        // the copies of stage k have landed (they are the oldest; up to RING - 2 younger stages may be in flight)
-        if (k + RING - 2 < stages) wait_vmcnt_e<(RING - 2) * LPS>();
-        else wait_vmcnt_e<0>();
-    };
-
 #pragma unroll
     for (int u = 0; u < RING; ++u)
         if (u < stages) {
@@ -223,45 +228,74 @@ __global__ __launch_bounds__(512) void experts_gemm_kernel(ExpertArgs a, int til
             u32x4 c[2];
         } op_t;
         const int c0 = ((2 * fk) ^ swz) * 16, c1 = ((2 * fk + 1) ^ swz) * 16;
+        // Tile (i, j) of the wave is slice q = i TJ + j of a stage: its MFMA, the fold of the slice two in front, and a
+        // share of the LDS reads and copies, with the scheduler fenced between slices (left alone it reads every fragment
+        // right in front of its MFMA).  The fragment of activation row tile i + 1 is read during tile i; the barrier
+        // stands before the last row tile, and a column's weight fragment for the next stage is read behind the last MFMA
+        // that uses the old one.
+        op_t fa[2], fb[TJ];
+        float sx[2], sw[TJ];
+        float4_t d[4];
+        float sc[4];
+        const float4_t zero4 = float4_t{0.f, 0.f, 0.f, 0.f};
+        auto read_a = [&](const unsigned char* base, int i, int buf) __attribute__((always_inline)) {
+            fa[buf].c[0] = *(const u32x4*)(base + a_row + i * 2048 + c0);
+            fa[buf].c[1] = *(const u32x4*)(base + a_row + i * 2048 + c1);
+            sx[buf] = *(const float*)(base + M_OFF + (wm * WM + i * 16 + fr) * 4);
+        };
+        auto read_b = [&](const unsigned char* base, int j) __attribute__((always_inline)) {
+            fb[j].c[0] = *(const u32x4*)(base + b_row + j * 2048 + c0);
+            fb[j].c[1] = *(const u32x4*)(base + b_row + j * 2048 + c1);
+            sw[j] = *(const float*)(base + M_OFF + (BM + wn * WC + j * 16 + 4 * fk) * 4);
+        };
+        constexpr int NS = TI * TJ;
+        auto fold = [&](int q) __attribute__((always_inline)) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[q / TJ][q % TJ][e] = __builtin_fmaf(d[q % 4][e], sc[q % 4], acc[q / TJ][q % TJ][e]);
+        };
+        static_assert(TJ == 4 && TI % 2 == 0, "slices");
+        read_a(smem, 0, 0);
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) read_b(smem, j);
+        const unsigned char* base = smem;
         int slot = 0;
-#pragma unroll 1
-        for (int k = 0; k < stages; ++k) {
-            const unsigned char* base = smem + slot * SH::STAGE;
-            op_t fb[TJ];
-            float sw[TJ];
+        auto stage = [&](int k, auto refill_tag) __attribute__((always_inline)) {
+            constexpr bool REFILL = decltype(refill_tag)::value;
+            const int next_slot = slot == RING - 1 ? 0 : slot + 1;
+            const unsigned char* next = smem + next_slot * SH::STAGE;
 #pragma unroll
-            for (int j = 0; j < TJ; ++j) {
-                fb[j].c[0] = *(const u32x4*)(base + b_row + j * 2048 + c0);
-                fb[j].c[1] = *(const u32x4*)(base + b_row + j * 2048 + c1);
-                sw[j] = *(const float*)(base + M_OFF + (BM + wn * WC + j * 16 + 4 * fk) * 4);
-            }
-            const float4_t zero4 = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < TI; ++i) {
-                op_t fa;
-                fa.c[0] = *(const u32x4*)(base + a_row + i * 2048 + c0);
-                fa.c[1] = *(const u32x4*)(base + a_row + i * 2048 + c1);
-                const float sx = *(const float*)(base + M_OFF + (wm * WM + i * 16 + fr) * 4);
-#pragma unroll
-                for (int j = 0; j < TJ; ++j) {
-                    const float4_t d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j].v, fa.v, zero4, 0, 0, 0, 127, 0, 127);
-                    const float sc = sx * sw[j];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(d[e], sc, acc[i][j][e]);
+            for (int q = 0; q < NS; ++q) {
+                const int i = q / TJ, j = q % TJ;
+                if (q == (TI - 1) * TJ) {
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    wait_vmcnt_e<REFILL ? (RING - 2) * LPS : 0>();
+                    bare_barrier();
                 }
-            }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            bare_barrier();  // everybody has read the slot
-            if (k + RING < stages) {
+                d[q % 4] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j].v, fa[i & 1].v, zero4, 0, 0, 0, 127, 0, 127);
+                sc[q % 4] = sx[i & 1] * sw[j];
+                if (q >= 2) fold(q - 2);
+                if (i + 1 < TI) {
+                    if (j == 0) read_a(base, i + 1, (i + 1) & 1);
+                } else {
+                    if (j == 0) read_a(next, 0, 0);
+                    read_b(next, j);
+                    if constexpr (REFILL) {
 #pragma unroll
-                for (int c = 0; c < LPS; ++c) issue_one(k + RING, slot, c);
-                wait_vmcnt_e<(RING - 1) * LPS>();
-            } else {
-                wait_vmcnt_e<0>();
+                        for (int c = j * LPS / TJ; c < (j + 1) * LPS / TJ; ++c) issue_one(k + RING, slot, c);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            bare_barrier();
-            slot = slot == RING - 1 ? 0 : slot + 1;
-        }
+            fold(NS - 2);
+            fold(NS - 1);
+            slot = next_slot;
+            base = next;
+        };
+        int k = 0;
+#pragma unroll 1
+        for (; k + RING < stages; ++k) stage(k, std::true_type{});
+#pragma unroll 1
+        for (; k < stages; ++k) stage(k, std::false_type{});
     } else {
         u32x4 fa[2][TI], fb[2][TJ];
         auto read_a = [&](const unsigned char* base, int s, int buf, int i) __attribute__((always_inline)) {
@@ -307,11 +341,19 @@ __global__ __launch_bounds__(512) void experts_gemm_kernel(ExpertArgs a, int til
         // register q (codes 2q, 2q + 1) of the operand of column set j
         auto dequant = [&](uint32_t w, const ColMeta<BF16>& m, int q) __attribute__((always_inline)) -> uint32_t {
             if constexpr (BF16) {
-                const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
+                uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
+                asm("" : "+v"(lo), "+v"(hi));  // opaque: whole bytes, so that each is one v_cvt_f32_ubyte
                 return pack_bf16x2(__builtin_fmaf((float)((lo >> (8 * q)) & 0xffu), m.s, m.z), __builtin_fmaf((float)((hi >> (8 * q)) & 0xffu), m.s, m.z));
             } else {
                 return dequant_pair<BF16>((__builtin_amdgcn_perm(w, w, 0x0c000c00u | (q << 16) | q) & nat_mask) | nat_magic, m, 1024.0f, 64.0f);
             }
+        };
+
+        // the copies of the last K-step's slice q (the slot is free behind the stage's barrier)
+        auto refill_slice = [&](int k, int slot, int q, bool on) __attribute__((always_inline)) {
+            if (!on) return;
+#pragma unroll
+            for (int c = q * LPS / (TI * TJ); c < (q + 1) * LPS / (TI * TJ); ++c) issue_one(k + RING, slot, c);
         };
 
         // ---- prologue: fragments of K-step 0
@@ -330,11 +372,10 @@ __global__ __launch_bounds__(512) void experts_gemm_kernel(ExpertArgs a, int til
             for (int j = 0; j < TJ; ++j) read_b(base, 0, 0, j);
         }
         int slot = 0;
-#pragma unroll 1
-        for (int k = 0; k < stages; ++k) {
+        auto stage = [&](int k, auto refill_tag) __attribute__((always_inline)) {
+            constexpr bool REFILL = decltype(refill_tag)::value;
             const int next_slot = slot == RING - 1 ? 0 : slot + 1;
             const unsigned char* next = smem + next_slot * SH::STAGE;
-            const bool refill = k + RING < stages;
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
                 const int cur = s & 1, nxt = cur ^ 1;
@@ -342,56 +383,56 @@ __global__ __launch_bounds__(512) void experts_gemm_kernel(ExpertArgs a, int til
                     // the fragments of this K-step are in registers; the next stage's copies have landed, here and (behind the
                     // barrier) everywhere, and nobody reads this stage's slot any more
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                    if (k + 1 < stages) wait_stage(k + 1);
+                    wait_vmcnt_e<REFILL ? (RING - 2) * LPS : 0>();
                     bare_barrier();
-                    if (refill) {
-#pragma unroll
-                        for (int c = 0; c < LPS; ++c) issue_one(k + RING, slot, c);
-                    }
                 }
                 const unsigned char* from = s == 3 ? next : base;
                 const int s1 = (s + 1) & 3;
+                // slices of one MFMA each, with the scheduler fenced between them (left alone it reads every fragment
+                // right in front of its MFMA)
                 if constexpr (W4) {
-                    // MFMAs of column set 0 with the dequantisation of set 1, then set 1 with set 0 of the next K-step
                     read_words(from, s1, nxt);
                     if (s == 3) read_meta(next);
+                    // MFMAs of column set 0 with the dequantisation of set 1, then set 1 with set 0 of the next K-step
 #pragma unroll
                     for (int j = 0; j < TJ; ++j) {
 #pragma unroll
                         for (int i = 0; i < TI; ++i) {
                             mfma(i, j, cur, fb[0][j]);
                             if (j == 0) read_a(from, s1, nxt, i);
-                            if (j + 1 < TJ) {
+                            if (i == 0 && j == TJ - 1 && s == 3) convert_meta(0);
 #pragma unroll
-                                for (int q = i * 4 / TI; q < (i + 1) * 4 / TI; ++q) fb[0][j + 1][q] = dequant(words[cur][j + 1], meta[s / 2][j + 1], q);
-                            } else if (TJ > 1) {
-                                if (i == 0 && s == 3) convert_meta(0);
-#pragma unroll
-                                for (int q = i * 4 / TI; q < (i + 1) * 4 / TI; ++q) fb[0][0][q] = dequant(words[nxt][0], meta[s == 3 ? 0 : s1 / 2][0], q);
-                            } else {
-                                // one column set: its registers for the next K-step are the other buffer
-                                if (i == 0 && s == 3) convert_meta(0);
-#pragma unroll
-                                for (int q = i * 4 / TI; q < (i + 1) * 4 / TI; ++q) fb[1][0][q] = dequant(words[nxt][0], meta[s == 3 ? 0 : s1 / 2][0], q);
+                            for (int q = i * 4 / TI; q < (i + 1) * 4 / TI; ++q) {
+                                if (j + 1 < TJ) fb[0][j + 1][q] = dequant(words[cur][j + 1], meta[s / 2][j + 1], q);
+                                // (one column set: its registers for the next K-step are the other buffer)
+                                else fb[TJ > 1 ? 0 : 1][0][q] = dequant(words[nxt][0], meta[s == 3 ? 0 : s1 / 2][0], q);
                             }
+                            if (s == 3) refill_slice(k, slot, j * TI + i, REFILL);
+                            __builtin_amdgcn_sched_barrier(0);
                         }
                     }
                     if constexpr (TJ == 1) fb[0][0] = fb[1][0];
                     if (s == 3) convert_meta(1);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < TJ; ++j) read_b(from, s1, nxt, j);
-#pragma unroll
-                    for (int i = 0; i < TI; ++i) {
-                        read_a(from, s1, nxt, i);
-#pragma unroll
-                        for (int j = 0; j < TJ; ++j) mfma(i, j, cur, fb[cur][j]);
+                    for (int q = 0; q < TI * TJ; ++q) {
+                        const int i = q / TJ, j = q % TJ;
+                        mfma(i, j, cur, fb[cur][j]);
+                        if (q < TJ) read_b(from, s1, nxt, q);
+                        if (j == 0) read_a(from, s1, nxt, i);
+                        if (s == 3) refill_slice(k, slot, q, REFILL);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
                 }
             }
             slot = next_slot;
             base = next;
-        }
+        };
+        int k = 0;
+#pragma unroll 1
+        for (; k + RING < stages; ++k) stage(k, std::true_type{});
+#pragma unroll 1
+        for (; k < stages; ++k) stage(k, std::false_type{});
     }
 
     // ---- epilogue: the lane holds row fr of an MFMA tile and runs of 4 columns
