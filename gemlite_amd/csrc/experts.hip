@@ -104,7 +104,7 @@ int validate(const gla_experts_args* p) {
     }
     if (p->tile_config != -1) {
         const int rows = p->tile_config % 1000, splits = p->tile_config / 1000;
-        if (p->tile_config < 0 || splits > 64 || (rows != 16 && rows != 32 && rows != 64 && rows != 128 && rows != 256) || (rows > 32 && splits > 1)) {
+        if (p->tile_config < 0 || splits > 64 || (rows != 4 && rows != 16 && rows != 64 && rows != 128 && rows != 256) || (rows > 16 && splits > 1)) {
             set_error("experts: tile_config %d", p->tile_config);
             return GLA_ERR_INVALID_ARGUMENT;
         }
@@ -172,8 +172,7 @@ int validate(const gla_experts_args* p) {
 
 struct ExpertPlanHost {
     int format;
-    int bm;      // 0: streaming kernel
-    int row_tiles;
+    int bm;      // rows per tile: 4, 16 (streaming kernel), 64, 128, 256 (tiled GEMM)
     int S;
     bool to_partials;
     bool quantise;                       // F8: a launch in front writes codes and scales to the workspace
@@ -183,17 +182,15 @@ struct ExpertPlanHost {
 ExpertPlanHost plan_of(const gla_experts_args& p) {
     ExpertPlanHost h;
     h.format = format_of(p);
-    h.bm = 0;
     const int want_rows = p.tile_config < 0 ? 0 : p.tile_config % 1000, want_s = p.tile_config < 0 ? 0 : p.tile_config / 1000;
     const int active = p.R < p.E ? p.R : p.E;
     const int per = active > 0 ? p.R / active : 0;
-    if (want_rows ? want_rows > 32 : per > 24) h.bm = want_rows ? want_rows : (per > 160 ? 256 : (per > 64 ? 128 : 64));
-    h.row_tiles = want_rows == 16 ? 1 : (want_rows == 32 || per > 8 ? 2 : 1);
+    h.bm = want_rows ? want_rows : (per > 160 ? 256 : per > 64 ? 128 : per > 8 ? 64 : per > 2 ? 16 : 4);
     h.S = want_s > 0 ? want_s : 1;
     h.to_partials = p.mode == GLA_EXPERTS_COMBINED || h.S > 1;
     h.partial_bytes = h.to_partials ? (int64_t)h.S * p.R * p.N * 4 : 0;
     const int64_t rows = p.mode == GLA_EXPERTS_GATED ? p.T : p.R;
-    h.quantise = h.format == kEF8 && (h.bm > 0 || h.row_tiles > 1);
+    h.quantise = h.format == kEF8 && h.bm > 16;
     h.code_bytes = h.quantise ? rows * p.K : 0;
     h.total_bytes = h.partial_bytes + h.code_bytes + (h.quantise ? rows * (p.K / 128) * 4 : 0);
     return h;
@@ -260,7 +257,7 @@ int gla_experts_matmul(const gla_experts_args* p, void* stream) {
         a.xsm = p->K;
         a.scales_x = scales_x;
     }
-    const int rc2 = h.bm > 0 ? launch_experts_gemm(a, h.format, bf16, h.bm, s) : launch_experts_stream(a, h.format, bf16, h.row_tiles, s);
+    const int rc2 = h.bm > 16 ? launch_experts_gemm(a, h.format, bf16, h.bm, s) : launch_experts_stream(a, h.format, bf16, h.bm, s);
     if (rc2 != GLA_OK || !h.to_partials) return rc2;
     const bool combined = p->mode == GLA_EXPERTS_COMBINED;
     FinishArgs f{a.partials, p->offsets, p->places, p->weights, p->out, p->out_stride_m, p->R, p->E, p->N, h.S, p->top_k, a.half};

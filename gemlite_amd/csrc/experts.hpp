@@ -14,11 +14,11 @@ namespace gla {
 enum ExpertFormat { kEW4 = 0, kEF8 = 1, kE16 = 2 };
 
 struct ExpertArgs {
-    const unsigned char* x;         // activation rows: fp16 / bf16, or e4m3 bytes (F8 with scales_x)
+    const unsigned char* x;         // activation rows: fp16 / bf16, or e4m3 bytes (F8, tiled GEMM)
     const unsigned char* w;         // expert 0's weights
     const unsigned char* scales;    // W4: [E][G][N] 16-bit; F8: [E][K/128][ceil(N/128)] fp32
     const unsigned char* zeros;     // W4: as scales, or NULL
-    const float* scales_x;          // F8: [rows of x][K/128]; NULL: x holds 16-bit rows and the kernel quantises them
+    const float* scales_x;          // F8, tiled GEMM: [rows of x][K/128] (the streaming kernel quantises 16-bit rows itself)
     const float* bias;              // [E][N] fp32 or NULL
     void* out;                      // 16-bit rows (rows / gated)
     float* partials;                // [S][R][N] fp32 (combined, or S > 1)
@@ -179,7 +179,7 @@ __device__ __forceinline__ float high16(uint32_t v) {
 // 16-bit rows -> e4m3 codes [rows][K] and scales [rows][K/128] (experts_quant.hip)
 int launch_experts_quantise(const void* x, bool bf16, int64_t xsm, int rows, int K, unsigned char* codes, float* scales, hipStream_t stream);
 
-int launch_experts_stream(const ExpertArgs& a, int format, bool bf16, int row_tiles, hipStream_t stream);
+int launch_experts_stream(const ExpertArgs& a, int format, bool bf16, int rows, hipStream_t stream);
 int launch_experts_gemm(const ExpertArgs& a, int format, bool bf16, int bm, hipStream_t stream);
 
 // logits NULL: the ids are given and only sorted.  counts: (E + 1) * route_blocks(T) integers of scratch.

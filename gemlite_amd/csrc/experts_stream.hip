@@ -1,22 +1,26 @@
-// Products grouped by expert, few rows per expert: every weight is read once, straight into registers, and meets one or
-// two 16-row MFMA tiles of activations.  Bound by the bytes of the experts that have rows.
+// Products grouped by expert, few rows per expert: every weight is read once and meets one 16-row MFMA tile that holds MR
+// (4 or 16) activation rows.  Bound by the bytes of the experts that have rows.
 //
-//  * A workgroup owns 64 columns of one expert's weights (gated: 32 gate and the same 32 up columns) for one tile of
-//    16 RT rows; its NW waves split K, so that a launch with few column tiles still has thousands of loads in flight,
-//    and meet once in LDS at the end.  gridDim.z splits K further when even that leaves the chip empty; those sums go
-//    to the workspace in fp32 and the finishing kernel adds them in order.
-//  * A wave walks its K range in units of 128 values (16-bit weights: 64) with a ring of D units of weights,
-//    activations and scales in registers, all loads issued D - 1 units ahead.  A unit past the end of the range loads
-//    the same few bytes for every lane instead (one request), which keeps the loop free of branches around loads.
-//  * W4: a lane's 128-bit load is the packed words of 4 adjacent columns of one word row; a word is 8 K-values of one
-//    column = the lane's share of the B operand of v_mfma_f32_16x16x32.  The codes go into the MFMA as they are (bf16
-//    128 + q, fp16 1024 + q: one shift and one masked OR per pair) and the group's scale and zero are applied to the
-//    sums: w = s q + z  =>  sum(x w) = s sum(x (off + q)) + (z - off s) sum(x), with sum(x) from one more MFMA against
-//    ones.  Per code that is 1 vector instruction against 2.5 for dequantising in front of the MFMA, which at 4 bits
-//    would be as slow as the memory, and the weights are never rounded.
-//  * F8: the e4m3 bytes of a 128-block go into one v_mfma_f32_16x16x128 that starts from zero; its result joins the fp32
-//    sum times the block's two scales.
+//  * A workgroup owns WC columns (64; 16-bit weights 32) of one expert for one tile of MR rows; gated calls take half of
+//    them from the gate and the same ones of the up projection.  Its NW waves split K and meet once in LDS at the end, so
+//    a launch with few column tiles still has thousands of loads in flight; gridDim.z splits K further where even that
+//    leaves the chip empty (fp32 sums to the workspace, added in order by the finishing kernel).
+//  * A wave walks its K range in units of 128 values and shares nothing with the others on the way: the load unit copies a
+//    unit's weights, activation rows and scales straight into the wave's own ring of D slots in LDS (global_load_lds), so
+//    what is in flight costs no registers and no barrier stands in the loop; the wave waits on its own copy counter.
+//    (With the same units in registers, 150 to 220 of them per lane, a CU held 8 waves: 64 columns of 8 experts, one
+//    token, 4-bit 4096 -> 2 x 14336: 46 us.)
+//  * W4: a 16-byte piece is the packed words of 4 adjacent columns of one word row; a word is 8 K-values of one column =
+//    the lane's share of the B operand of v_mfma_f32_16x16x32.  The codes go into the MFMA as they are (bf16 128 + q, fp16
+//    1024 + q: one shift and one masked OR per pair) and the group's scale and zero are applied to the sums:
+//    w = s q + z  =>  sum(x w) = s sum(x (off + q)) + (z - off s) sum(x), with sum(x) from one more MFMA against ones.
+//    Per code that is 1 vector instruction against 3 for dequantising in front of the MFMA, which at 4 bits would be as
+//    slow as the memory, and the weights are never rounded.
+//  * F8: 16-bit rows are quantised on the way into the MFMA, 4 lanes to a row's 128 values; the e4m3 bytes of a 128-block
+//    go into one v_mfma_f32_16x16x128 that starts from zero, and its result joins the fp32 sum times the two scales.
 //  * 16-bit weights: plain MFMAs.
+#include <type_traits>
+
 #include "common.hpp"
 #include "experts.hpp"
 
@@ -27,6 +31,15 @@ namespace {
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 
+__device__ __align__(16) unsigned char g_zero_piece[16];  // what activations past the end of K are read from
+
+template <int N>
+__device__ __forceinline__ void wait_vmcnt_s() {
+    static_assert(N >= 0 && N < 64, "vmcnt is a 6-bit counter");
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+    asm volatile("" ::: "memory");
+}
+
 template <bool BF16>
 __device__ __forceinline__ float4_t mfma16(const u32x4& a, const u32x4& b, float4_t c) {
     if constexpr (BF16)
@@ -35,181 +48,182 @@ __device__ __forceinline__ float4_t mfma16(const u32x4& a, const u32x4& b, float
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
 }
 
-__device__ __forceinline__ u32x4 load16(const unsigned char* p) { return *(const u32x4*)p; }
-__device__ __forceinline__ u32x4 load16_streaming(const unsigned char* p) { return __builtin_nontemporal_load((const u32x4*)p); }
-
-// Four consecutive K-values and the four after them as registers (k, k + 4): the order of the packed codes.
+// Eight consecutive K-values as registers (k, k + 4): the order of the packed codes.
 __device__ __forceinline__ u32x4 pairs_of(const u32x4& v) {
     return u32x4{__builtin_amdgcn_perm(v.z, v.x, 0x05040100u), __builtin_amdgcn_perm(v.z, v.x, 0x07060302u),
                  __builtin_amdgcn_perm(v.w, v.y, 0x05040100u), __builtin_amdgcn_perm(v.w, v.y, 0x07060302u)};
 }
 
 // FU: K-values between two folds of a W4 group's constants (the largest of 128, 64, 32 that divides the group).
-// QX (F8): x holds 16-bit rows and every wave quantises its share of a unit itself, 4 lanes to a row's 128 values (decode:
-// one launch less; the work is repeated by every column tile, which is why more rows are quantised by a launch in front).
-template <int FMT, bool BF16, int RT, int FU, int NW, int D, bool QX>
-__global__ __launch_bounds__(NW * 64) void experts_stream_kernel(ExpertArgs a) {
-    constexpr int KU = FMT == kE16 ? 64 : 128;            // K-values per unit
-    constexpr int NT = 4;                                 // 16-column MFMA tiles per wave
-    constexpr int WL = FMT == kEW4 ? 4 : 2 * NT;          // weight loads per lane and unit
-    constexpr int XL = FMT == kEW4 || QX ? 4 : 2;         // activation loads per lane, row tile and unit
-    constexpr int FOLDS = KU / FU;
-    constexpr int GL = FMT == kEW4 ? FOLDS : 1;
+template <int FMT, int MR, int FU>
+struct StreamShape {
+    static constexpr int WC = FMT == kE16 ? 32 : 64;
+    static constexpr int NT = WC / 16;
+    static constexpr int FOLDS = 128 / FU;
+    static constexpr int W_OPS = FMT == kEW4 ? 4 : 8, X_OPS = MR / 4, M_OPS = FMT == kEW4 ? FOLDS : (FMT == kEF8 ? 1 : 0);
+    static constexpr int OPS = W_OPS + X_OPS + M_OPS;
+    static constexpr int W_BYTES = W_OPS * 1024, X_BYTES = X_OPS * 1024, SLOT = W_BYTES + X_BYTES + M_OPS * 256;
+    static constexpr int NW = 4;
+    static constexpr int D = FMT == kEW4 && MR == 4 ? 3 : 2;
+    static constexpr int RING = D * SLOT;                     // per wave
+    static constexpr int LDS = NW * (RING > 16 * WC * 4 ? RING : 16 * WC * 4);
+};
 
+template <int FMT, bool BF16, int MR, int FU>
+__global__ __launch_bounds__(256) void experts_stream_kernel(ExpertArgs a) {
+    using SH = StreamShape<FMT, MR, FU>;
+    constexpr int WC = SH::WC, NT = SH::NT, NW = SH::NW, D = SH::D, OPS = SH::OPS;
+    constexpr int X_OFF = SH::W_BYTES, M_OFF = X_OFF + SH::X_BYTES;
+
+    extern __shared__ __align__(16) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int cg = lane & 15, kb = lane >> 4;
-    const ExpertTile tile = find_tile<16 * RT>(a.offsets, a.E, a.R, !a.to_partials, [](int) { return (int)blockIdx.y; });
-    if (tile.expert < 0) return;
     const int ct = blockIdx.x, split = blockIdx.z;
-    extern __shared__ __align__(16) float red[];  // [NW][16 RT][64]
+    const ExpertTile tile = find_tile<MR>(a.offsets, a.E, a.R, !a.to_partials, [](int) { return (int)blockIdx.y; });
+    if (tile.expert < 0) return;
+    float* red = (float*)smem;  // [NW][16][WC], when the ring is done
 
     if (tile.expert < a.E) {
+        unsigned char* ring = smem + wave * SH::RING;
         const unsigned char* we = a.w + (int64_t)tile.expert * a.w_stride_e;
         const unsigned char* se = a.scales + (int64_t)tile.expert * a.meta_stride_e;
         const unsigned char* ze = a.zeros == nullptr ? se : a.zeros + (int64_t)tile.expert * a.meta_stride_e;
-        const int units = (a.K + KU - 1) / KU;
-        const int slots = a.S * NW, slot = split * NW + wave;
-        const int u0 = units * slot / slots, u1 = units * (slot + 1) / slots;
+        const int units = (a.K + 127) / 128;
+        const int slots = a.S * NW, slot_id = split * NW + wave;
+        const int u0 = (int)((int64_t)units * slot_id / slots), u1 = (int)((int64_t)units * (slot_id + 1) / slots);
 
-        // ---- addresses
-        const unsigned char* xr[RT];
-        const float* sxr[RT];
+        // ---- copy plan: a wave-uniform base that advances per unit plus 32-bit lane offsets; activation rows have
+        // 64-bit addresses of their own
+        const unsigned char* x_src[SH::X_OPS];
+        int x_piece[SH::X_OPS];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            int r = tile.row0 + 16 * rt + cg;
-            if (r > tile.row_end - 1) r = tile.row_end - 1;  // computed, never stored
-            const int64_t src = source_row(a, r);
-            xr[rt] = a.x + src * a.xsm;
-            if constexpr (FMT == kEF8 && !QX) sxr[rt] = a.scales_x + src * (a.K / 128);
+        for (int q = 0; q < SH::X_OPS; ++q) {
+            const int row = 4 * q + kb;
+            int r = tile.row0 + row;
+            if (r > tile.row_end - 1) r = tile.row_end - 1;  // multiplied, never stored
+            x_piece[q] = (cg ^ row) * 16;                    // piece p of row r lies at position p ^ r
+            x_src[q] = a.x + source_row(a, r) * a.xsm + x_piece[q];
         }
-        uint32_t w_off[FMT == kEW4 ? 1 : NT];
-        uint32_t m_off[NT];
-        auto column = [&](int c) __attribute__((always_inline)) { return unit_column_inside<64>(a.half, a.N, ct, c); };
+        uint32_t w_off[FMT == kEW4 ? 1 : SH::W_OPS];
         if constexpr (FMT == kEW4) {
-            w_off[0] = (uint32_t)column(4 * cg) * 4u + (uint32_t)kb * (uint32_t)a.N * 4u;
-            m_off[0] = (uint32_t)column(4 * cg) * 2u;
+            w_off[0] = ((uint32_t)unit_column_inside<WC>(a.half, a.N, ct, 4 * cg) + (uint32_t)kb * (uint32_t)a.N) * 4u;
         } else {
+            constexpr int BYTES = FMT == kE16 ? 256 : 128, LANES = BYTES / 16, ROWS = 64 / LANES;  // of a column per unit
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const int n = column(16 * t + cg);
-                w_off[t] = FMT == kEF8 ? (uint32_t)n * (uint32_t)a.K + (uint32_t)kb * 32u : ((uint32_t)n * (uint32_t)a.K + (uint32_t)kb * 16u) * 2u;
-                m_off[t] = (uint32_t)(column(16 * t + 4 * kb) >> 7) * 4u;
+            for (int q = 0; q < SH::W_OPS; ++q) {
+                const int c = q * ROWS + lane / LANES;
+                const int p = FMT == kE16 ? (lane & 15) ^ (c & 15) : (lane & 7) ^ ((c >> 1) & 7);
+                w_off[q] = (uint32_t)unit_column_inside<WC>(a.half, a.N, ct, c) * (uint32_t)(a.K * (FMT == kE16 ? 2 : 1));
+                w_off[q] += (uint32_t)(p * 16);
             }
+        }
+        uint32_t m_off = 0;
+        const unsigned char* m_base = se;
+        if constexpr (FMT == kEW4) {
+            const int c = 2 * (lane & 31);  // a pair lies inside its run of 4
+            m_off = (uint32_t)(unit_column_inside<WC>(a.half, a.N, ct, c & ~3) + (c & 3)) * 2u;
+            m_base = lane < 32 ? se : ze;
+        } else if constexpr (FMT == kEF8) {
+            m_off = (uint32_t)(unit_column_inside<WC>(a.half, a.N, ct, lane & ~3) >> 7) * 4u;
         }
         const int groups = FMT == kEW4 ? a.K / a.group : 0;
-        const int nblk = (a.N + 127) / 128;
-
-        struct Unit {
-            u32x4 w[WL];
-            u32x4 x[RT][XL];
-            u32x2 s[GL], z[GL];           // W4
-            float sx[RT], sw[NT];         // F8
-        };
-        Unit buf[D];
-        auto group_at = [&](int k) __attribute__((always_inline)) {
-            const int g = a.group == FU ? k / FU : k / a.group;
-            return g > groups - 1 ? groups - 1 : g;
-        };
-        auto load = [&](Unit& b, int u) __attribute__((always_inline)) {
-            const uint32_t on = u < u1 ? 0xffffffffu : 0u;
-            const int uc = u < u1 ? u : u0;
+        const int Kb = a.K * 2;
+        const unsigned char* zero_piece = g_zero_piece;
+        asm volatile("" : "+s"(zero_piece));
+        typedef const __attribute__((address_space(1))) void* gptr;
+        typedef __attribute__((address_space(3))) void* lptr;
+        auto issue = [&](int u, unsigned char* slot) __attribute__((always_inline)) {
             if constexpr (FMT == kEW4) {
-                const uint32_t row = (uint32_t)a.N * 4u;
+                const unsigned char* base = we + (int64_t)u * 16 * a.N * 4;
+                const int rows = a.K / 8 - u * 16;  // word rows past the end of K: the unit's first ones again (they meet zeros)
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    // (a unit may end past K: its last steps read the unit's first ones again and meet zeros)
-                    const int step = uc * 128 + s * 32 < a.K ? s : 0;
-                    b.w[s] = load16_streaming(we + (int64_t)(uc * 16 + 4 * step) * row + (w_off[0] & on));
+                for (int s = 0; s < 4; ++s)
+                    __builtin_amdgcn_global_load_lds((gptr)(base + (int64_t)(4 * s < rows ? 4 * s : 0) * a.N * 4 + w_off[0]), (lptr)(slot + s * 1024), 16, 0, 2);
+            } else {
+                const unsigned char* base = we + (int64_t)u * (FMT == kE16 ? 256 : 128);
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) b.x[rt][s] = load16(xr[rt] + (int64_t)(uc * 256 + step * 64) + (((uint32_t)kb * 16u) & on));
+                for (int q = 0; q < SH::W_OPS; ++q) {
+                    uint32_t off = w_off[q];
+                    if constexpr (FMT == kE16) {
+                        // a unit may end past K: those pieces are the column's first ones of the unit (they meet zeros)
+                        const int p = ((lane & 15) ^ ((q * 4 + kb) & 15)) * 16;
+                        if (u * 256 + p >= Kb) off -= (uint32_t)p;
+                    }
+                    __builtin_amdgcn_global_load_lds((gptr)(base + off), (lptr)(slot + q * 1024), 16, 0, 2);
                 }
+            }
 #pragma unroll
-                for (int h = 0; h < GL; ++h) {
-                    const int64_t g = (int64_t)group_at(uc * 128 + h * FU) * (a.N * 2);
-                    b.s[h] = *(const u32x2*)(se + g + (m_off[0] & on));
-                    b.z[h] = *(const u32x2*)(ze + g + (m_off[0] & on));
+            for (int q = 0; q < SH::X_OPS; ++q) {
+                const unsigned char* p = x_src[q] + (int64_t)u * 256;
+                if constexpr (FMT != kEF8) p = u * 256 + x_piece[q] < Kb ? p : zero_piece;
+                __builtin_amdgcn_global_load_lds((gptr)p, (lptr)(slot + X_OFF + q * 1024), 16, 0, 0);
+            }
+            if constexpr (FMT == kEW4) {
+#pragma unroll
+                for (int h = 0; h < SH::FOLDS; ++h) {
+                    int g = a.group == FU ? u * SH::FOLDS + h : (u * 128 + h * FU) / a.group;
+                    if (g > groups - 1) g = groups - 1;
+                    __builtin_amdgcn_global_load_lds((gptr)(m_base + (int64_t)g * a.N * 2 + m_off), (lptr)(slot + M_OFF + h * 256), 4, 0, 0);
                 }
             } else if constexpr (FMT == kEF8) {
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const unsigned char* p = we + (int64_t)uc * 128 + (w_off[t] & on);
-                    b.w[2 * t] = load16_streaming(p);
-                    b.w[2 * t + 1] = load16_streaming(p + 16);
-                    b.sw[t] = *(const float*)(se + (int64_t)uc * nblk * 4 + m_off[t]);
-                }
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    const unsigned char* p = xr[rt] + (int64_t)uc * (QX ? 256 : 128) + (((uint32_t)kb * (QX ? 64u : 32u)) & on);
-#pragma unroll
-                    for (int i = 0; i < XL; ++i) b.x[rt][i] = load16(p + 16 * i);
-                    if constexpr (!QX) b.sx[rt] = sxr[rt][uc];
-                }
-            } else {
-                const bool in = uc * 64 + kb * 16 < a.K;  // the last unit may be half one
-                const int64_t k = (int64_t)uc * 128;
-                const uint32_t back = in ? 0u : (uint32_t)kb * 32u;
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const unsigned char* p = we + k + ((w_off[t] - back) & on);
-                    b.w[2 * t] = load16_streaming(p);
-                    b.w[2 * t + 1] = load16_streaming(p + 16);
-                }
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    const unsigned char* p = xr[rt] + k + (((uint32_t)kb * 32u - back) & on);
-                    b.x[rt][0] = load16(p);
-                    b.x[rt][1] = load16(p + 16);
-                }
+                __builtin_amdgcn_global_load_lds((gptr)(se + (int64_t)u * ((a.N + 127) / 128) * 4 + m_off), (lptr)(slot + M_OFF), 4, 0, 0);
             }
         };
 
-        float4_t acc[RT][NT];
+        float4_t acc[NT];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int t = 0; t < NT; ++t) acc[rt][t] = float4_t{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < NT; ++t) acc[t] = float4_t{0.f, 0.f, 0.f, 0.f};
         const float4_t zero4 = float4_t{0.f, 0.f, 0.f, 0.f};
         uint32_t mask = 0x000f000fu, magic = BF16 ? 0x43004300u : 0x64006400u;
         asm volatile("" : "+s"(mask), "+v"(magic));  // registers, so that v_and_or_b32 is selected
         const uint32_t one = BF16 ? 0x3f803f80u : 0x3c003c00u;
         const u32x4 ones = u32x4{one, one, one, one};
+        const int x_row = cg < MR ? cg : MR - 1;
+        auto x_at = [&](const unsigned char* slot, int piece) __attribute__((always_inline)) {
+            return *(const u32x4*)(slot + X_OFF + x_row * 256 + ((piece ^ x_row) & 15) * 16);
+        };
 
-        auto compute = [&](Unit& b, int u) __attribute__((always_inline)) {
+        // one unit: its operands from LDS into registers, `refill` of the slot, then the arithmetic
+        auto unit = [&](const unsigned char* slot, auto refill) __attribute__((always_inline)) {
             if constexpr (FMT == kEW4) {
+                u32x4 w[4], x[4];
+                u32x2 rs[SH::FOLDS], rz[SH::FOLDS];
 #pragma unroll
-                for (int h = 0; h < FOLDS; ++h) {
-                    float4_t dot[RT][NT], sum[RT];
+                for (int s = 0; s < 4; ++s) {
+                    w[s] = *(const u32x4*)(slot + s * 1024 + lane * 16);
+                    x[s] = x_at(slot, 4 * s + kb);
+                }
+#pragma unroll
+                for (int h = 0; h < SH::FOLDS; ++h) {
+                    rs[h] = *(const u32x2*)(slot + M_OFF + h * 256 + cg * 8);
+                    rz[h] = *(const u32x2*)(slot + M_OFF + h * 256 + 128 + cg * 8);
+                }
+                refill();
+#pragma unroll
+                for (int h = 0; h < SH::FOLDS; ++h) {
+                    float4_t dot[NT], sum;
 #pragma unroll
                     for (int s2 = 0; s2 < FU / 32; ++s2) {
                         const int s = h * (FU / 32) + s2;
-                        u32x4 xa[RT];
-#pragma unroll
-                        for (int rt = 0; rt < RT; ++rt) {
-                            xa[rt] = pairs_of(b.x[rt][s]);
-                            if (u * 128 + s * 32 >= a.K) xa[rt] = u32x4{0, 0, 0, 0};
-                            sum[rt] = mfma16<BF16>(xa[rt], ones, s2 == 0 ? zero4 : sum[rt]);
-                        }
+                        const u32x4 xa = pairs_of(x[s]);
+                        sum = mfma16<BF16>(xa, ones, s2 == 0 ? zero4 : sum);
 #pragma unroll
                         for (int t = 0; t < NT; ++t) {
-                            const uint32_t w = b.w[s][t];
-                            const u32x4 q = u32x4{(w & mask) | magic, ((w >> 4) & mask) | magic, ((w >> 8) & mask) | magic, ((w >> 12) & mask) | magic};
-#pragma unroll
-                            for (int rt = 0; rt < RT; ++rt) dot[rt][t] = mfma16<BF16>(xa[rt], q, s2 == 0 ? zero4 : dot[rt][t]);
+                            const uint32_t v = w[s][t];
+                            const u32x4 q = u32x4{(v & mask) | magic, ((v >> 4) & mask) | magic, ((v >> 8) & mask) | magic, ((v >> 12) & mask) | magic};
+                            dot[t] = mfma16<BF16>(xa, q, s2 == 0 ? zero4 : dot[t]);
                         }
                     }
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
-                        const uint32_t rs = b.s[h][t / 2] >> (16 * (t & 1)), rz = b.z[h][t / 2] >> (16 * (t & 1));
-                        const float sc = a.meta_bf16 ? bf16_bits_to_float((uint16_t)rs) : half_bits_to_float((uint16_t)rs);
-                        float zp = a.meta_bf16 ? bf16_bits_to_float((uint16_t)rz) : half_bits_to_float((uint16_t)rz);
+                        const uint32_t vs = rs[h][t / 2] >> (16 * (t & 1)), vz = rz[h][t / 2] >> (16 * (t & 1));
+                        const float sc = a.meta_bf16 ? bf16_bits_to_float((uint16_t)vs) : half_bits_to_float((uint16_t)vs);
+                        float zp = a.meta_bf16 ? bf16_bits_to_float((uint16_t)vz) : half_bits_to_float((uint16_t)vz);
                         zp = a.zeros == nullptr ? 0.0f : zp * __builtin_fmaf(a.c2, sc, a.c1);
                         const float off = __builtin_fmaf(BF16 ? -128.0f : -1024.0f, sc, zp);
 #pragma unroll
-                        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                acc[rt][t][r] = __builtin_fmaf(off, sum[rt][r], __builtin_fmaf(sc, dot[rt][t][r], acc[rt][t][r]));
+                        for (int r = 0; r < 4; ++r) acc[t][r] = __builtin_fmaf(off, sum[r], __builtin_fmaf(sc, dot[t][r], acc[t][r]));
                     }
                 }
             } else if constexpr (FMT == kEF8) {
@@ -217,78 +231,91 @@ __global__ __launch_bounds__(NW * 64) void experts_stream_kernel(ExpertArgs a) {
                     int8_t_v v;
                     u32x4 c[2];
                 } op_t;
+                op_t wo[NT], xo;
+                float sw[NT], f[32], amax = 0.0f, sx, inv;
+                const int swz = (cg >> 1) & 7;
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    op_t xo;
-                    if constexpr (QX) {
-                        float f[32], amax = 0.0f, inv;
+                for (int t = 0; t < NT; ++t) {
+                    wo[t].c[0] = *(const u32x4*)(slot + (16 * t + cg) * 128 + ((2 * kb) ^ swz) * 16);
+                    wo[t].c[1] = *(const u32x4*)(slot + (16 * t + cg) * 128 + ((2 * kb + 1) ^ swz) * 16);
+                    sw[t] = *(const float*)(slot + M_OFF + (16 * t + 4 * kb) * 4);
+                }
+                u32x4 x[4];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const uint32_t v = b.x[rt][i / 4][i % 4];
-                            f[2 * i] = low16<BF16>(v);
-                            f[2 * i + 1] = high16<BF16>(v);
-                            amax = fmaxf(amax, fmaxf(fabsf(f[2 * i]), fabsf(f[2 * i + 1])));
-                        }
-                        amax = fmaxf(amax, wave_xor(amax, 16));
-                        amax = fmaxf(amax, wave_xor(amax, 32));
-                        block_scale(amax, b.sx[rt], inv);
+                for (int i = 0; i < 4; ++i) x[i] = x_at(slot, 4 * kb + i);
+                refill();
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            xo.c[i / 4][i % 4] = quantise4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3], inv);
-                    } else {
-                        xo.c[0] = b.x[rt][0];
-                        xo.c[1] = b.x[rt][1];
-                    }
+                for (int i = 0; i < 16; ++i) {
+                    const uint32_t v = x[i / 4][i % 4];
+                    f[2 * i] = low16<BF16>(v);
+                    f[2 * i + 1] = high16<BF16>(v);
+                    amax = fmaxf(amax, fmaxf(fabsf(f[2 * i]), fabsf(f[2 * i + 1])));
+                }
+                amax = fmaxf(amax, wave_xor(amax, 16));
+                amax = fmaxf(amax, wave_xor(amax, 32));
+                block_scale(amax, sx, inv);
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        op_t wo;
-                        wo.c[0] = b.w[2 * t];
-                        wo.c[1] = b.w[2 * t + 1];
-                        const float4_t d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wo.v, xo.v, zero4, 0, 0, 0, 127, 0, 127);
-                        const float sc = b.sx[rt] * b.sw[t];
+                for (int i = 0; i < 8; ++i) xo.c[i / 4][i % 4] = quantise4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3], inv);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) acc[rt][t][r] = __builtin_fmaf(sc, d[r], acc[rt][t][r]);
-                    }
+                for (int t = 0; t < NT; ++t) {
+                    const float4_t d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wo[t].v, xo.v, zero4, 0, 0, 0, 127, 0, 127);
+                    const float sc = sx * sw[t];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[t][r] = __builtin_fmaf(sc, d[r], acc[t][r]);
                 }
             } else {
-                const bool in = u * 64 + kb * 16 < a.K;
+                u32x4 w[NT][4], x[4];
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
+                for (int s = 0; s < 4; ++s) {
+                    x[s] = x_at(slot, 4 * s + kb);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        u32x4 xa = b.x[rt][h];
-                        if (!in) xa = u32x4{0, 0, 0, 0};
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) acc[rt][t] = mfma16<BF16>(b.w[2 * t + h], xa, acc[rt][t]);
-                    }
+                    for (int t = 0; t < NT; ++t) w[t][s] = *(const u32x4*)(slot + (16 * t + cg) * 256 + ((4 * s + kb) ^ cg) * 16);
                 }
+                refill();
+#pragma unroll
+                for (int s = 0; s < 4; ++s)
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) acc[t] = mfma16<BF16>(w[t][s], x[s], acc[t]);
             }
         };
 
-        if (u0 < u1) {
 #pragma unroll
-            for (int d = 0; d < D - 1; ++d) load(buf[d], u0 + d);
+        for (int d = 0; d < D; ++d)
+            if (u0 + d < u1) issue(u0 + d, ring + d * SH::SLOT);
+        int u = u0, at = 0;
 #pragma unroll 1
-            for (int u = u0; u < u1; u += D) {
-#pragma unroll
-                for (int d = 0; d < D; ++d) {
-                    load(buf[(d + D - 1) % D], u + d + D - 1);
-                    if (u + d < u1) compute(buf[d], u + d);
-                }
-            }
+        for (; u + D < u1; ++u) {
+            wait_vmcnt_s<(D - 1) * OPS>();
+            unsigned char* slot = ring + at * SH::SLOT;
+            unit(slot, [&]() __attribute__((always_inline)) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot has been read
+                issue(u + D, slot);
+            });
+            at = at == D - 1 ? 0 : at + 1;
         }
-        // ---- the waves' sums meet in LDS.  W4: the lane holds rows 4 kb + r of columns 4 cg + t; else (weights were the
-        // row operand) row cg of columns 16 t + 4 kb + r
-        float* mine = red + wave * (16 * RT * 64);
+#pragma unroll 1
+        for (; u < u1; ++u) {
+            // (the last D units: the counter cannot tell them apart by one constant)
+            if (D > 2 && u + 2 < u1) wait_vmcnt_s<(D - 1) * OPS>();
+            else if (u + 1 < u1) wait_vmcnt_s<OPS>();
+            else wait_vmcnt_s<0>();
+            unit(ring + at * SH::SLOT, []() __attribute__((always_inline)) {});
+            at = at == D - 1 ? 0 : at + 1;
+        }
+        __syncthreads();  // every ring is done
+
+        // ---- the waves' sums.  W4: the lane holds rows 4 kb + r of columns 4 cg + t; else (weights were the row operand)
+        // row cg of columns 16 t + 4 kb + r
+        float* mine = red + wave * (16 * WC);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (FMT == kEW4)
-                    *(float4_t*)(mine + (16 * rt + 4 * kb + i) * 64 + 4 * cg) = float4_t{acc[rt][0][i], acc[rt][1][i], acc[rt][2][i], acc[rt][3][i]};
-                else
-                    *(float4_t*)(mine + (16 * rt + cg) * 64 + 16 * i + 4 * kb) = acc[rt][i];
-            }
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (FMT == kEW4)
+                *(float4_t*)(mine + (4 * kb + i) * WC + 4 * cg) = float4_t{acc[0][i], acc[1][i], acc[2][i], acc[3][i]};
+            else if (i < NT)
+                *(float4_t*)(mine + cg * WC + 16 * i + 4 * kb) = acc[i < NT ? i : 0];
+        }
+    } else {
+        __syncthreads();
     }
     __syncthreads();
 
@@ -298,28 +325,24 @@ __global__ __launch_bounds__(NW * 64) void experts_stream_kernel(ExpertArgs a) {
         float4_t v = float4_t{0.f, 0.f, 0.f, 0.f};
         if (none) return v;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) v += *(const float4_t*)(red + w * (16 * RT * 64) + row * 64 + c);
-        if (a.bias != nullptr && split == 0) {
-            const float* b = a.bias + (int64_t)tile.expert * a.N + unit_column<64>(a.half, ct, c);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] += b[i];
-        }
+        for (int w = 0; w < NW; ++w) v += *(const float4_t*)(red + w * (16 * WC) + row * WC + c);
+        if (a.bias != nullptr && split == 0) v += *(const float4_t*)(a.bias + (int64_t)tile.expert * a.N + unit_column<WC>(a.half, ct, c));
         return v;
     };
     const bool pairs = a.half != 0 && !a.to_partials;
-    const int per_row = pairs ? 8 : 16, width = a.half ? a.half : a.N;
-    for (int i = tid; i < 16 * RT * per_row; i += NW * 64) {
+    const int per_row = pairs ? WC / 8 : WC / 4, width = a.half ? a.half : a.N;
+    for (int i = tid; i < MR * per_row; i += NW * 64) {
         const int row = i / per_row, c = (i % per_row) * 4;
         const int r = tile.row0 + row;
-        const int in_half = a.half ? ct * 32 + (c & 31) : ct * 64 + c;
+        const int in_half = a.half ? ct * (WC / 2) + (c % (WC / 2)) : ct * WC + c;
         if (r >= tile.row_end || in_half >= width) continue;  // N (half) is a multiple of 8: whole vectors
         float4_t v = total(row, c);
         if (a.to_partials) {
-            *(float4_t*)(a.partials + ((int64_t)split * a.R + r) * a.N + unit_column<64>(a.half, ct, c)) = v;
+            *(float4_t*)(a.partials + ((int64_t)split * a.R + r) * a.N + unit_column<WC>(a.half, ct, c)) = v;
             continue;
         }
         if (pairs) {
-            const float4_t up = total(row, c + 32);
+            const float4_t up = total(row, c + WC / 2);
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] = silu_mul(v[j], up[j]);
         }
@@ -327,53 +350,51 @@ __global__ __launch_bounds__(NW * 64) void experts_stream_kernel(ExpertArgs a) {
     }
 }
 
-template <int FMT, bool BF16, int RT, int FU, bool QX = false>
+template <int FMT, bool BF16, int MR, int FU>
 int launch_one(const ExpertArgs& a, hipStream_t stream) {
-    constexpr int NW = 8, D = 3;
-    const int64_t tiles = max_row_tiles(a.R, a.E, 16 * RT);
+    using SH = StreamShape<FMT, MR, FU>;
+    static_assert(SH::LDS <= 160 * 1024 && SH::D * SH::OPS < 64, "ring does not fit LDS or the counter");
+    static_assert(SH::D == 2 || SH::D == 3, "waits of the last units");
+    const int64_t tiles = max_row_tiles(a.R, a.E, MR);
     if (tiles > 65535 || a.S > 65535) {
         set_error("experts: %lld row tiles exceed the grid", (long long)tiles);
         return GLA_ERR_INVALID_ARGUMENT;
     }
-    const int lds = NW * 16 * RT * 64 * 4;
-    const auto kernel = experts_stream_kernel<FMT, BF16, RT, FU, NW, D, QX>;
+    const auto kernel = experts_stream_kernel<FMT, BF16, MR, FU>;
     static DeviceOnce once;
     if (once.first()) {
-        const int rc = check_hip(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds), "hipFuncSetAttribute");
+        const int rc = check_hip(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, SH::LDS), "hipFuncSetAttribute");
         if (rc != GLA_OK) return rc;
     }
-    const int tiles_n = a.half ? (a.half + 31) / 32 : (a.N + 63) / 64;
-    kernel<<<dim3(tiles_n, (unsigned)tiles, a.S), NW * 64, lds, stream>>>(a);
+    const int cols = a.half ? SH::WC / 2 : SH::WC, width = a.half ? a.half : a.N;
+    kernel<<<dim3((width + cols - 1) / cols, (unsigned)tiles, a.S), SH::NW * 64, SH::LDS, stream>>>(a);
     return check_hip(hipGetLastError(), "experts_stream");
 }
 
-template <int FMT, bool BF16, int RT>
+template <int FMT, bool BF16, int MR>
 int launch_fold(const ExpertArgs& a, hipStream_t stream) {
     if constexpr (FMT == kEW4) {
-        if (a.group % 128 == 0) return launch_one<FMT, BF16, RT, 128>(a, stream);
-        if (a.group % 64 == 0) return launch_one<FMT, BF16, RT, 64>(a, stream);
-        return launch_one<FMT, BF16, RT, 32>(a, stream);
-    } else if constexpr (FMT == kEF8) {
-        if (a.scales_x == nullptr) return launch_one<FMT, BF16, RT, 128, true>(a, stream);
-        return launch_one<FMT, BF16, RT, 128>(a, stream);
+        if (a.group % 128 == 0) return launch_one<FMT, BF16, MR, 128>(a, stream);
+        if (a.group % 64 == 0) return launch_one<FMT, BF16, MR, 64>(a, stream);
+        return launch_one<FMT, BF16, MR, 32>(a, stream);
     } else {
-        return launch_one<FMT, BF16, RT, 64>(a, stream);
+        return launch_one<FMT, BF16, MR, 128>(a, stream);
     }
 }
 
 template <int FMT>
-int launch_format(const ExpertArgs& a, bool bf16, int row_tiles, hipStream_t stream) {
-    if (bf16) return row_tiles > 1 ? launch_fold<FMT, true, 2>(a, stream) : launch_fold<FMT, true, 1>(a, stream);
-    return row_tiles > 1 ? launch_fold<FMT, false, 2>(a, stream) : launch_fold<FMT, false, 1>(a, stream);
+int launch_format(const ExpertArgs& a, bool bf16, int rows, hipStream_t stream) {
+    if (bf16) return rows > 4 ? launch_fold<FMT, true, 16>(a, stream) : launch_fold<FMT, true, 4>(a, stream);
+    return rows > 4 ? launch_fold<FMT, false, 16>(a, stream) : launch_fold<FMT, false, 4>(a, stream);
 }
 
 }  // namespace
 
-int launch_experts_stream(const ExpertArgs& a, int format, bool bf16, int row_tiles, hipStream_t stream) {
+int launch_experts_stream(const ExpertArgs& a, int format, bool bf16, int rows, hipStream_t stream) {
     switch (format) {
-        case kEW4: return launch_format<kEW4>(a, bf16, row_tiles, stream);
-        case kEF8: return launch_format<kEF8>(a, bf16, row_tiles, stream);
-        default: return launch_format<kE16>(a, bf16, row_tiles, stream);
+        case kEW4: return launch_format<kEW4>(a, bf16, rows, stream);
+        case kEF8: return launch_format<kEF8>(a, bf16, rows, stream);
+        default: return launch_format<kE16>(a, bf16, rows, stream);
     }
 }
 

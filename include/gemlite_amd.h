@@ -376,7 +376,7 @@ typedef struct gla_experts_args {
     int32_t input_dtype, output_dtype, meta_dtype; /* input_dtype FP8: x is quantised first, see below */
     int32_t x_dtype;       /* of x, fp16 or bf16: the output type */
     int32_t channel_scale_mode, W_group_mode;
-    int32_t tile_config;   /* -1: the library chooses; else rows per tile (16, 32: streaming kernel; 64, 128, 256: tiled
+    int32_t tile_config;   /* -1: the library chooses; else rows per tile (4, 16: streaming kernel; 64, 128, 256: tiled
                               GEMM) + 1000 * K splits (0: the library's number; streaming kernel only) */
 } gla_experts_args;
 

@@ -293,7 +293,7 @@ def test_bias(fmt, dtype):
         run_case(fmt, dtype, 4, T, 2, 256, 160, drop=0.2, bias=True)
 
 
-TILES = [16, 32, 2016, 3032, 64, 128, 256]
+TILES = [4, 16, 2016, 3004, 64, 128, 256]
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
