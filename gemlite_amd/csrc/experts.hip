@@ -83,8 +83,8 @@ int validate(const gla_experts_args* p) {
         return GLA_ERR_UNSUPPORTED_MODE;
     }
     const bool combined = p->mode == GLA_EXPERTS_COMBINED, gated = p->mode == GLA_EXPERTS_GATED;
-    if (p->R < 0 || p->T < 0 || p->E <= 0 || p->E > GLA_EXPERTS_MAX || p->N <= 0 || p->K <= 0) {
-        set_error("experts: R=%d T=%d E=%d (1..%d) N=%d K=%d", p->R, p->T, p->E, GLA_EXPERTS_MAX, p->N, p->K);
+    if (p->R < 0 || p->T < 0 || p->E <= 0 || p->E > GLA_EXPERTS_MAX || p->N <= 0 || p->K <= 0 || p->K > (1 << 20)) {
+        set_error("experts: R=%d T=%d E=%d (1..%d) N=%d K=%d (at most 2^20)", p->R, p->T, p->E, GLA_EXPERTS_MAX, p->N, p->K);
         return GLA_ERR_INVALID_ARGUMENT;
     }
     if (p->output_dtype != GLA_DT_FP16 && p->output_dtype != GLA_DT_BF16) {
@@ -158,8 +158,8 @@ int validate(const gla_experts_args* p) {
             set_error("experts: W_group_mode %d of 4-bit codes (scale, shift and scale, fma are built)", p->W_group_mode);
             return GLA_ERR_UNSUPPORTED_MODE;
         }
-        if (p->meta_dtype != GLA_DT_FP16 && p->meta_dtype != GLA_DT_BF16) {
-            set_error("experts: scales of type %d (fp16 and bf16 are built)", p->meta_dtype);
+        if (p->meta_dtype != p->x_dtype) {
+            set_error("experts: scales of type %d with activations of type %d (they have to be the same)", p->meta_dtype, p->x_dtype);
             return GLA_ERR_UNSUPPORTED_DTYPE;
         }
         if (p->R > 0 && (!p->scales || (p->W_group_mode != GLA_WGM_SCALE && !p->zeros))) {
@@ -244,7 +244,11 @@ int gla_experts_matmul(const gla_experts_args* p, void* stream) {
     a.S = h.S;
     a.to_partials = h.to_partials;
     a.group = p->group_size;
-    a.meta_bf16 = p->meta_dtype == GLA_DT_BF16;
+    a.groups = h.format == kEW4 ? p->K / p->group_size : 0;
+    a.group_mul = divide_mul(h.format == kEW4 ? p->group_size / 32 : 1);
+    a.top_k_mul = divide_mul(p->top_k);
+    const int waves = 4 * h.S, units = (p->K + 127) / 128;  // of the streaming kernel
+    a.chunk = (units + waves - 1) / waves;
     a.c1 = p->W_group_mode == GLA_WGM_FMA ? 1.0f : 0.0f;
     a.c2 = p->W_group_mode == GLA_WGM_SHIFT_SCALE ? -1.0f : 0.0f;
     hipStream_t s = (hipStream_t)stream;

@@ -159,7 +159,7 @@ __global__ __launch_bounds__(512) void experts_gemm_kernel(ExpertArgs a, int til
         }
         m_dst = M_OFF + q * 256;
     }
-    const int groups = W4 ? a.K / a.group : 0;
+    const int groups = a.groups;
     const unsigned char* zero_chunk = g_zero_chunk;
     asm volatile("" : "+s"(zero_chunk));  // its address stays in registers
     typedef const __attribute__((address_space(1))) void* gptr;
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(512) void experts_gemm_kernel(ExpertArgs a, int til
                 __builtin_amdgcn_global_load_lds((gptr)(b_base + (b_off[i] + chunk)), (lptr)(base + B_OFF + (wave + 8 * i) * 1024), 16, 0, 0);
             }
         } else if constexpr (W4) {
-            int g = (k * 64 + m_half * 32) / a.group;
+            int g = (int)divide_by((uint32_t)(k * 2 + m_half), a.group_mul);
             if (g > groups - 1) g = groups - 1;
             __builtin_amdgcn_global_load_lds((gptr)(m_src + (int64_t)g * a.N * 2 + m_off), (lptr)(base + m_dst), 4, 0, 0);
         } else if constexpr (F8) {
@@ -330,8 +330,8 @@ __global__ __launch_bounds__(512) void experts_gemm_kernel(ExpertArgs a, int til
         auto convert_meta = [&](int h) __attribute__((always_inline)) {
 #pragma unroll
             for (int j = 0; j < TJ; ++j) {
-                const float s = a.meta_bf16 ? bf16_bits_to_float((uint16_t)raw_s[h][j]) : half_bits_to_float((uint16_t)raw_s[h][j]);
-                float z = a.meta_bf16 ? bf16_bits_to_float((uint16_t)raw_z[h][j]) : half_bits_to_float((uint16_t)raw_z[h][j]);
+                const float s = low16<BF16>(raw_s[h][j]);
+                float z = low16<BF16>(raw_z[h][j]);
                 z = a.zeros == nullptr ? 0.0f : z * __builtin_fmaf(a.c2, s, a.c1);
                 meta[h][j] = make_meta<BF16, 0>(s, z);
             }

@@ -60,20 +60,23 @@ struct StreamShape {
     static constexpr int WC = FMT == kE16 ? 32 : 64;
     static constexpr int NT = WC / 16;
     static constexpr int FOLDS = 128 / FU;
-    static constexpr int W_OPS = FMT == kEW4 ? 4 : 8, X_OPS = MR / 4, M_OPS = FMT == kEW4 ? FOLDS : (FMT == kEF8 ? 1 : 0);
-    static constexpr int OPS = W_OPS + X_OPS + M_OPS;
-    static constexpr int W_BYTES = W_OPS * 1024, X_BYTES = X_OPS * 1024, SLOT = W_BYTES + X_BYTES + M_OPS * 256;
+    static constexpr int W_OPS = FMT == kEW4 ? 4 : 8, M_OPS = FMT == kEW4 ? FOLDS : (FMT == kEF8 ? 1 : 0);
+    static constexpr int W_BYTES = W_OPS * 1024;
     static constexpr int NW = 4;
-    static constexpr int D = FMT == kEW4 && MR == 4 ? 3 : 2;
-    static constexpr int RING = D * SLOT;                     // per wave
-    static constexpr int LDS = NW * (RING > 16 * WC * 4 ? RING : 16 * WC * 4);
+    // XO: activation copies per unit, 4 rows each
+    static constexpr int ops(int xo) { return W_OPS + xo + M_OPS; }
+    static constexpr int slot(int xo) { return W_BYTES + xo * 1024 + M_OPS * 256; }
+    static constexpr int depth(int xo) { return FMT == kEW4 && xo <= 2 ? 3 : 2; }
+    static constexpr int ring(int xo) { return depth(xo) * slot(xo); }
+    static constexpr int most(int a, int b) { return a > b ? a : b; }
+    static constexpr int RING = most(ring(MR / 4), most(ring(1), MR > 4 ? ring(2) : 0));  // per wave
+    static constexpr int LDS = NW * most(RING, 16 * WC * 4);
 };
 
 template <int FMT, bool BF16, int MR, int FU>
 __global__ __launch_bounds__(256) void experts_stream_kernel(ExpertArgs a) {
     using SH = StreamShape<FMT, MR, FU>;
-    constexpr int WC = SH::WC, NT = SH::NT, NW = SH::NW, D = SH::D, OPS = SH::OPS;
-    constexpr int X_OFF = SH::W_BYTES, M_OFF = X_OFF + SH::X_BYTES;
+    constexpr int WC = SH::WC, NT = SH::NT, NW = SH::NW;
 
     extern __shared__ __align__(16) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -84,21 +87,23 @@ __global__ __launch_bounds__(256) void experts_stream_kernel(ExpertArgs a) {
     if (tile.expert < 0) return;
     float* red = (float*)smem;  // [NW][16][WC], when the ring is done
 
-    if (tile.expert < a.E) {
+    // the K loop for a tile of up to 4 XO rows: only rows that are there are copied
+    auto run = [&](auto xo_tag) __attribute__((always_inline)) {
+        constexpr int XO = decltype(xo_tag)::value, D = SH::depth(XO), OPS = SH::ops(XO), SLOT = SH::slot(XO);
+        constexpr int X_OFF = SH::W_BYTES, M_OFF = X_OFF + XO * 1024;
         unsigned char* ring = smem + wave * SH::RING;
         const unsigned char* we = a.w + (int64_t)tile.expert * a.w_stride_e;
         const unsigned char* se = a.scales + (int64_t)tile.expert * a.meta_stride_e;
         const unsigned char* ze = a.zeros == nullptr ? se : a.zeros + (int64_t)tile.expert * a.meta_stride_e;
         const int units = (a.K + 127) / 128;
-        const int slots = a.S * NW, slot_id = split * NW + wave;
-        const int u0 = (int)((int64_t)units * slot_id / slots), u1 = (int)((int64_t)units * (slot_id + 1) / slots);
+        const int u0 = (split * NW + wave) * a.chunk, u1 = u0 + a.chunk < units ? u0 + a.chunk : units;
 
         // ---- copy plan: a wave-uniform base that advances per unit plus 32-bit lane offsets; activation rows have
         // 64-bit addresses of their own
-        const unsigned char* x_src[SH::X_OPS];
-        int x_piece[SH::X_OPS];
+        const unsigned char* x_src[XO];
+        int x_piece[XO];
 #pragma unroll
-        for (int q = 0; q < SH::X_OPS; ++q) {
+        for (int q = 0; q < XO; ++q) {
             const int row = 4 * q + kb;
             int r = tile.row0 + row;
             if (r > tile.row_end - 1) r = tile.row_end - 1;  // multiplied, never stored
@@ -127,7 +132,7 @@ __global__ __launch_bounds__(256) void experts_stream_kernel(ExpertArgs a) {
         } else if constexpr (FMT == kEF8) {
             m_off = (uint32_t)(unit_column_inside<WC>(a.half, a.N, ct, lane & ~3) >> 7) * 4u;
         }
-        const int groups = FMT == kEW4 ? a.K / a.group : 0;
+        const int groups = a.groups;
         const int Kb = a.K * 2;
         const unsigned char* zero_piece = g_zero_piece;
         asm volatile("" : "+s"(zero_piece));
@@ -154,7 +159,7 @@ __global__ __launch_bounds__(256) void experts_stream_kernel(ExpertArgs a) {
                 }
             }
 #pragma unroll
-            for (int q = 0; q < SH::X_OPS; ++q) {
+            for (int q = 0; q < XO; ++q) {
                 const unsigned char* p = x_src[q] + (int64_t)u * 256;
                 if constexpr (FMT != kEF8) p = u * 256 + x_piece[q] < Kb ? p : zero_piece;
                 __builtin_amdgcn_global_load_lds((gptr)p, (lptr)(slot + X_OFF + q * 1024), 16, 0, 0);
@@ -162,7 +167,7 @@ __global__ __launch_bounds__(256) void experts_stream_kernel(ExpertArgs a) {
             if constexpr (FMT == kEW4) {
 #pragma unroll
                 for (int h = 0; h < SH::FOLDS; ++h) {
-                    int g = a.group == FU ? u * SH::FOLDS + h : (u * 128 + h * FU) / a.group;
+                    int g = (int)divide_by((uint32_t)(u * 4 + h * (FU / 32)), a.group_mul);
                     if (g > groups - 1) g = groups - 1;
                     __builtin_amdgcn_global_load_lds((gptr)(m_base + (int64_t)g * a.N * 2 + m_off), (lptr)(slot + M_OFF + h * 256), 4, 0, 0);
                 }
@@ -179,7 +184,7 @@ __global__ __launch_bounds__(256) void experts_stream_kernel(ExpertArgs a) {
         asm volatile("" : "+s"(mask), "+v"(magic));  // registers, so that v_and_or_b32 is selected
         const uint32_t one = BF16 ? 0x3f803f80u : 0x3c003c00u;
         const u32x4 ones = u32x4{one, one, one, one};
-        const int x_row = cg < MR ? cg : MR - 1;
+        const int x_row = cg < 4 * XO ? cg : 4 * XO - 1;
         auto x_at = [&](const unsigned char* slot, int piece) __attribute__((always_inline)) {
             return *(const u32x4*)(slot + X_OFF + x_row * 256 + ((piece ^ x_row) & 15) * 16);
         };
@@ -217,9 +222,8 @@ __global__ __launch_bounds__(256) void experts_stream_kernel(ExpertArgs a) {
                     }
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
-                        const uint32_t vs = rs[h][t / 2] >> (16 * (t & 1)), vz = rz[h][t / 2] >> (16 * (t & 1));
-                        const float sc = a.meta_bf16 ? bf16_bits_to_float((uint16_t)vs) : half_bits_to_float((uint16_t)vs);
-                        float zp = a.meta_bf16 ? bf16_bits_to_float((uint16_t)vz) : half_bits_to_float((uint16_t)vz);
+                        const float sc = t & 1 ? high16<BF16>(rs[h][t / 2]) : low16<BF16>(rs[h][t / 2]);
+                        float zp = t & 1 ? high16<BF16>(rz[h][t / 2]) : low16<BF16>(rz[h][t / 2]);
                         zp = a.zeros == nullptr ? 0.0f : zp * __builtin_fmaf(a.c2, sc, a.c1);
                         const float off = __builtin_fmaf(BF16 ? -128.0f : -1024.0f, sc, zp);
 #pragma unroll
@@ -281,12 +285,13 @@ __global__ __launch_bounds__(256) void experts_stream_kernel(ExpertArgs a) {
 
 #pragma unroll
         for (int d = 0; d < D; ++d)
-            if (u0 + d < u1) issue(u0 + d, ring + d * SH::SLOT);
+            if (u0 + d < u1) issue(u0 + d, ring + d * SLOT);
+        static_assert(D == 2 || D == 3, "waits of the last units");
         int u = u0, at = 0;
 #pragma unroll 1
         for (; u + D < u1; ++u) {
             wait_vmcnt_s<(D - 1) * OPS>();
-            unsigned char* slot = ring + at * SH::SLOT;
+            unsigned char* slot = ring + at * SLOT;
             unit(slot, [&]() __attribute__((always_inline)) {
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot has been read
                 issue(u + D, slot);
@@ -299,7 +304,7 @@ __global__ __launch_bounds__(256) void experts_stream_kernel(ExpertArgs a) {
             if (D > 2 && u + 2 < u1) wait_vmcnt_s<(D - 1) * OPS>();
             else if (u + 1 < u1) wait_vmcnt_s<OPS>();
             else wait_vmcnt_s<0>();
-            unit(ring + at * SH::SLOT, []() __attribute__((always_inline)) {});
+            unit(ring + at * SLOT, []() __attribute__((always_inline)) {});
             at = at == D - 1 ? 0 : at + 1;
         }
         __syncthreads();  // every ring is done
@@ -314,8 +319,13 @@ __global__ __launch_bounds__(256) void experts_stream_kernel(ExpertArgs a) {
             else if (i < NT)
                 *(float4_t*)(mine + cg * WC + 16 * i + 4 * kb) = acc[i < NT ? i : 0];
         }
-    } else {
-        __syncthreads();
+    };
+    if (tile.expert < a.E) {
+        const int rows = tile.row_end - tile.row0;
+        if constexpr (MR == 4) run(std::integral_constant<int, 1>{});
+        else if (rows <= 4) run(std::integral_constant<int, 1>{});
+        else if (rows <= 8) run(std::integral_constant<int, 2>{});
+        else run(std::integral_constant<int, 4>{});
     }
     __syncthreads();
 
@@ -353,8 +363,7 @@ __global__ __launch_bounds__(256) void experts_stream_kernel(ExpertArgs a) {
 template <int FMT, bool BF16, int MR, int FU>
 int launch_one(const ExpertArgs& a, hipStream_t stream) {
     using SH = StreamShape<FMT, MR, FU>;
-    static_assert(SH::LDS <= 160 * 1024 && SH::D * SH::OPS < 64, "ring does not fit LDS or the counter");
-    static_assert(SH::D == 2 || SH::D == 3, "waits of the last units");
+    static_assert(SH::LDS <= 160 * 1024 && 3 * SH::ops(4) < 64, "ring does not fit LDS or the counter");
     const int64_t tiles = max_row_tiles(a.R, a.E, MR);
     if (tiles > 65535 || a.S > 65535) {
         set_error("experts: %lld row tiles exceed the grid", (long long)tiles);

@@ -260,8 +260,9 @@ class GemLiteExperts(torch.nn.Module):
                 meta[2], meta[9], meta[10] = K, 0, 2 if wgm == 0 else 3
             elif csm != 0 or wgm not in (2, 3, 4):
                 raise NotImplementedError(f"4-bit experts with W_group_mode {wgm} and channel_scale_mode {csm} are not built")
-            if meta[2] % 32 != 0 or first.scales.dtype not in (torch.float16, torch.bfloat16):
-                raise NotImplementedError(f"4-bit experts with groups of {meta[2]} and scales of type {first.scales.dtype} are not built")
+            if meta[2] % 32 != 0 or first.scales.dtype != DTYPE_TO_TORCH[first.output_dtype.value]:
+                raise NotImplementedError(f"4-bit experts with groups of {meta[2]} and scales of type {first.scales.dtype} for outputs of type "
+                                          f"{first.output_dtype} are not built")
             W_q = torch.stack([layer.W_q.data.contiguous() for layer in layers])
             scales = torch.stack([layer.scales.data.contiguous() for layer in layers])
             zeros = none

@@ -353,7 +353,7 @@ typedef struct gla_experts_args {
     const void* x;         /* ROWS, COMBINED: [R, K] sorted by expert; GATED: [T, K].  fp16 / bf16 */
     const void* w;         /* [E] experts, w_stride_e bytes apart, each laid out as gla_matmul takes it: packed words
                               [K/8, N], or K-contiguous bytes / 16-bit values [N, K] */
-    const void* scales;    /* 4-bit: [E][K/group_size, N] fp16 / bf16; fp8: [E][K/128, ceil(N/128)] fp32; 16-bit: NULL */
+    const void* scales;    /* 4-bit: [E][K/group_size, N] of x's type; fp8: [E][K/128, ceil(N/128)] fp32; 16-bit: NULL */
     const void* zeros;     /* 4-bit: as scales (group modes 3 and 4), else NULL */
     const float* bias;     /* [E, N] or NULL */
     void* out;
