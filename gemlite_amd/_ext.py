@@ -5,7 +5,6 @@ The library is built in-tree by ``gemlite_amd/csrc/Makefile`` (or
 object is missing, or a call returns a non-zero status, the caller gets an
 exception.
 """
-import contextlib
 import ctypes
 import os
 import threading
@@ -171,7 +170,7 @@ SYMBOLS = {
         ctypes.c_int,
         [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_void_p],
     ),
-    "gla_route_workspace_bytes": (ctypes.c_int64, [ctypes.c_int, ctypes.c_int]),
+    "gla_route_workspace_bytes": (ctypes.c_int64, [ctypes.c_int, ctypes.c_int, ctypes.c_int]),
     "gla_route_experts": (
         ctypes.c_int,
         [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
@@ -572,60 +571,73 @@ def unpack_over_cols(packed: torch.Tensor, out: torch.Tensor, rows: int, pcols: 
 # ---------------------------------------------------------------------------
 # mixture of experts
 # ---------------------------------------------------------------------------
-def _on_device(device: torch.device):
-    """Makes ``device`` the current one for a launch (nothing to do where it is already)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+_ROUTE_WORKSPACE = {}  # (T, E, k) -> bytes
+
+
+def _route_need(T, E, k):
+    need = _ROUTE_WORKSPACE.get((T, E, k))
+    if need is None:
+        need = load_library().gla_route_workspace_bytes(T, E, k)
+        if need < 0:
+            _check(int(need), "gla_route_workspace_bytes")
+        if len(_ROUTE_WORKSPACE) > 4096:
+            _ROUTE_WORKSPACE.clear()
+        _ROUTE_WORKSPACE[(T, E, k)] = need
+    return need
+
+
+def _on_current_device(call, tensor):
+    """``call(stream)`` with ``tensor``'s device current and its current stream."""
+    index = tensor.device.index
+    if index == torch.cuda.current_device():
+        return call(torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return call(torch._C._cuda_getCurrentRawStream(index))
 
 
 def route_experts(logits, top_k, scoring, renormalize, scale, weights, ids, offsets, order, places):
-    _require_cuda(logits, weights, ids, offsets, order, places)
     lib = load_library()
     T, E = logits.shape
-    need = lib.gla_route_workspace_bytes(T, E)
-    if need < 0:
-        _check(int(need), "gla_route_workspace_bytes")
-    with _on_device(logits.device):
-        counts = torch.empty(need, dtype=torch.uint8, device=logits.device)
-        _check(
-            lib.gla_route_experts(
-                logits.data_ptr(), TORCH_TO_DTYPE[logits.dtype].value if logits.dtype in TORCH_TO_DTYPE else -1, logits.stride(0),
-                T, E, int(top_k), int(scoring), int(bool(renormalize)), float(scale), weights.data_ptr(), ids.data_ptr(),
-                offsets.data_ptr(), order.data_ptr(), places.data_ptr(), counts.data_ptr(), need, _stream_ptr(logits.device),
-            ),
-            "gla_route_experts",
-        )
+    dtype = TORCH_TO_DTYPE.get(logits.dtype)
+    need = _route_need(T, E, top_k)
+    counts = logits.new_empty(need, dtype=torch.uint8) if need else None
+    status = _on_current_device(lambda stream: lib.gla_route_experts(
+        logits.data_ptr(), -1 if dtype is None else dtype.value, logits.stride(0), T, E, top_k, scoring, renormalize, scale,
+        weights.data_ptr(), ids.data_ptr(), offsets.data_ptr(), order.data_ptr(), places.data_ptr(),
+        None if counts is None else counts.data_ptr(), need, stream), logits)
+    if status != GLA_OK:
+        _check(status, "gla_route_experts")
 
 
 def plan_experts(ids, num_experts, offsets, order, places):
-    _require_cuda(ids, offsets, order, places)
     lib = load_library()
     T, k = ids.shape
-    need = lib.gla_route_workspace_bytes(T, int(num_experts))
-    if need < 0:
-        _check(int(need), "gla_route_workspace_bytes")
-    with _on_device(ids.device):
-        counts = torch.empty(need, dtype=torch.uint8, device=ids.device)
-        _check(
-            lib.gla_plan_experts(ids.data_ptr(), T, int(num_experts), k, offsets.data_ptr(), order.data_ptr(), places.data_ptr(),
-                                 counts.data_ptr(), need, _stream_ptr(ids.device)),
-            "gla_plan_experts",
-        )
+    need = _route_need(T, int(num_experts), k)
+    counts = ids.new_empty(need, dtype=torch.uint8) if need else None
+    status = _on_current_device(lambda stream: lib.gla_plan_experts(
+        ids.data_ptr(), T, int(num_experts), k, offsets.data_ptr(), order.data_ptr(), places.data_ptr(),
+        None if counts is None else counts.data_ptr(), need, stream), ids)
+    if status != GLA_OK:
+        _check(status, "gla_plan_experts")
 
 
-def experts_matmul(args: ExpertsArgs, device: torch.device):
-    """Launch ``gla_experts_matmul`` on the current stream of ``device``.  Its workspace (fp32 rows, contents arbitrary)
-    comes from torch's allocator for this call, so calls on several streams or in several captured graphs share none."""
-    lib = load_library()
+def experts_workspace_need(args: ExpertsArgs) -> int:
     args.struct_size = ctypes.sizeof(ExpertsArgs)
-    ref = ctypes.byref(args)
-    need = lib.gla_experts_workspace_bytes(ref)
+    need = load_library().gla_experts_workspace_bytes(ctypes.byref(args))
     if need < 0:
         _check(int(need), "gla_experts_workspace_bytes")
-    with _on_device(device):
-        if need > 0:
-            workspace = torch.empty(need, dtype=torch.uint8, device=device)
-            args.workspace = workspace.data_ptr()
-            args.workspace_bytes = need
-        _check(lib.gla_experts_matmul(ref, _stream_ptr(device)), "gla_experts_matmul")
+    return int(need)
+
+
+def experts_matmul(args: ExpertsArgs, need: int, x: torch.Tensor):
+    """Launch ``gla_experts_matmul`` on the current stream of ``x``'s device.  Its workspace (``need`` bytes, contents
+    arbitrary) comes from torch's allocator for this call, so calls on several streams or in several captured graphs share
+    none."""
+    lib = load_library()
+    if need > 0:
+        workspace = x.new_empty(need, dtype=torch.uint8)
+        args.workspace = workspace.data_ptr()
+        args.workspace_bytes = need
+    status = _on_current_device(lambda stream: lib.gla_experts_matmul(ctypes.byref(args), stream), x)
+    if status != GLA_OK:
+        _check(status, "gla_experts_matmul")

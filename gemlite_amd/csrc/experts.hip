@@ -104,7 +104,7 @@ int validate(const gla_experts_args* p) {
     }
     if (p->tile_config != -1) {
         const int rows = p->tile_config % 1000, splits = p->tile_config / 1000;
-        if (p->tile_config < 0 || splits > 64 || (rows != 4 && rows != 16 && rows != 64 && rows != 128 && rows != 256) || (rows > 16 && splits > 1)) {
+        if (p->tile_config < 0 || splits > 64 || (rows != 4 && rows != 16 && rows != 64 && rows != 128 && rows != 256) ) {
             set_error("experts: tile_config %d", p->tile_config);
             return GLA_ERR_INVALID_ARGUMENT;
         }
@@ -173,20 +173,66 @@ int validate(const gla_experts_args* p) {
 struct ExpertPlanHost {
     int format;
     int bm;      // rows per tile: 4, 16 (streaming kernel), 64, 128, 256 (tiled GEMM)
-    int S;
+    int S, chunk;
     bool to_partials;
     bool quantise;                       // F8: a launch in front writes codes and scales to the workspace
     int64_t partial_bytes, code_bytes, total_bytes;  // of the workspace: fp32 rows, codes, scales
 };
 
+// Rows per tile from the mean rows per expert with any (the distribution itself is on the device).  Times in us, both sides
+// of each threshold, at the sizes named (E experts, k of them per token):
+//  * 4-bit, 4096 -> 2 x 14336, E = 8, k = 2: 16-row streaming tiles against 64-row ones at 8 rows per expert 116 / 170, at 16
+//    168 / 164, at 24 240 / 164; 64 against 128 rows at 32 rows per expert 177 / 201, at 64 236 / 229, at 100 352 / 261.
+//    256-row tiles leave one workgroup per CU, 128-row ones two: 1091 / 1014 at 512 rows per expert.
+//  * 16-bit, 4096^2, E = 16: 16 against 64 at 6 rows per expert 72 / 88, at 12 113 / 98; 64 against 128 at 28 112 / 116, at 57
+//    125 / 114.  Above, 128- and 256-row tiles cost 1.0 to 1.7 and run in rounds of one per CU: whichever needs less.
+//  * fp8: the streaming kernel quantises in every wave and needs long K ranges: 4096 -> 2 x 2048, E = 32, k = 4: 4 / 16 / 64 rows
+//    at 1 row per expert 57 / 66 / 73, at 4 109 / 93 / 119; 2048 -> 2 x 768, E = 128, k = 8 at 4 91 / 83 / 57; 768 -> 2048 at
+//    1 token 12.0 / 11.9 / 15.0, at 8 tokens 30 / 40 / 26.  64 against 128 at 62 rows per expert 119 / 121, at 125 168 / 147; 128
+//    against 256 at 250 151 / 174 and 232 / 222, at 512 449 / 404.
+int choose_rows(int format, int K, int64_t R, int64_t active, int64_t width_of_128) {
+    const int64_t per = active > 0 ? R / active : 0;
+    if (format == kEF8) {
+        if (K >= 4096 ? per <= 8 : per <= 1 && active * width_of_128 <= 256) return per > 2 ? 16 : 4;
+        return per <= 64 ? 64 : per <= 300 ? 128 : 256;
+    }
+    if (format == kE16) {
+        if (per <= 9) return per <= 2 ? 4 : 16;
+        if (per <= 32) return 64;
+        const int64_t wide = (width_of_128 + 1) / 2;
+        auto rounds = [&](int64_t bm) {
+            const int64_t partly = (R + bm * active / 2) / bm;  // tiles, if the last one of an expert is half full
+            return ((partly > active ? partly : active) * wide + 255) / 256;
+        };
+        return rounds(256) * 17 <= rounds(128) * 10 ? 256 : 128;
+    }
+    return per <= 16 ? 16 : per <= 48 ? 64 : 128;
+}
+
 ExpertPlanHost plan_of(const gla_experts_args& p) {
     ExpertPlanHost h;
     h.format = format_of(p);
     const int want_rows = p.tile_config < 0 ? 0 : p.tile_config % 1000, want_s = p.tile_config < 0 ? 0 : p.tile_config / 1000;
-    const int active = p.R < p.E ? p.R : p.E;
-    const int per = active > 0 ? p.R / active : 0;
-    h.bm = want_rows ? want_rows : (per > 160 ? 256 : per > 64 ? 128 : per > 8 ? 64 : per > 2 ? 16 : 4);
-    h.S = want_s > 0 ? want_s : 1;
+    const int64_t active = p.R < p.E ? p.R : p.E;
+    // workgroups side by side for BN columns of weights (gated: half of them from either half)
+    auto across = [&](int bn) { return (int64_t)(p.N + bn - 1) / bn; };
+    h.bm = want_rows ? want_rows : choose_rows(h.format, p.K, p.R, active, across(128));
+    if (h.format == kEW4) h.bm = h.bm == 4 ? 16 : h.bm == 256 ? 128 : h.bm;  // (not built for 4-bit weights: never better)
+    // K splits until every CU has work: a finishing launch adds them (combined calls have one anyway; others split only
+    // where that leaves most of the chip empty)
+    const int steps = (p.K + 127) / 128;
+    const bool stream = h.bm <= 16;
+    const int64_t tiles = stream ? active * across(h.format == kE16 ? 32 : 64)
+                                 : (p.R / h.bm + active) * across(h.bm == 64 && h.format != kEW4 ? 128 : 256);
+    const int64_t enough = stream ? 256 : h.format == kEW4 ? 768 : h.bm == 64 ? 384 : 192;
+    int s = 1;
+    while (tiles * s < enough && s < 8 && steps >= 16 * s) s *= 2;
+    if (p.mode != GLA_EXPERTS_COMBINED && (s < 4 || tiles > 96)) s = 1;
+    h.S = want_s > 0 ? want_s : s;
+    const int unit = stream || h.format == kEF8 ? 128 : 64, parts = stream ? 4 * h.S : h.S;
+    const int n_units = (p.K + unit - 1) / unit;
+    h.chunk = (n_units + parts - 1) / parts;
+    if (!stream) h.S = (n_units + h.chunk - 1) / h.chunk;  // every split has a stage
     h.to_partials = p.mode == GLA_EXPERTS_COMBINED || h.S > 1;
     h.partial_bytes = h.to_partials ? (int64_t)h.S * p.R * p.N * 4 : 0;
     const int64_t rows = p.mode == GLA_EXPERTS_GATED ? p.T : p.R;
@@ -247,8 +293,7 @@ int gla_experts_matmul(const gla_experts_args* p, void* stream) {
     a.groups = h.format == kEW4 ? p->K / p->group_size : 0;
     a.group_mul = divide_mul(h.format == kEW4 ? p->group_size / 32 : 1);
     a.top_k_mul = divide_mul(p->top_k);
-    const int waves = 4 * h.S, units = (p->K + 127) / 128;  // of the streaming kernel
-    a.chunk = (units + waves - 1) / waves;
+    a.chunk = h.chunk;
     a.c1 = p->W_group_mode == GLA_WGM_FMA ? 1.0f : 0.0f;
     a.c2 = p->W_group_mode == GLA_WGM_SHIFT_SCALE ? -1.0f : 0.0f;
     hipStream_t s = (hipStream_t)stream;
@@ -277,11 +322,17 @@ int gla_experts_matmul(const gla_experts_args* p, void* stream) {
     return check_hip(hipGetLastError(), "experts_finish");
 }
 
-static int check_route(int64_t T, int E, int top_k, const void* ids, const void* offsets, const void* order, const void* places) {
+static int check_route_sizes(int64_t T, int E, int top_k) {
     if (T < 0 || E <= 0 || E > GLA_EXPERTS_MAX || top_k <= 0 || top_k > 64 || T * top_k >= ((int64_t)1 << 31)) {
         set_error("route: T=%lld E=%d (1..%d) top_k=%d (1..64)", (long long)T, E, GLA_EXPERTS_MAX, top_k);
         return GLA_ERR_INVALID_ARGUMENT;
     }
+    return GLA_OK;
+}
+
+static int check_route(int64_t T, int E, int top_k, const void* ids, const void* offsets, const void* order, const void* places) {
+    const int rc = check_route_sizes(T, E, top_k);
+    if (rc != GLA_OK) return rc;
     if (offsets == nullptr || (T > 0 && (ids == nullptr || order == nullptr || places == nullptr))) {
         set_error("route: NULL pointer");
         return GLA_ERR_INVALID_ARGUMENT;
@@ -289,17 +340,14 @@ static int check_route(int64_t T, int E, int top_k, const void* ids, const void*
     return GLA_OK;
 }
 
-int64_t gla_route_workspace_bytes(int T, int E) {
-    if (T < 0 || E <= 0 || E > GLA_EXPERTS_MAX) {
-        set_error("route: T=%d E=%d (1..%d)", T, E, GLA_EXPERTS_MAX);
-        return GLA_ERR_INVALID_ARGUMENT;
-    }
-    return (int64_t)(E + 1) * route_blocks(T) * 4;
+int64_t gla_route_workspace_bytes(int T, int E, int top_k) {
+    const int rc = check_route_sizes(T, E, top_k);
+    return rc != GLA_OK ? rc : route_counts(T, E, top_k) * 4;
 }
 
-static int check_counts(int T, int E, const void* workspace, int64_t bytes) {
-    const int64_t need = gla_route_workspace_bytes(T, E);
-    if (workspace == nullptr || bytes < need || !aligned(workspace, 16)) {
+static int check_counts(int T, int E, int top_k, const void* workspace, int64_t bytes) {
+    const int64_t need = route_counts(T, E, top_k) * 4;
+    if (need > 0 && (workspace == nullptr || bytes < need || !aligned(workspace, 16))) {
         set_error("route: a 16-byte aligned workspace of %lld bytes required, %lld given", (long long)need, (long long)bytes);
         return GLA_ERR_WORKSPACE_TOO_SMALL;
     }
@@ -323,7 +371,7 @@ int gla_route_experts(const void* logits, int dtype, int64_t stride, int T, int 
         set_error("route: NULL pointer, or rows %lld apart with %d logits", (long long)stride, E);
         return GLA_ERR_INVALID_ARGUMENT;
     }
-    if ((rc = check_counts(T, E, workspace, workspace_bytes)) != GLA_OK) return rc;
+    if ((rc = check_counts(T, E, top_k, workspace, workspace_bytes)) != GLA_OK) return rc;
     return launch_route(logits, T > 0 ? dtype : GLA_DT_FP32, stride, T, E, top_k, scoring == GLA_SCORING_SIGMOID, renormalize, scale, weights, ids,
                         offsets, order, places, (int32_t*)workspace, (hipStream_t)stream);
 }
@@ -332,7 +380,7 @@ int gla_plan_experts(const int32_t* ids, int T, int E, int top_k, int32_t* offse
                      int64_t workspace_bytes, void* stream) {
     int rc = check_route(T, E, top_k, ids, offsets, order, places);
     if (rc != GLA_OK) return rc;
-    if ((rc = check_counts(T, E, workspace, workspace_bytes)) != GLA_OK) return rc;
+    if ((rc = check_counts(T, E, top_k, workspace, workspace_bytes)) != GLA_OK) return rc;
     return launch_route(nullptr, 0, 0, T, E, top_k, 0, 0, 1.0f, nullptr, const_cast<int32_t*>(ids), offsets, order, places, (int32_t*)workspace,
                         (hipStream_t)stream);
 }

@@ -35,7 +35,7 @@ struct ExpertArgs {
     int group;                      // W4: K-values per group (scales and zeros have the activations' type)
     uint32_t group_mul, top_k_mul;  // n / (group / 32) and n / top_k as the high half of n * this (0: see divide_by)
     int groups;                     // W4: K / group
-    int chunk;                      // streaming kernel: units of 128 K-values per wave
+    int chunk;                      // streaming kernel: units of 128 K-values per wave; tiled GEMM: stages per split
     float c1, c2;                   // W4: zero-point term of a weight = zero * (c1 + c2 * scale)
 };
 
@@ -158,10 +158,18 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     else return pack_half2(lo, hi);
 }
 
-// The scale and the reciprocal that a block of 128 activations of amax is quantised with.  (The constant's reciprocal, not
-// a division: the codes of values that lie on a border between two depend on it.)
+// Larger magnitudes of two pairs of fp16 / bf16 values, as 15-bit integers (their order is the values', NaN above infinity:
+// a NaN is never lost).
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t magnitude_max(uint32_t m, uint32_t v) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m), __builtin_bit_cast(u16x2, v & 0x7fff7fffu)));
+}
+
+// The scale and the reciprocal that a block of 128 activations of amax is quantised with (NaN if it holds one).  (The
+// constant's reciprocal, not a division: the codes of values that lie on a border between two depend on it.)
 __device__ __forceinline__ void block_scale(float amax, float& s, float& inv) {
-    s = fmaxf(amax * (1.0f / 448.0f), 1e-6f);
+    s = amax * (1.0f / 448.0f);
+    s = s < 1e-6f ? 1e-6f : s;
     inv = 1.0f / s;
 }
 
@@ -189,8 +197,8 @@ int launch_experts_quantise(const void* x, bool bf16, int64_t xsm, int rows, int
 int launch_experts_stream(const ExpertArgs& a, int format, bool bf16, int rows, hipStream_t stream);
 int launch_experts_gemm(const ExpertArgs& a, int format, bool bf16, int bm, hipStream_t stream);
 
-// logits NULL: the ids are given and only sorted.  counts: (E + 1) * route_blocks(T) integers of scratch.
-int route_blocks(int T);
+// logits NULL: the ids are given and only sorted.  counts: route_counts() integers of scratch.
+int64_t route_counts(int T, int E, int top_k);
 int launch_route(const void* logits, int dtype, int64_t stride, int T, int E, int top_k, int sigmoid, int renormalize, float scale,
                  float* weights, int32_t* ids, int32_t* offsets, int32_t* order, int32_t* places, int32_t* counts, hipStream_t stream);
 

@@ -28,11 +28,12 @@ __global__ __launch_bounds__(256) void experts_quantise_kernel(const unsigned ch
         f[2 * i] = low16<BF16>(v[i]);
         f[2 * i + 1] = high16<BF16>(v[i]);
     }
-    float amax = 0.0f;
+    uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(f[i]));
+    for (int i = 0; i < 4; ++i) m = magnitude_max(m, v[i]);
 #pragma unroll
-    for (int m = 1; m < 16; m <<= 1) amax = fmaxf(amax, wave_xor(amax, m));
+    for (int x = 1; x < 16; x <<= 1) m = magnitude_max(m, wave_xor(m, x));
+    const float amax = low16<BF16>((m & 0xffffu) > (m >> 16) ? m & 0xffffu : m >> 16);
     float s, inv;
     block_scale(amax, s, inv);
     *(u32x2*)(codes + row * K + k) = u32x2{quantise4(f[0], f[1], f[2], f[3], inv), quantise4(f[4], f[5], f[6], f[7], inv)};

@@ -6,7 +6,7 @@
 //   order      flat indices token * k + slot, sorted by expert, within an expert in rising order; slots without an expert
 //              come last.  offsets[e] is where expert e's begin; places is the inverse of order
 //
-// A wave per token: lane l holds logits l, l + 64, ...; each of the k rounds is one wave-wide maximum and one wave-wide
+// A wave per token (32 tokens and 16 waves to a workgroup): lane l holds logits l, l + 64, ...; each of the k rounds is one wave-wide maximum and one wave-wide
 // minimum of the indices that have it (DPP, no LDS).  Up to kSmallSlots (token, slot) pairs one workgroup does everything
 // in one launch.  Above, a first launch selects and counts each block's slots per expert, and a second one sorts: every
 // block adds up the counts of the blocks in front of it for itself (they are a few kilobytes in L2), so no third launch
@@ -21,6 +21,7 @@ namespace {
 constexpr int kSmallSlots = 1024;
 constexpr int kMaxBlocks = 256;
 constexpr int kMinTokens = 32;  // tokens per block, at least
+constexpr int kThreads = 1024;
 
 struct RouteArgs {
     const void* logits;  // NULL: ids are given
@@ -207,58 +208,55 @@ __global__ __launch_bounds__(1024) void route_small_kernel(RouteArgs a, int bits
 
 // Block b: selects for its tokens (or reads their ids) and counts them per class.
 template <int DT, int V>
-__global__ __launch_bounds__(256) void route_select_kernel(RouteArgs a) {
+__global__ __launch_bounds__(kThreads) void route_select_kernel(RouteArgs a) {
     extern __shared__ int lds[];  // [classes]
     const int classes = a.E + 1, b = blockIdx.x;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int e = threadIdx.x; e < classes; e += 256) lds[e] = 0;
+    for (int e = threadIdx.x; e < classes; e += kThreads) lds[e] = 0;
     __syncthreads();
     const int64_t t0 = (int64_t)b * a.tokens;
     const int64_t t1 = t0 + a.tokens < a.T ? t0 + a.tokens : a.T;
     if constexpr (DT >= 0) {
-        for (int64_t t = t0 + wave; t < t1; t += 4) {
+        for (int64_t t = t0 + wave; t < t1; t += kThreads / 64) {
             const int id = select_token<DT, V>(a, (int)t);
             if (lane < a.k) atomicAdd(&lds[class_of(id, a.E)], 1);
         }
     } else {
-        for (int64_t i = t0 * a.k + threadIdx.x; i < t1 * a.k; i += 256) atomicAdd(&lds[class_of(a.ids[i], a.E)], 1);
+        for (int64_t i = t0 * a.k + threadIdx.x; i < t1 * a.k; i += kThreads) atomicAdd(&lds[class_of(a.ids[i], a.E)], 1);
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < classes; e += 256) a.counts[(int64_t)e * a.blocks + b] = lds[e];
+    for (int e = threadIdx.x; e < classes; e += kThreads) a.counts[(int64_t)e * a.blocks + b] = lds[e];
 }
 
 // Block b: where its slots go.
-__global__ __launch_bounds__(256) void route_sort_kernel(RouteArgs a, int bits) {
+__global__ __launch_bounds__(kThreads) void route_sort_kernel(RouteArgs a, int bits) {
     extern __shared__ int lds[];
+    constexpr int WAVES = kThreads / 64;
     const int classes = a.E + 1, b = blockIdx.x;
     int* totals = lds;             // [classes]: all slots of the class, then where the class begins
     int* next = lds + classes;     // [classes]: of this class in the blocks in front, then the next free place
-    int* counts = next + classes;  // [4][classes]
+    int* counts = next + classes;  // [WAVES][classes]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (int i = tid; i < 4 * classes; i += 256) counts[i] = 0;
-    for (int e = tid; e < classes; e += 256) {
-        const int4* c = (const int4*)(a.counts + (int64_t)e * a.blocks);  // blocks is a multiple of 4
-        int all = 0, front = 0;
-#pragma unroll 8
-        for (int i = 0; i < a.blocks / 4; ++i) {
-            const int4 v = c[i];
-            all += v.x + v.y + v.z + v.w;
-            front += (4 * i < b ? v.x : 0) + (4 * i + 1 < b ? v.y : 0) + (4 * i + 2 < b ? v.z : 0) + (4 * i + 3 < b ? v.w : 0);
-        }
-        totals[e] = all;
-        next[e] = front;
+    for (int i = tid; i < WAVES * classes; i += kThreads) counts[i] = 0;
+    // a wave per class: lane l has the counts of blocks 4 l .. 4 l + 3 (at most 256 blocks, a multiple of 4)
+    for (int e = wave; e < classes; e += WAVES) {
+        int4 v = int4{0, 0, 0, 0};
+        if (4 * lane < a.blocks) v = *(const int4*)(a.counts + (int64_t)e * a.blocks + 4 * lane);
+        const int upto = wave_inclusive_sum(v.x + v.y + v.z + v.w);
+        if (lane == 63) totals[e] = upto;
+        if (lane == b >> 2) next[e] = upto - (v.x + v.y + v.z + v.w) + ((b & 3) > 0 ? v.x : 0) + ((b & 3) > 1 ? v.y : 0) + ((b & 3) > 2 ? v.z : 0);
     }
     __syncthreads();
     scan_classes(totals, classes);
     __syncthreads();
-    for (int e = tid; e < classes; e += 256) {
+    for (int e = tid; e < classes; e += kThreads) {
         if (b == 0) a.offsets[e] = totals[e];
         next[e] += totals[e];
     }
     __syncthreads();
     const int64_t t0 = (int64_t)b * a.tokens;
     const int64_t t1 = t0 + a.tokens < a.T ? t0 + a.tokens : a.T;
-    for (int64_t i0 = t0 * a.k; i0 < t1 * a.k; i0 += 256) {
+    for (int64_t i0 = t0 * a.k; i0 < t1 * a.k; i0 += kThreads) {
         const int64_t i = i0 + tid;
         const int cls = i < t1 * a.k ? class_of(a.ids[i], a.E) : -1;
         int rank, count;
@@ -278,7 +276,6 @@ __global__ __launch_bounds__(256) void route_sort_kernel(RouteArgs a, int bits) 
         }
         __syncthreads();
     }
-    (void)lane;
 }
 
 int bits_of(int classes) {
@@ -304,8 +301,13 @@ int launch_dt(RouteArgs a, hipStream_t stream) {
         route_small_kernel<DT, V><<<1, waves * 64, lds, stream>>>(a, bits);
         return check_hip(hipGetLastError(), "route_small");
     }
-    route_select_kernel<DT, V><<<a.blocks, 256, classes * 4, stream>>>(a);
-    route_sort_kernel<<<a.blocks, 256, 6 * classes * 4, stream>>>(a, bits);
+    static DeviceOnce once;
+    if (once.first()) {
+        const int rc = check_hip(hipFuncSetAttribute((const void*)route_sort_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024), "hipFuncSetAttribute");
+        if (rc != GLA_OK) return rc;
+    }
+    route_select_kernel<DT, V><<<a.blocks, kThreads, classes * 4, stream>>>(a);
+    route_sort_kernel<<<a.blocks, kThreads, (2 + kThreads / 64) * classes * 4, stream>>>(a, bits);
     return check_hip(hipGetLastError(), "route_sort");
 }
 
@@ -320,11 +322,13 @@ int launch_v(const RouteArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-int route_blocks(int T) {
+static int route_blocks(int T) {
     int b = (T + kMinTokens - 1) / kMinTokens;
     if (b > kMaxBlocks) b = kMaxBlocks;
     return b < 4 ? 4 : (b + 3) / 4 * 4;
 }
+
+int64_t route_counts(int T, int E, int top_k) { return (int64_t)T * top_k <= kSmallSlots ? 0 : (int64_t)(E + 1) * route_blocks(T); }
 
 int launch_route(const void* logits, int dtype, int64_t stride, int T, int E, int top_k, int sigmoid, int renormalize, float scale,
                  float* weights, int32_t* ids, int32_t* offsets, int32_t* order, int32_t* places, int32_t* counts, hipStream_t stream) {

@@ -236,7 +236,8 @@ __global__ __launch_bounds__(256) void experts_stream_kernel(ExpertArgs a) {
                     u32x4 c[2];
                 } op_t;
                 op_t wo[NT], xo;
-                float sw[NT], f[32], amax = 0.0f, sx, inv;
+                float sw[NT], f[32], sx, inv;
+                uint32_t m = 0;
                 const int swz = (cg >> 1) & 7;
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
@@ -253,11 +254,11 @@ __global__ __launch_bounds__(256) void experts_stream_kernel(ExpertArgs a) {
                     const uint32_t v = x[i / 4][i % 4];
                     f[2 * i] = low16<BF16>(v);
                     f[2 * i + 1] = high16<BF16>(v);
-                    amax = fmaxf(amax, fmaxf(fabsf(f[2 * i]), fabsf(f[2 * i + 1])));
+                    m = magnitude_max(m, v);
                 }
-                amax = fmaxf(amax, wave_xor(amax, 16));
-                amax = fmaxf(amax, wave_xor(amax, 32));
-                block_scale(amax, sx, inv);
+                m = magnitude_max(m, wave_xor(m, 16));
+                m = magnitude_max(m, wave_xor(m, 32));
+                block_scale(low16<BF16>((m & 0xffffu) > (m >> 16) ? m & 0xffffu : m >> 16), sx, inv);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) xo.c[i / 4][i % 4] = quantise4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3], inv);
 #pragma unroll
@@ -393,8 +394,11 @@ int launch_fold(const ExpertArgs& a, hipStream_t stream) {
 
 template <int FMT>
 int launch_format(const ExpertArgs& a, bool bf16, int rows, hipStream_t stream) {
-    if (bf16) return rows > 4 ? launch_fold<FMT, true, 16>(a, stream) : launch_fold<FMT, true, 4>(a, stream);
-    return rows > 4 ? launch_fold<FMT, false, 16>(a, stream) : launch_fold<FMT, false, 4>(a, stream);
+    // (4-bit units are small enough for two workgroups per CU with room for 16 rows as well: no shorter tile)
+    if constexpr (FMT != kEW4) {
+        if (rows <= 4) return bf16 ? launch_fold<FMT, true, 4>(a, stream) : launch_fold<FMT, false, 4>(a, stream);
+    }
+    return bf16 ? launch_fold<FMT, true, 16>(a, stream) : launch_fold<FMT, false, 16>(a, stream);
 }
 
 }  // namespace

@@ -11,6 +11,7 @@ and the row counts stay on the GPU.
 ``GemLiteExperts`` stacks packed ``GemLiteLinear`` layers of one kind; ``GemLiteMoE`` is the three lines above as a module.
 As everywhere in this package the products have no backward pass: outputs carry no gradient.
 """
+import threading
 from typing import List, NamedTuple, Optional
 
 import torch
@@ -43,11 +44,12 @@ class ExpertPlan(NamedTuple):
 # ---------------------------------------------------------------------------
 # routing
 # ---------------------------------------------------------------------------
-def _empty_plan(T, k, E, device):
-    def make(*shape):
-        return torch.empty(shape, dtype=torch.int32, device=device)
-
-    return make(T, k), make(E + 1), make(T * k), make(T, k)
+def _empty_plan(like, T, k, E):
+    """(ids, offsets, order, places), views of one allocation (the kernels address them element by element)."""
+    n = T * k
+    ints = like.new_empty(3 * n + E + 1, dtype=torch.int32)
+    return (ints.as_strided((T, k), (k, 1), 0), ints.as_strided((E + 1,), (1,), 3 * n), ints.as_strided((n,), (1,), n),
+            ints.as_strided((T, k), (k, 1), 2 * n))
 
 
 def route_experts(logits: Tensor, top_k: int, scoring: str = "softmax", renormalize: bool = True, scale: float = 1.0) -> ExpertPlan:
@@ -67,8 +69,8 @@ def route_experts(logits: Tensor, top_k: int, scoring: str = "softmax", renormal
         raise ValueError(f"top_k: expected 1 .. {min(E, 64)}, got {top_k}")
     if logits.stride(1) != 1 or (T > 1 and logits.stride(0) < E):
         logits = logits.contiguous()
-    weights = torch.empty((T, top_k), dtype=torch.float32, device=logits.device)
-    ids, offsets, order, places = _empty_plan(T, top_k, E, logits.device)
+    weights = logits.new_empty((T, top_k), dtype=torch.float32)
+    ids, offsets, order, places = _empty_plan(logits, T, top_k, E)
     _ext.route_experts(logits, top_k, SCORINGS[scoring], renormalize, scale, weights, ids, offsets, order, places)
     return ExpertPlan(weights, ids, offsets, order, places)
 
@@ -86,7 +88,7 @@ def plan_experts(expert_ids: Tensor, weights: Tensor, num_experts: int) -> Exper
         expert_ids = expert_ids.clamp(-1, 2 ** 31 - 1)
     ids = expert_ids.to(torch.int32).contiguous()
     T, k = ids.shape
-    _, offsets, order, places = _empty_plan(T, k, int(num_experts), ids.device)
+    _, offsets, order, places = _empty_plan(ids, T, k, int(num_experts))
     _ext.plan_experts(ids, num_experts, offsets, order, places)
     return ExpertPlan(weights.to(torch.float32).contiguous(), ids, offsets, order, places)
 
@@ -130,7 +132,16 @@ def _weights_of(tensor_args, meta_args):
     return E, N, K
 
 
-def _launch(mode, x, bias, tensor_args, meta_args, offsets, plan, tile_config):
+# Filling and checking a gla_experts_args takes longer than a decode-sized launch, so a filled struct is kept per kind of
+# call (shapes, strides, types, devices, modes: never addresses or objects) and later calls of the kind only set the
+# addresses.  Entries are per thread: the struct is rewritten in place on every call.
+_PREPARED = {}
+_PREPARED_LIMIT = 4096
+_thread_id = threading.get_ident
+
+
+def _prepare(mode, x, fits, bias, tensor_args, meta_args, offsets, plan, tile_config):
+    """Checks a call and returns (struct, workspace bytes, shape of the output, its type)."""
     W_q, scales, zeros = tensor_args[0], tensor_args[1], tensor_args[2]
     meta = [int(v) for v in meta_args]
     (scaled, nbits, group, _, e, _, out_code, _, _, csm, wgm, _) = meta
@@ -170,25 +181,61 @@ def _launch(mode, x, bias, tensor_args, meta_args, offsets, plan, tile_config):
             a.weights = _plan_tensor("plan.weights", plan.weights, (T, k), torch.float32, device)
     else:
         a.R = rows
-    out = torch.empty((out_rows, out_cols), dtype=DTYPE_TO_TORCH[out_code], device=device)
     if bias is not None:
         a.bias = _plan_tensor("bias", bias, (E, N), torch.float32, device)
-
-    if x.stride(1) != 1 or x.stride(0) % 8 != 0 or x.stride(0) < K or x.data_ptr() % 16 != 0:
-        x = x.clone(memory_format=torch.contiguous_format)
     a.x_dtype = TORCH_TO_DTYPE[x.dtype].value
     a.input_dtype = DType.FP8.value if scaled else a.x_dtype
-    a.x, a.x_stride_m = x.data_ptr(), x.stride(0) if rows > 1 else K
-    a.out, a.out_stride_m = out.data_ptr(), out_cols
-    a.w, a.w_stride_e = W_q.data_ptr(), (W_q.stride(0) if E > 1 else W_q.shape[1] * N) * W_q.element_size()
+    a.x_stride_m, a.out_stride_m = (x.stride(0) if fits and rows > 1 else K), out_cols
+    a.w_stride_e = (W_q.stride(0) if E > 1 else W_q.shape[1] * N) * W_q.element_size()
     if nbits == 4:
         a.meta_dtype = TORCH_TO_DTYPE[scales.dtype].value
-        a.scales, a.meta_stride_e = scales.data_ptr(), scales.stride(0) * 2
-        a.zeros = zeros.data_ptr() if wgm != 2 else None
+        a.meta_stride_e = scales.stride(0) * 2
     elif nbits == 8:
         a.meta_dtype = DType.FP32.value
-        a.scales, a.meta_stride_e = scales.data_ptr(), scales.stride(0) * 4
-    _ext.experts_matmul(a, device)
+        a.meta_stride_e = scales.stride(0) * 4
+    # (addresses that stand for the operands until the first launch sets them: checks look at alignment only)
+    a.x = a.w = a.out = 4096
+    a.scales = 4096 if scales.numel() > 0 else None
+    a.zeros = 4096 if zeros.numel() > 0 and wgm != 2 else None
+    return a, _ext.experts_workspace_need(a), (out_rows, out_cols), DTYPE_TO_TORCH[out_code]
+
+
+def _launch(mode, x, bias, tensor_args, meta_args, offsets, plan, tile_config):
+    W_q, scales, zeros = tensor_args[0], tensor_args[1], tensor_args[2]
+    # whether the kernels can read the rows of x where they are (16-byte pieces); a copy is made of other ones
+    fits = x.data_ptr() % 16 == 0 and x.dim() == 2 and x.stride(1) == 1 and (
+        x.shape[0] <= 1 or (x.stride(0) % 8 == 0 and x.stride(0) >= x.shape[1]))
+    key = (mode, fits, tile_config, _thread_id(), x.shape, x.stride(), x.dtype, x.device, W_q.shape, W_q.stride(), W_q.dtype, W_q.device,
+           scales.shape, scales.stride(), scales.dtype, scales.device, zeros.shape, zeros.stride(), zeros.dtype, zeros.device,
+           offsets.shape, offsets.stride(), offsets.dtype, offsets.device, *meta_args)
+    if plan is not None:
+        p = plan.order if mode == _GATED else plan.weights
+        key += (plan.places.shape, plan.places.stride(), plan.places.dtype, plan.places.device, p.shape, p.stride(), p.dtype, p.device)
+    if bias is not None:
+        key += (bias.shape, bias.stride(), bias.dtype, bias.device)
+    entry = _PREPARED.get(key)
+    if entry is None:
+        entry = _prepare(mode, x, fits, bias, tensor_args, meta_args, offsets, plan, tile_config)
+        if len(_PREPARED) >= _PREPARED_LIMIT:
+            _PREPARED.clear()
+        _PREPARED[key] = entry
+    a, need, out_shape, out_dtype = entry
+    if not fits:
+        x = x.clone(memory_format=torch.contiguous_format)
+    out = x.new_empty(out_shape, dtype=out_dtype)
+    a.x, a.w, a.out, a.offsets = x.data_ptr(), W_q.data_ptr(), out.data_ptr(), offsets.data_ptr()
+    if a.scales is not None:
+        a.scales = scales.data_ptr()
+    if a.zeros is not None:
+        a.zeros = zeros.data_ptr()
+    if bias is not None:
+        a.bias = bias.data_ptr()
+    if mode == _GATED:
+        a.order = plan.order.data_ptr()
+    elif mode == _COMBINED:
+        a.places, a.weights = plan.places.data_ptr(), plan.weights.data_ptr()
+    if out_shape[0] > 0:
+        _ext.experts_matmul(a, need, x)
     return out
 
 

@@ -324,8 +324,8 @@ int gla_unpack_over_cols(const void* packed, uint8_t* out, int64_t rows, int64_t
  * stride_t elements apart), largest first, ties to the lower expert; NaN and -inf are never chosen (id -1, weight 0).
  * weights: softmax or sigmoid in fp32, divided by their sum over the chosen ones if `renormalize`, times `scale`.
  * Then the plan of these ids: offsets [E + 1], order [T * top_k], places [T * top_k].  top_k <= 64.
- * workspace: gla_route_workspace_bytes(T, E) bytes, 16-byte aligned, contents arbitrary. */
-int64_t gla_route_workspace_bytes(int T, int E);
+ * workspace: gla_route_workspace_bytes(T, E, top_k) bytes (0 for small calls), 16-byte aligned, contents arbitrary. */
+int64_t gla_route_workspace_bytes(int T, int E, int top_k);
 int gla_route_experts(const void* logits, int dtype, int64_t stride_t, int T, int E, int top_k, int scoring, int renormalize, float scale,
                       float* weights, int32_t* ids, int32_t* offsets, int32_t* order, int32_t* places, void* workspace,
                       int64_t workspace_bytes, void* stream);
@@ -377,7 +377,7 @@ typedef struct gla_experts_args {
     int32_t x_dtype;       /* of x, fp16 or bf16: the output type */
     int32_t channel_scale_mode, W_group_mode;
     int32_t tile_config;   /* -1: the library chooses; else rows per tile (4, 16: streaming kernel; 64, 128, 256: tiled
-                              GEMM) + 1000 * K splits (0: the library's number; streaming kernel only) */
+                              GEMM) + 1000 * K splits (0: the library's number) */
 } gla_experts_args;
 
 int64_t gla_experts_workspace_bytes(const gla_experts_args* args);

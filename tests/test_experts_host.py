@@ -48,7 +48,7 @@ def _args(**kw):
     (dict(struct_size=4), -1), (dict(mode=3), -3), (dict(E=0), -1), (dict(E=2000), -1), (dict(R=-1), -1), (dict(N=60), -4), (dict(K=240), -4),
     (dict(mode=1, N=56, out_stride_m=28), -4), (dict(output_dtype=0), -2), (dict(x_dtype=1), -2), (dict(W_nbits=2), -3),
     (dict(channel_scale_mode=1), -3), (dict(group_size=48), -4), (dict(group_size=96), -4), (dict(W_group_mode=1), -3), (dict(meta_dtype=0), -2),
-    (dict(scales=None), -1), (dict(zeros=None), -1), (dict(x=None), -1), (dict(offsets=None), -1), (dict(x=4104), -1), (dict(x_stride_m=252), -1),
+    (dict(scales=None), -1), (dict(K=1 << 21, N=8, out_stride_m=8, x_stride_m=1 << 21, w_stride_e=1 << 24), -1), (dict(zeros=None), -1), (dict(x=None), -1), (dict(offsets=None), -1), (dict(x=4104), -1), (dict(x_stride_m=252), -1),
     (dict(x_stride_m=128), -1), (dict(out_stride_m=32), -1), (dict(out=4100), -1), (dict(w_stride_e=16), -1), (dict(mode=1, order=None), -1),
     (dict(mode=2, places=None), -1), (dict(mode=2, weights=None), -1), (dict(mode=1, T=3), -1), (dict(mode=2, top_k=0), -1), (dict(tile_config=7), -1),
     (dict(tile_config=-3), -1), (dict(tile_config=99016), -1), (dict(N=1 << 20, K=1 << 14, w_stride_e=1 << 34, out_stride_m=1 << 20, x_stride_m=1 << 14), -3),
@@ -79,7 +79,7 @@ def test_library_refuses_routes():
     lib = _ext.load_library()
     p = 4096
 
-    def route(logits=p, dtype=0, stride=8, T=4, E=8, k=2, scoring=0, ws=p, n=1 << 20, offsets=p):
+    def route(logits=p, dtype=0, stride=8, T=4000, E=8, k=2, scoring=0, ws=p, n=1 << 20, offsets=p):
         return lib.gla_route_experts(logits, dtype, stride, T, E, k, scoring, 1, 1.0, p, p, offsets, p, p, ws, n, None)
 
     assert route(T=-1) == -1 and route(E=0) == -1 and route(E=1025) == -1 and route(k=0) == -1 and route(k=65, E=100) == -1
@@ -87,8 +87,9 @@ def test_library_refuses_routes():
     assert route(ws=None) == -5 and route(n=16) == -5 and route(ws=p + 4) == -5 and route(offsets=None) == -1
     assert route(T=1 << 30, k=4) == -1
     assert lib.gla_plan_experts(None, 4, 8, 2, p, p, p, p, 1 << 20, None) == -1
-    assert lib.gla_plan_experts(p, 4, 8, 2, p, p, p, p, 8, None) == -5
-    assert lib.gla_route_workspace_bytes(4, 0) == -1 and lib.gla_route_workspace_bytes(0, 8) > 0
+    assert lib.gla_plan_experts(p, 4000, 8, 2, p, p, p, p, 8, None) == -5
+    assert lib.gla_route_workspace_bytes(4, 0, 1) == -1 and lib.gla_route_workspace_bytes(0, 8, 1) == 0
+    assert lib.gla_route_workspace_bytes(4000, 8, 2) > 0
 
 
 def _w4_layers(E=3, K=128, N=32, gs=64, bias=False, dtype=torch.float16):

@@ -302,3 +302,197 @@ TILES = [4, 16, 2016, 3004, 64, 128, 256]
 def test_every_kernel_variant(fmt, dtype, tile_config):
     for T, K, N, gs in ((1, 512, 144, 128), (77, 1024, 272, 64), (330, 384, 528, 32)):
         run_case(fmt, dtype, 5, T, 2, K, N, gs, drop=0.05, tile_config=tile_config, bias=T == 77)
+
+
+# ---------------------------------------------------------------------------
+# operands as callers have them
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_strided_and_misaligned_activations(fmt):
+    E, T, k, K, N = 4, 37, 2, 256, 96
+    layers, _ = make_layers(fmt, "bf16", E, K, N)
+    experts = GemLiteExperts.from_layers(layers)
+    ids, w = make_ids(T, E, k)
+    plan = gemlite_amd.plan_experts(ids.cuda(), w.cuda(), E)
+    x = make_x(T, K, "bf16").cuda()
+    want = experts.forward_gated(x, plan)
+    wide = torch.zeros((T, K + 24), dtype=x.dtype, device="cuda")
+    for lo in (0, 8, 3, 16):            # rows 16-byte aligned, then rows that are not
+        view = wide[:, lo:lo + K]
+        view.copy_(x)
+        assert torch.equal(experts.forward_gated(view, plan), want)
+    odd = torch.zeros((T, K + 5), dtype=x.dtype, device="cuda")[:, :K]
+    odd.copy_(x)
+    assert torch.equal(experts.forward_gated(odd, plan), want)
+    assert torch.equal(experts.forward_gated(x.t().contiguous().t(), plan), want)
+    flat = torch.zeros(T * K + 1, dtype=x.dtype, device="cuda")[1:].view(T, K)
+    flat.copy_(x)
+    assert torch.equal(experts.forward_gated(flat, plan), want)
+    every_second = torch.zeros((2 * T, K), dtype=x.dtype, device="cuda")[::2]
+    every_second.copy_(x)
+    assert torch.equal(experts.forward_gated(every_second, plan), want)
+
+
+def _moe(fmt, dtype, E, hidden, inter, seed=0):
+    up, Wu = make_layers(fmt, dtype, E, hidden, 2 * inter, 64, seed)
+    down, Wd = make_layers(fmt, dtype, E, inter, hidden, 64, seed + 50)
+    return GemLiteExperts.from_layers(up), GemLiteExperts.from_layers(down), Wu, Wd
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("T", [1, 9, 250])
+def test_block_of_experts(fmt, T):
+    """Routing and both products as a module runs them, against 64 bits."""
+    E, k, hidden, inter = 8, 2, 256, 128
+    gate_up, down, Wu, Wd = _moe(fmt, "bf16", E, hidden, inter)
+    moe = GemLiteMoE(gate_up, down, k)
+    x = make_x(T, hidden, "bf16")
+    logits = torch.randn((T, E), generator=_gen(5))
+    y = moe(x.cuda().view(1, T, hidden), logits.cuda().view(1, T, E)).cpu().double()
+    w, ids = ref_route(logits, k, "softmax", True, 1.0)
+    ref = torch.zeros((T, hidden), dtype=torch.float64)
+    xd = quantised(x) if fmt == "fp8" else x.double()
+    for t in range(T):
+        for j in range(k):
+            z = xd[t] @ Wu[ids[t, j]]
+            h = (silu(z[:inter]) * z[inter:]).to(torch.bfloat16)
+            hd = quantised(h[None])[0] if fmt == "fp8" else h.double()
+            ref[t] += w[t, j] * (hd @ Wd[ids[t, j]])
+    assert y.shape == (1, T, hidden)
+    # h is rounded to bf16 on both sides but from sums that differ by fp32 or, for rounded 4-bit weights, bf16 noise: up to
+    # one more rounding of h (and, fp8, of its codes: 2^-4 of the few that cross a border) and one of the result
+    u = 2.0 ** -9
+    assert float((y[0] - ref).norm() / ref.norm()) <= (2 * u if fmt != "fp8" else 4 * u) * 2
+
+
+def test_graph_replays_equal_eager_calls():
+    E, k, hidden, inter, T = 8, 2, 256, 128, 24
+    for fmt in FORMATS:
+        gate_up, down, _, _ = _moe(fmt, "fp16", E, hidden, inter)
+        moe = GemLiteMoE(gate_up, down, k)
+        x, logits = make_x(T, hidden, "fp16").cuda(), torch.randn((T, E), generator=_gen(1)).cuda()
+        moe(x, logits)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = moe(x, logits)
+        other = torch.cuda.CUDAGraph()
+        x2, logits2 = make_x(T, hidden, "fp16", 9).cuda(), torch.randn((T, E), generator=_gen(9)).cuda()
+        with torch.cuda.graph(other):
+            y2 = moe(x2, logits2)
+        for i in range(4):
+            x.copy_(make_x(T, hidden, "fp16", 20 + i).cuda())
+            logits.copy_(torch.randn((T, E), generator=_gen(30 + i)).cuda())
+            want, want2 = moe(x, logits), moe(x2, logits2)
+            torch.cuda.synchronize()
+            graph.replay()
+            other.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, want) and torch.equal(y2, want2)
+
+
+def test_streams_and_threads_do_not_share_scratch():
+    import threading
+
+    E, k, hidden, inter, T = 8, 4, 256, 128, 100
+    gate_up, down, _, _ = _moe("w4", "bf16", E, hidden, inter)
+    moe = GemLiteMoE(gate_up, down, k)
+    inputs = [(make_x(T, hidden, "bf16", s).cuda(), torch.randn((T, E), generator=_gen(s)).cuda()) for s in range(4)]
+    want = [moe(*i) for i in inputs]
+    torch.cuda.synchronize()
+    got = [None] * 4
+
+    def work(n):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got[n] = moe(*inputs[n])
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_offsets_that_are_not_a_plan(fmt):
+    """Whatever offsets, order and places hold, rows outside the call are neither read nor written."""
+    E, R, K, N = 4, 40, 128, 64
+    layers, _ = make_layers(fmt, "bf16", E, K, N)
+    e = GemLiteExperts.from_layers(layers)
+    x = make_x(R, K, "bf16").cuda()
+    good = torch.tensor([0, 10, 20, 30, 40], dtype=torch.int32, device="cuda")
+    full = e(x, good)
+    for off in ([0, 10, 20, 30, 10 ** 6], [-5, 10, 20, 30, 40]):
+        assert torch.equal(e(x, torch.tensor(off, dtype=torch.int32, device="cuda")), full)
+    y = e(x, torch.tensor([0, 10, 20, 30, 33], dtype=torch.int32, device="cuda"))
+    assert torch.equal(y[:33], full[:33]) and not y[33:].any()
+    for off in ([40, 0, 40, 0, 40], [7, 7, 7, 7, 7]):
+        assert e(x, torch.tensor(off, dtype=torch.int32, device="cuda")).shape == (R, N)
+    big = torch.full((R,), 2 ** 31 - 1, dtype=torch.int32, device="cuda")
+    plan = ExpertPlan(torch.ones((R // 2, 2), device="cuda"), big.view(-1, 2), good, big, big.view(-1, 2))
+    assert e.forward_gated(x[: R // 2], plan).shape == (R, N // 2)
+    assert not e.forward_combined(x, plan).any()      # no place is one of the rows
+    plan = plan._replace(order=-big, places=-big.view(-1, 2))
+    e.forward_gated(x[: R // 2], plan)
+    assert not e.forward_combined(x, plan).any()
+    torch.cuda.synchronize()
+
+
+def test_values_that_are_not_finite_stay_in_their_rows():
+    """A row with an infinity or a NaN changes no other row, and slots without an expert are not looked at."""
+    for fmt in FORMATS:
+        E, T, k, K, N = 4, 20, 2, 256, 64
+        layers, _ = make_layers(fmt, "bf16", E, K, N)
+        e = GemLiteExperts.from_layers(layers)
+        ids, w = make_ids(T, E, k)
+        plan = gemlite_amd.plan_experts(ids.cuda(), w.cuda(), E)
+        x = make_x(T, K, "bf16")
+        clean = e.forward_gated(x.cuda(), plan).cpu()
+        x[3, 7], x[11, 100] = float("inf"), float("nan")
+        dirty = e.forward_gated(x.cuda(), plan).cpu()
+        rows = plan.order.cpu() // k
+        ok = (rows != 3) & (rows != 11)
+        assert torch.equal(clean[ok], dirty[ok]) and not torch.isfinite(dirty[rows == 11].float()).any()
+        ids[5, 1] = -1
+        plan = gemlite_amd.plan_experts(ids.cuda(), w.cuda(), E)
+        h = make_x(T * k, K, "bf16").cuda()
+        y = e.forward_combined(h, plan)
+        h[int(plan.places[5, 1])] = float("nan")
+        weights = plan.weights.clone()
+        weights[5, 1] = float("nan")
+        assert torch.equal(e.forward_combined(h, plan._replace(weights=weights)), y)
+
+
+def test_empty_calls():
+    for fmt in FORMATS:
+        layers, _ = make_layers(fmt, "bf16", 4, 128, 64)
+        e = GemLiteExperts.from_layers(layers)
+        x = torch.empty((0, 128), dtype=torch.bfloat16, device="cuda")
+        assert e(x, torch.zeros(5, dtype=torch.int32, device="cuda")).shape == (0, 64)
+        plan = gemlite_amd.route_experts(torch.empty((0, 4), device="cuda"), 2)
+        assert e.forward_gated(x, plan).shape == (0, 32) and e.forward_combined(x, plan).shape == (0, 64)
+
+
+def test_refusals_on_the_gpu():
+    layers, _ = make_layers("w4", "bf16", 4, 128, 64)
+    e = GemLiteExperts.from_layers(layers)
+    x = make_x(8, 128, "bf16").cuda()
+    off = torch.tensor([0, 2, 4, 6, 8], dtype=torch.int32, device="cuda")
+    plan = gemlite_amd.route_experts(torch.zeros((4, 4), device="cuda"), 2)
+    for bad, exc in ((lambda: e(x[:, :64], off), ValueError), (lambda: e(x.float(), off), NotImplementedError), (lambda: e(x.half(), off), NotImplementedError),
+                     (lambda: e(x, off.long()), ValueError), (lambda: e(x, off[:4]), ValueError), (lambda: e(x, off.cpu()), RuntimeError),
+                     (lambda: e.forward_gated(x, plan), ValueError), (lambda: e.forward_combined(x[:4], plan), ValueError),
+                     (lambda: e.forward_combined(x, plan._replace(weights=plan.weights.half())), ValueError),
+                     (lambda: e.forward_combined(x, plan._replace(places=plan.places.t())), ValueError),
+                     (lambda: e.forward_gated(x[:4], plan._replace(order=plan.order[::2])), ValueError),
+                     (lambda: gemlite_amd.route_experts(torch.zeros((4, 4), device="cuda"), 5), ValueError),
+                     (lambda: gemlite_amd.route_experts(torch.zeros((4, 4), device="cuda", dtype=torch.float64), 2), NotImplementedError),
+                     (lambda: gemlite_amd.route_experts(torch.zeros((4, 2000), device="cuda"), 2), ValueError)):
+        for _ in range(2):   # the second time as the first: nothing refused is remembered as accepted
+            with pytest.raises(exc):
+                bad()
+    assert e(x, off).shape == (8, 64)
