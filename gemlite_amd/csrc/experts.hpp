@@ -35,6 +35,7 @@ struct ExpertArgs {
     int group;                      // W4: K-values per group (scales and zeros have the activations' type)
     uint32_t group_mul, top_k_mul;  // n / (group / 32) and n / top_k as the high half of n * this (0: see divide_by)
     int groups;                     // W4: K / group
+    int stream_waves;               // streaming kernel: waves of a workgroup, 4 (W4: or 2)
     int chunk;                      // streaming kernel: units of 128 K-values per wave; tiled GEMM: stages per split
     float c1, c2;                   // W4: zero-point term of a weight = zero * (c1 + c2 * scale)
 };

@@ -17,7 +17,7 @@
 //  * gridDim.y splits K where the tiles do not fill the chip (fp32 sums to the workspace, added in order by the
 //    finishing kernel).
 //  * A workgroup's tile is found from the offsets on the device; the tiles that exist are dealt to the 8 XCDs in
-//    contiguous bands, and a band is walked in groups of 1024 rows x all columns, so that the L2 of an XCD keeps a
+//    contiguous bands, and a band is walked in groups of 8 row tiles x all columns, so that the L2 of an XCD keeps a
 //    weight panel for all row tiles of the group.
 #include <type_traits>
 
@@ -210,7 +210,7 @@ __device__ __forceinline__ void gemm_tile(const ExpertArgs& a, const ExpertTile&
             u32x4 c[2];
         } op_t;
         const int c0 = ((2 * fk) ^ swz) * 16, c1 = ((2 * fk + 1) ^ swz) * 16;
-        // Tile (i, j) of the wave is slice q = i TJ + j of a stage: its MFMA, the fold of the slice two in front, and a
+        // Tile (i, j) of the wave is slice q = i TJ + j of a stage: its MFMA, the fold of the slice three in front, and a
         // share of the LDS reads and copies, with the scheduler fenced between slices (left alone it reads every fragment
         // right in front of its MFMA).  The fragment of activation row tile i + 1 is read during tile i; the barrier
         // stands before the last row tile, and a column's weight fragment for the next stage is read behind the last MFMA
@@ -255,7 +255,7 @@ __device__ __forceinline__ void gemm_tile(const ExpertArgs& a, const ExpertTile&
                 }
                 d[q % 4] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j].v, fa[i & 1].v, zero4, 0, 0, 0, 127, 0, 127);
                 sc[q % 4] = sx[i & 1] * sw[j];
-                if (q >= 2) fold(q - 2);
+                if (q >= 3) fold(q - 3);
                 if (i + 1 < TI) {
                     if (j == 0) read_a(base, i + 1, (i + 1) & 1);
                 } else {
@@ -268,6 +268,7 @@ __device__ __forceinline__ void gemm_tile(const ExpertArgs& a, const ExpertTile&
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
+            fold(NS - 3);
             fold(NS - 2);
             fold(NS - 1);
             slot = next_slot;
@@ -474,7 +475,7 @@ __global__ __launch_bounds__((GemmShape<FMT, BM, BN>::THREADS)) void experts_gem
         if (pid >= total) return -1;
         const int xcd = pid & 7, q = total >> 3, r = total & 7;
         const int t = xcd * q + (xcd < r ? xcd : r) + (pid >> 3);
-        constexpr int GROUP = 1024 / BM;
+        constexpr int GROUP = 8;
         const int width = GROUP * tiles_n, group = t / width, first = group * GROUP;
         const int rows = total_m - first < GROUP ? total_m - first : GROUP;
         ct = (t - group * width) / rows;

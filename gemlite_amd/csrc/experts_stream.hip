@@ -2,7 +2,7 @@
 // (4 or 16) activation rows.  Bound by the bytes of the experts that have rows.
 //
 //  * A workgroup owns WC columns (64; 16-bit weights 32) of one expert for one tile of MR rows; gated calls take half of
-//    them from the gate and the same ones of the up projection.  Its NW waves split K and meet once in LDS at the end, so
+//    them from the gate and the same ones of the up projection.  Its 4 (2) waves split K and meet once in LDS at the end, so
 //    a launch with few column tiles still has thousands of loads in flight; gridDim.z splits K further where even that
 //    leaves the chip empty (fp32 sums to the workspace, added in order by the finishing kernel).
 //  * A wave walks its K range in units of 128 values and shares nothing with the others on the way: the load unit copies a
@@ -55,14 +55,14 @@ __device__ __forceinline__ u32x4 pairs_of(const u32x4& v) {
 }
 
 // FU: K-values between two folds of a W4 group's constants (the largest of 128, 64, 32 that divides the group).
-template <int FMT, int MR, int FU>
+// NW: waves of a workgroup.
+template <int FMT, int MR, int FU, int NW>
 struct StreamShape {
     static constexpr int WC = FMT == kE16 ? 32 : 64;
     static constexpr int NT = WC / 16;
     static constexpr int FOLDS = 128 / FU;
     static constexpr int W_OPS = FMT == kEW4 ? 4 : 8, M_OPS = FMT == kEW4 ? FOLDS : (FMT == kEF8 ? 1 : 0);
     static constexpr int W_BYTES = W_OPS * 1024;
-    static constexpr int NW = 4;
     // XO: activation copies per unit, 4 rows each
     static constexpr int ops(int xo) { return W_OPS + xo + M_OPS; }
     static constexpr int slot(int xo) { return W_BYTES + xo * 1024 + M_OPS * 256; }
@@ -73,10 +73,10 @@ struct StreamShape {
     static constexpr int LDS = NW * most(RING, 16 * WC * 4);
 };
 
-template <int FMT, bool BF16, int MR, int FU>
-__global__ __launch_bounds__(256) void experts_stream_kernel(ExpertArgs a) {
-    using SH = StreamShape<FMT, MR, FU>;
-    constexpr int WC = SH::WC, NT = SH::NT, NW = SH::NW;
+template <int FMT, bool BF16, int MR, int FU, int NW>
+__global__ __launch_bounds__(NW * 64, 2) void experts_stream_kernel(ExpertArgs a) {
+    using SH = StreamShape<FMT, MR, FU, NW>;
+    constexpr int WC = SH::WC, NT = SH::NT;
 
     extern __shared__ __align__(16) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -361,34 +361,35 @@ __global__ __launch_bounds__(256) void experts_stream_kernel(ExpertArgs a) {
     }
 }
 
-template <int FMT, bool BF16, int MR, int FU>
+template <int FMT, bool BF16, int MR, int FU, int NW>
 int launch_one(const ExpertArgs& a, hipStream_t stream) {
-    using SH = StreamShape<FMT, MR, FU>;
+    using SH = StreamShape<FMT, MR, FU, NW>;
     static_assert(SH::LDS <= 160 * 1024 && 3 * SH::ops(4) < 64, "ring does not fit LDS or the counter");
     const int64_t tiles = max_row_tiles(a.R, a.E, MR);
     if (tiles > 65535 || a.S > 65535) {
         set_error("experts: %lld row tiles exceed the grid", (long long)tiles);
         return GLA_ERR_INVALID_ARGUMENT;
     }
-    const auto kernel = experts_stream_kernel<FMT, BF16, MR, FU>;
+    const auto kernel = experts_stream_kernel<FMT, BF16, MR, FU, NW>;
     static DeviceOnce once;
     if (once.first()) {
         const int rc = check_hip(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, SH::LDS), "hipFuncSetAttribute");
         if (rc != GLA_OK) return rc;
     }
     const int cols = a.half ? SH::WC / 2 : SH::WC, width = a.half ? a.half : a.N;
-    kernel<<<dim3((width + cols - 1) / cols, (unsigned)tiles, a.S), SH::NW * 64, SH::LDS, stream>>>(a);
+    kernel<<<dim3((width + cols - 1) / cols, (unsigned)tiles, a.S), NW * 64, SH::LDS, stream>>>(a);
     return check_hip(hipGetLastError(), "experts_stream");
 }
 
 template <int FMT, bool BF16, int MR>
 int launch_fold(const ExpertArgs& a, hipStream_t stream) {
     if constexpr (FMT == kEW4) {
-        if (a.group % 128 == 0) return launch_one<FMT, BF16, MR, 128>(a, stream);
-        if (a.group % 64 == 0) return launch_one<FMT, BF16, MR, 64>(a, stream);
-        return launch_one<FMT, BF16, MR, 32>(a, stream);
+        const bool two = a.stream_waves == 2;
+        if (a.group % 128 == 0) return two ? launch_one<FMT, BF16, MR, 128, 2>(a, stream) : launch_one<FMT, BF16, MR, 128, 4>(a, stream);
+        if (a.group % 64 == 0) return two ? launch_one<FMT, BF16, MR, 64, 2>(a, stream) : launch_one<FMT, BF16, MR, 64, 4>(a, stream);
+        return two ? launch_one<FMT, BF16, MR, 32, 2>(a, stream) : launch_one<FMT, BF16, MR, 32, 4>(a, stream);
     } else {
-        return launch_one<FMT, BF16, MR, 128>(a, stream);
+        return launch_one<FMT, BF16, MR, 128, 4>(a, stream);
     }
 }
 

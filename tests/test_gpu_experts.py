@@ -304,6 +304,12 @@ def test_every_kernel_variant(fmt, dtype, tile_config):
         run_case(fmt, dtype, 5, T, 2, K, N, gs, drop=0.05, tile_config=tile_config, bias=T == 77)
 
 
+@pytest.mark.parametrize("gs", [32, 64, 128])
+def test_many_column_tiles_of_4_bit_weights(gs):
+    """Enough workgroups for two-wave ones (K of 16 units and more), a K range that does not divide evenly."""
+    run_case("w4", "bf16", 8, 40, 2, 2176, 6240, gs, drop=0.1)
+
+
 # ---------------------------------------------------------------------------
 # operands as callers have them
 # ---------------------------------------------------------------------------
