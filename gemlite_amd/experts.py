@@ -59,6 +59,12 @@ def route_experts(logits: Tensor, top_k: int, scoring: str = "softmax", renormal
     the remaining slots get id -1 and weight 0.  Weights are ``scoring`` ("softmax" or "sigmoid") of the logits in fp32,
     with ``renormalize`` divided by their sum over the chosen ones, times ``scale``.
     """
+    if torch.compiler.is_compiling():
+        return ExpertPlan(*route_experts_op(logits, top_k, scoring, renormalize, scale))
+    return _route_experts(logits, top_k, scoring, renormalize, scale)
+
+
+def _route_experts(logits, top_k, scoring, renormalize, scale):
     if logits.dim() != 2:
         raise ValueError(f"logits: expected [tokens, experts], got shape {tuple(logits.shape)}")
     if scoring not in SCORINGS:
@@ -250,7 +256,7 @@ def experts_functional(x: Tensor, bias: Optional[Tensor], tensor_args: List[Tens
     divide by 448 where this multiplies: a value on the border between two codes, which is where 16-bit values over
     their block's maximum often lie, may get the other neighbour.)
     """
-    return _launch(_ROWS, x, bias, tensor_args, meta_args, offsets, None, tile_config)
+    return _dispatch(_ROWS, x, bias, tensor_args, meta_args, offsets, None, tile_config)
 
 
 def experts_gated_functional(x: Tensor, bias: Optional[Tensor], tensor_args: List[Tensor], meta_args: List[int], plan: ExpertPlan,
@@ -258,14 +264,14 @@ def experts_gated_functional(x: Tensor, bias: Optional[Tensor], tensor_args: Lis
     """``silu(x[t] @ W_gate[e]) * (x[t] @ W_up[e])`` for every (token, expert) pair of the plan, as rows sorted by expert
     [T k, N / 2].  The first half of an expert's N columns is the gate, the second the up projection.  The activation is
     applied to the fp32 sums.  Rows without an expert are zeros."""
-    return _launch(_GATED, x, bias, tensor_args, meta_args, plan.offsets, plan, tile_config)
+    return _dispatch(_GATED, x, bias, tensor_args, meta_args, plan.offsets, plan, tile_config)
 
 
 def experts_combined_functional(h: Tensor, bias: Optional[Tensor], tensor_args: List[Tensor], meta_args: List[int], plan: ExpertPlan,
                                 tile_config: int = -1) -> Tensor:
     """``sum over a token's slots of weight * (h[place] @ W[e])`` for rows ``h`` [T k, K] sorted by expert: [T, N].  Products
     and sum are fp32, rounded once; slots without an expert add nothing."""
-    return _launch(_COMBINED, h, bias, tensor_args, meta_args, plan.offsets, plan, tile_config)
+    return _dispatch(_COMBINED, h, bias, tensor_args, meta_args, plan.offsets, plan, tile_config)
 
 
 class GemLiteExperts(torch.nn.Module):
@@ -423,7 +429,7 @@ class GemLiteMoE(torch.nn.Module):
         x2d, logits2d = x.reshape(-1, x.shape[-1]), logits.reshape(-1, logits.shape[-1])
         if x2d.shape[0] != logits2d.shape[0] or logits2d.shape[1] != self.gate_up.num_experts:
             raise ValueError(f"x of shape {tuple(x.shape)} and logits of shape {tuple(logits.shape)} for {self.gate_up.num_experts} experts")
-        plan = _dispatch_route(logits2d, self.top_k, self.scoring, self.renormalize, self.scale)
+        plan = route_experts(logits2d, self.top_k, self.scoring, self.renormalize, self.scale)
         y = self.down.forward_combined(self.gate_up.forward_gated(x2d, plan), plan)
         return y.view(x.shape[:-1] + (self.down.out_features,))
 
@@ -433,7 +439,8 @@ class GemLiteMoE(torch.nn.Module):
 # ---------------------------------------------------------------------------
 @torch.library.custom_op("gemlite::route_experts", mutates_args=())
 def route_experts_op(logits: Tensor, top_k: int, scoring: str, renormalize: bool, scale: float) -> List[Tensor]:
-    return list(route_experts(logits, top_k, scoring, renormalize, scale))
+    # (a plan's integers are views of one allocation; the outputs of an op must not share memory)
+    return [t.clone() for t in _route_experts(logits, top_k, scoring, renormalize, scale)]
 
 
 @route_experts_op.register_fake
@@ -459,16 +466,10 @@ def _(mode, x, bias, tensor_args, meta_args, offsets, plan):
     return torch.empty((rows, N // 2 if mode == _GATED else N), dtype=DTYPE_TO_TORCH[int(meta_args[6])], device=x.device)
 
 
-def _dispatch(mode, x, bias, tensor_args, meta_args, offsets, plan):
+def _dispatch(mode, x, bias, tensor_args, meta_args, offsets, plan, tile_config=-1):
     if torch.compiler.is_compiling():
         return experts_op(mode, x, bias, tensor_args, meta_args, offsets, [] if plan is None else list(plan))
-    return _launch(mode, x, bias, tensor_args, meta_args, offsets, plan, -1)
-
-
-def _dispatch_route(logits, top_k, scoring, renormalize, scale):
-    if torch.compiler.is_compiling():
-        return ExpertPlan(*route_experts_op(logits, top_k, scoring, renormalize, scale))
-    return route_experts(logits, top_k, scoring, renormalize, scale)
+    return _launch(mode, x, bias, tensor_args, meta_args, offsets, plan, tile_config)
 
 
 __all__ = [

@@ -502,3 +502,37 @@ def test_refusals_on_the_gpu():
             with pytest.raises(exc):
                 bad()
     assert e(x, off).shape == (8, 64)
+
+
+def test_compiled_module_equals_the_eager_one():
+    E, k, hidden, inter, T = 8, 2, 256, 128, 12
+    for fmt in FORMATS:
+        gate_up, down, _, _ = _moe(fmt, "bf16", E, hidden, inter)
+        moe = GemLiteMoE(gate_up, down, k)
+        x, logits = make_x(T, hidden, "bf16").cuda(), torch.randn((T, E), generator=_gen(1)).cuda()
+        graphs = []
+
+        def backend(graph, _):
+            graphs.append(graph)
+            return graph.forward
+
+        compiled = torch.compile(moe, backend=backend, fullgraph=True)
+        assert torch.equal(compiled(x, logits), moe(x, logits))
+        names = [str(n.target) for g in graphs for n in g.graph.nodes if n.op == "call_function"]
+        assert sum("route_experts" in n for n in names) == 1 and sum("gemlite.experts" in n for n in names) == 2
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("tile_config", [4, 16, 64, 128, 256])
+def test_a_nan_reaches_its_row_in_every_kernel(fmt, tile_config):
+    E, T, k, K, N = 2, 30, 1, 256, 64
+    layers, _ = make_layers(fmt, "bf16", E, K, N)
+    e = GemLiteExperts.from_layers(layers)
+    off = torch.tensor([0, 13, 30], dtype=torch.int32, device="cuda")
+    x = make_x(T, K, "bf16").cuda()
+    args = (None, e.get_tensor_args(), e.get_meta_args(), off)
+    clean = gemlite_amd.experts_functional(x, *args, tile_config=tile_config)
+    x[20, 200] = float("nan")
+    dirty = gemlite_amd.experts_functional(x, *args, tile_config=tile_config)
+    rest = torch.arange(T, device="cuda") != 20
+    assert torch.equal(clean[rest], dirty[rest]) and bool(torch.isnan(dirty[20].float()).all())
