@@ -21,7 +21,8 @@ struct FinishArgs {
 
 // out[r] = sum of the splits (gated: silu(gate) * up of it), or zeros where the row has no expert; combined: out[t] =
 // sum over the token's slots of weight * sum of the splits of its row.  All sums in fp32, in a fixed order; bound by the
-// fp32 rows it reads.  A thread takes 4 columns of one row.
+// fp32 rows it reads (32008 rows of 2048 to 4001 tokens: 50 us for 278 MB).  The rows are not rounded to 16 bits on the way,
+// which would halve that: it would add an error as large as that of rounding the result.  A thread takes 4 columns of one row.
 template <bool BF16, bool COMBINED>
 __global__ __launch_bounds__(256) void experts_finish_kernel(FinishArgs a) {
     const int64_t row = blockIdx.x;

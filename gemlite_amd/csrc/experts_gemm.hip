@@ -1,7 +1,7 @@
 // Products grouped by expert, many rows per expert: a tiled MFMA GEMM over ragged row blocks.
 //
-//  * Workgroup tile BM rows of one expert x 256 (BM = 64: 128) columns, 8 (4) waves; pipeline stage of 128 bytes of K per activation row (64
-//    16-bit values or 128 e4m3 codes).  Operand tiles, scales and zeros are copied global -> LDS by the load unit
+//  * Workgroup tile BM rows of one expert x 256 (BM = 64: 128) columns, 8 (4) waves; pipeline stage of 128 bytes of K per
+//    activation row (64 16-bit values or 128 e4m3 codes).  Operand tiles, scales and zeros are copied global -> LDS by the load unit
 //    (global_load_lds) into a ring of stages, all of them in flight; gated calls gather their activation rows on the
 //    way.  16-byte chunk c of a 128-byte row r lies at position c ^ ((r >> 1) & 7), chosen on the global side of the copy,
 //    so that the 16 lanes of an LDS read phase hit 16 different bank groups.
@@ -11,7 +11,10 @@
 //    matrix pipe has work while the waves meet and the first fragments of the next stage arrive.
 //  * W4: the packed words lie in LDS as they are in memory (a word = 8 K-values of a column = a lane's share of a
 //    K-step's operand) and are dequantised into the operand registers between the MFMAs, w = s q + z in fp32 for bf16,
-//    in packed fp16 for fp16, rounded once to the activation type.
+//    in packed fp16 for fp16, rounded once to the activation type, as the dense layers' tiled GEMM does: 2^-9 (bf16) of
+//    each weight at most, which makes the error of a sum 1.4 times that of rounding the result alone.  (Codes with the
+//    constants applied to the sums, as in the streaming kernel, would need a second set of accumulators: 128 rows would
+//    no longer fit two workgroups on a CU, and with one the call below takes 1190 us.)
 //  * F8: v_mfma_f32_16x16x128 starts from zero on every 128-block and its result joins the fp32 sum times the block's two
 //    scales.
 //  * gridDim.y splits K where the tiles do not fill the chip (fp32 sums to the workspace, added in order by the
@@ -19,6 +22,15 @@
 //  * A workgroup's tile is found from the offsets on the device; the tiles that exist are dealt to the 8 XCDs in
 //    contiguous bands, and a band is walked in groups of 8 row tiles x all columns, so that the L2 of an XCD keeps a
 //    weight panel for all row tiles of the group.
+//
+// Measured: 4-bit, E = 8, top 2, 4096 -> 2 x 14336, 2048 tokens 1020 us (940 TFLOP/s); fp8, E = 32, top 4, 4096 -> 2 x 2048, 4096
+// tokens 383 us (1430 TFLOP/s); 16-bit, 16 experts of 4096^2, 8200 rows 320 us (860; 930 at 16000 rows).  Bound by the copies
+// into LDS beside the reads from it: reads and writes together keep the LDS port busy for as many clocks as the MFMAs
+// take (256 rows, 64 K-values: 192 KB read, 64 KB written, 2048 clocks either way).  Without the copies of the K loop the
+// three calls take 890, 324 and (16000 rows) 444 us instead of 1029, 412 and 576; the fold of the fp8 scales costs nothing.
+// Measured and not kept: four waves with 128 x 128 wave tiles (a third less read from LDS, one wave per SIMD: 635 against 576
+// us at 16000 rows, 4-bit 1222 against 1009), 256 x 128 tiles on four waves with two workgroups per CU (667), stages of 64
+// bytes of K in a ring of four (600; 128 rows 733 against 598).
 #include <type_traits>
 
 #include "common.hpp"

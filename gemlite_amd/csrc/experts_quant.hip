@@ -2,7 +2,7 @@
 // kernel does in registers for a few rows, as a launch of its own in front of it or of the tiled GEMM.
 //
 // 16 lanes share a block of 128 values (8 each, one 16-byte load), so a wave step is 4 blocks = 1 KB in, 512 bytes out.
-// Bound by these bytes.
+// Bound by these bytes (32008 rows of 1408: 27 us for 135 MB).
 #include "common.hpp"
 #include "experts.hpp"
 
