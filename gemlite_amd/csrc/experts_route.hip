@@ -6,14 +6,15 @@
 //   order      flat indices token * k + slot, sorted by expert, within an expert in rising order; slots without an expert
 //              come last.  offsets[e] is where expert e's begin; places is the inverse of order
 //
-// A wave per token (32 tokens and 16 waves to a workgroup): lane l holds logits l, l + 64, ...; each of the k rounds is one wave-wide maximum and one wave-wide
-// minimum of the indices that have it (DPP, no LDS).  Up to kSmallSlots (token, slot) pairs one workgroup does everything
-// in one launch.  Above, a first launch selects and counts each block's slots per expert, and a second one sorts: every
-// block adds up the counts of the blocks in front of it for itself (they are a few kilobytes in L2), so no third launch
-// has to.  Counting by ballots and integer sums only: the result does not depend on the order of execution.
+// A wave per token (32 tokens and 16 waves to a workgroup): lane l holds logits l, l + 64, ...; each of the k rounds is one
+// wave-wide maximum and, where several lanes have it, one minimum of their indices (DPP, no LDS).  Up to kSmallSlots
+// (token, slot) pairs one workgroup does everything in one launch.  Above, a first launch selects and counts each block's
+// slots per expert, and a second one sorts: every block adds up the counts of the blocks in front of it for itself (they
+// are a few kilobytes in L2), so no third launch has to.  Counting by ballots and integer sums only: the result does not
+// depend on the order of execution.
 //
-// Bound by latency: 8191 tokens of 128 fp32 logits, top 8 (4 MB): 11.6 + 7.8 us, a token's 8 rounds being a chain of about 100
-// dependent instructions each; one token of 64: 4 us.
+// Bound by the selection's instructions and by latency: 8191 tokens of 128 fp32 logits, top 8 (4 MB): 8.4 + 6.1 us (with the
+// rounds on floats and both reductions in each: 11.4); one token of 64: 3.8 us.
 #include "common.hpp"
 #include "experts.hpp"
 
@@ -39,9 +40,23 @@ struct RouteArgs {
     int blocks, tokens;  // tokens per block
 };
 
-__device__ __forceinline__ float wave_max(float v) {
-#define GLA_STEP(ctrl, rm) \
-    v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v), (ctrl), (rm), 0xf, false)))
+// Logits as integers of the same order (both zeros the same, NaN as -inf): the wave-wide maximum of integers is one
+// instruction per step, that of floats three.
+__device__ __forceinline__ uint32_t key_of(float v) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v == v ? v + 0.0f : -__builtin_inff());
+    return b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t key) {
+    return __builtin_bit_cast(float, key ^ ((key & 0x80000000u) != 0 ? 0x80000000u : 0xffffffffu));
+}
+constexpr uint32_t kNoneKey = 0x007fffffu;  // of -inf
+
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+#define GLA_STEP(ctrl, rm)                                                                           \
+    {                                                                                                \
+        const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, (ctrl), (rm), 0xf, false); \
+        v = o > v ? o : v;                                                                           \
+    }
     GLA_STEP(0x111, 0xf);
     GLA_STEP(0x112, 0xf);
     GLA_STEP(0x114, 0xf);
@@ -49,7 +64,7 @@ __device__ __forceinline__ float wave_max(float v) {
     GLA_STEP(0x142, 0xa);
     GLA_STEP(0x143, 0xc);
 #undef GLA_STEP
-    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
 __device__ __forceinline__ int wave_min(int v) {
@@ -83,52 +98,60 @@ __device__ __forceinline__ float logit_at(const void* row, int i) {
 
 constexpr float kNone = -__builtin_inff();
 
-// One token by one wave: its id (or -1) in lane j < k; ids and weights stored.
+// The logits of token t, lane l those of experts l, l + 64, ..
 template <int DT, int V>
-__device__ __forceinline__ int select_token(const RouteArgs& a, int t) {
+__device__ __forceinline__ void load_token(const RouteArgs& a, int t, float (&v)[V]) {
     const int lane = threadIdx.x & 63;
     const int DTS = DT == GLA_DT_FP32 ? 4 : 2;
     const char* row = (const char*)a.logits + (int64_t)t * a.stride * DTS;
-    float v[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int e = j * 64 + lane;
-        v[j] = e < a.E ? logit_at<DT>(row, e) : kNone;
-        if (!(v[j] == v[j])) v[j] = kNone;
-    }
-    float top = 0.0f, denom = 0.0f, val = kNone;
+    for (int j = 0; j < V; ++j) v[j] = j * 64 + lane < a.E ? logit_at<DT>(row, j * 64 + lane) : kNone;
+}
+
+// One token by one wave: its id (or -1) in lane j < k; ids and weights stored.
+template <int V>
+__device__ __forceinline__ int select_token(const RouteArgs& a, int t, const float (&v)[V]) {
+    const int lane = threadIdx.x & 63;
+    uint32_t key[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) key[j] = key_of(v[j]);
+    float top = 0.0f, denom = 0.0f;
+    uint32_t val = kNoneKey;
     int id = -1;
     for (int r = 0; r < a.k; ++r) {
-        float best = v[0];
+        uint32_t best = key[0];
         int at = lane;
 #pragma unroll
         for (int j = 1; j < V; ++j)
-            if (v[j] > best) {
-                best = v[j];
+            if (key[j] > best) {
+                best = key[j];
                 at = j * 64 + lane;
             }
-        const float m = wave_max(best);
+        const uint32_t m = wave_max(best);
         if (r == 0) {
-            top = m;
+            top = value_of(m);
             if (!a.renormalize && !a.sigmoid) {  // softmax over all experts
                 float s = 0.0f;
 #pragma unroll
-                for (int j = 0; j < V; ++j) s += v[j] == kNone ? 0.0f : (v[j] == top ? 1.0f : expf(v[j] - top));
+                for (int j = 0; j < V; ++j) s += key[j] == kNoneKey ? 0.0f : (key[j] == m ? 1.0f : expf(value_of(key[j]) - top));
                 denom = wave_sum(s);
             }
         }
-        if (m == kNone) break;
-        const int c = wave_min(best == m ? at : 0x7fffffff);
+        if (m == kNoneKey) break;
+        const unsigned long long has = __ballot(best == m);
+        // the lane that has it; several: the lowest expert of theirs
+        const int c = (has & (has - 1)) == 0 ? __builtin_amdgcn_readlane(at, __builtin_ctzll(has)) : wave_min(best == m ? at : 0x7fffffff);
 #pragma unroll
         for (int j = 0; j < V; ++j)
-            if (c == j * 64 + lane) v[j] = kNone;
+            if (c == j * 64 + lane) key[j] = kNoneKey;
         if (lane == r) {
             val = m;
             id = c;
         }
     }
+    const float x = value_of(val);
     // (equal to the maximum: 1, also where that is infinite)
-    float w = id < 0 ? 0.0f : (a.sigmoid ? 1.0f / (1.0f + expf(-val)) : (val == top ? 1.0f : expf(val - top)));
+    float w = id < 0 ? 0.0f : (a.sigmoid ? 1.0f / (1.0f + expf(-x)) : (x == top ? 1.0f : expf(x - top)));
     if (a.renormalize) denom = wave_sum(w);
     if (a.renormalize || !a.sigmoid) w = denom > 0.0f ? w / denom : 0.0f;
     if (lane < a.k) {
@@ -177,7 +200,9 @@ __global__ __launch_bounds__(1024) void route_small_kernel(RouteArgs a, int bits
     for (int i = tid; i < waves * classes; i += blockDim.x) counts[i] = 0;
     if constexpr (DT >= 0) {
         for (int t = wave; t < a.T; t += waves) {
-            const int id = select_token<DT, V>(a, t);
+            float v[V];
+            load_token<DT, V>(a, t, v);
+            const int id = select_token<V>(a, t, v);
             if (lane < a.k) ids[t * a.k + lane] = id;
         }
     } else {
@@ -220,9 +245,15 @@ __global__ __launch_bounds__(kThreads) void route_select_kernel(RouteArgs a) {
     const int64_t t0 = (int64_t)b * a.tokens;
     const int64_t t1 = t0 + a.tokens < a.T ? t0 + a.tokens : a.T;
     if constexpr (DT >= 0) {
+        float v[V], ahead[V];  // the next token's logits arrive while this one's are selected from
+        if (t0 + wave < t1) load_token<DT, V>(a, (int)(t0 + wave), v);
         for (int64_t t = t0 + wave; t < t1; t += kThreads / 64) {
-            const int id = select_token<DT, V>(a, (int)t);
+            const int64_t next = t + kThreads / 64;
+            load_token<DT, V>(a, (int)(next < t1 ? next : t), ahead);
+            const int id = select_token<V>(a, (int)t, v);
             if (lane < a.k) atomicAdd(&lds[class_of(id, a.E)], 1);
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = ahead[j];
         }
     } else {
         for (int64_t i = t0 * a.k + threadIdx.x; i < t1 * a.k; i += kThreads) atomicAdd(&lds[class_of(a.ids[i], a.E)], 1);
@@ -242,12 +273,24 @@ __global__ __launch_bounds__(kThreads) void route_sort_kernel(RouteArgs a, int b
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     for (int i = tid; i < WAVES * classes; i += kThreads) counts[i] = 0;
     // a wave per class: lane l has the counts of blocks 4 l .. 4 l + 3 (at most 256 blocks, a multiple of 4)
-    for (int e = wave; e < classes; e += WAVES) {
-        int4 v = int4{0, 0, 0, 0};
-        if (4 * lane < a.blocks) v = *(const int4*)(a.counts + (int64_t)e * a.blocks + 4 * lane);
-        const int upto = wave_inclusive_sum(v.x + v.y + v.z + v.w);
-        if (lane == 63) totals[e] = upto;
-        if (lane == b >> 2) next[e] = upto - (v.x + v.y + v.z + v.w) + ((b & 3) > 0 ? v.x : 0) + ((b & 3) > 1 ? v.y : 0) + ((b & 3) > 2 ? v.z : 0);
+    constexpr int AHEAD = 8;  // classes whose counts a wave has in flight
+    for (int e0 = wave; e0 < classes; e0 += AHEAD * WAVES) {
+        int4 c[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int e = e0 + i * WAVES;
+            c[i] = int4{0, 0, 0, 0};
+            if (4 * lane < a.blocks && e < classes) c[i] = *(const int4*)(a.counts + (int64_t)e * a.blocks + 4 * lane);
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int e = e0 + i * WAVES;
+            const int4 v = c[i];
+            const int upto = wave_inclusive_sum(v.x + v.y + v.z + v.w);
+            if (e >= classes) continue;
+            if (lane == 63) totals[e] = upto;
+            if (lane == b >> 2) next[e] = upto - (v.x + v.y + v.z + v.w) + ((b & 3) > 0 ? v.x : 0) + ((b & 3) > 1 ? v.y : 0) + ((b & 3) > 2 ? v.z : 0);
+        }
     }
     __syncthreads();
     scan_classes(totals, classes);
