@@ -10,11 +10,13 @@
 //    front of it.  The barrier of a stage stands before its last K-step, whose fragments are in registers by then: the
 //    matrix pipe has work while the waves meet and the first fragments of the next stage arrive.
 //  * W4: the packed words lie in LDS as they are in memory (a word = 8 K-values of a column = a lane's share of a
-//    K-step's operand) and are dequantised into the operand registers between the MFMAs, w = s q + z in fp32 for bf16,
-//    in packed fp16 for fp16, rounded once to the activation type, as the dense layers' tiled GEMM does: 2^-9 (bf16) of
-//    each weight at most, which makes the error of a sum 1.4 times that of rounding the result alone.  (Codes with the
-//    constants applied to the sums, as in the streaming kernel, would need a second set of accumulators: 128 rows would
-//    no longer fit two workgroups on a CU, and with one the call below takes 1190 us.)
+//    K-step's operand) and are dequantised into the operand registers between the MFMAs, w = s q + z, rounded once to the
+//    activation type, as the dense layers' tiled GEMM does: 2^-8 (bf16) or 2^-11 (fp16) of each weight at most, which makes
+//    the error of a sum 1.4 times that of rounding the result alone.  (Codes with the constants applied to the sums, as in
+//    the streaming kernel, would need a second set of accumulators: 128 rows would no longer fit two workgroups on a CU, and
+//    with one the call below takes 1190 us.)  bf16: in fp32, then converted.  fp16: one packed fma where z is an fp16 value
+//    as it stands; where it is a product zero * s (Z32) in fp32 as for bf16, since that product rounded to fp16 first would be
+//    an error that all codes of a group share and that grows with the sum of the activations.
 //  * F8: v_mfma_f32_16x16x128 starts from zero on every 128-block and its result joins the fp32 sum times the block's two
 //    scales.
 //  * gridDim.y splits K where the tiles do not fill the chip (fp32 sums to the workspace, added in order by the
@@ -74,12 +76,13 @@ struct GemmShape {
 };
 
 // One tile of up to BM rows x BN columns.
-template <int FMT, bool BF16, int BM, int BN>
+template <int FMT, bool BF16, bool Z32, int BM, int BN>
 __device__ __forceinline__ void gemm_tile(const ExpertArgs& a, const ExpertTile& tile, int ct, unsigned char* smem) {
     using SH = GemmShape<FMT, BM, BN>;
     constexpr int WAVES = SH::WAVES;
     constexpr int RING = SH::RING, LPS = SH::LPS, WC = SH::WC, WM = SH::WM;
     constexpr bool F8 = FMT == kEF8, W4 = FMT == kEW4;
+    constexpr bool W32 = BF16 || Z32;                  // W4: weights computed in fp32
     constexpr int MT = F8 ? 16 : 32;                   // MFMA tile edge
     constexpr int TI = WM / MT, TJ = WC / MT;
     constexpr int KS = F8 ? 128 : 64;                  // K-values per stage
@@ -307,7 +310,7 @@ __device__ __forceinline__ void gemm_tile(const ExpertArgs& a, const ExpertTile&
         };
         // W4: words of the K-step at hand and the next one, constants of the stage's two 32-halves
         uint32_t words[2][TJ];
-        ColMeta<BF16> meta[2][TJ];
+        ColMeta<W32> meta[2][TJ];
         uint32_t raw_s[2][TJ], raw_z[2][TJ];
         auto read_words = [&](const unsigned char* base, int s, int buf) __attribute__((always_inline)) {
 #pragma unroll
@@ -328,17 +331,17 @@ __device__ __forceinline__ void gemm_tile(const ExpertArgs& a, const ExpertTile&
                 const float s = low16<BF16>(raw_s[h][j]);
                 float z = low16<BF16>(raw_z[h][j]);
                 z = a.zeros == nullptr ? 0.0f : z * __builtin_fmaf(a.c2, s, a.c1);
-                meta[h][j] = make_meta<BF16, 0>(s, z);
+                meta[h][j] = make_meta<W32, 0>(s, z);
             }
         };
         uint32_t nat_mask = 0x00F0000Fu, nat_magic = 0x54006400u;
         asm volatile("" : "+s"(nat_mask), "+v"(nat_magic));
         // register q (codes 2q, 2q + 1) of the operand of column set j
-        auto dequant = [&](uint32_t w, const ColMeta<BF16>& m, int q) __attribute__((always_inline)) -> uint32_t {
-            if constexpr (BF16) {
+        auto dequant = [&](uint32_t w, const ColMeta<W32>& m, int q) __attribute__((always_inline)) -> uint32_t {
+            if constexpr (W32) {
                 uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
                 asm("" : "+v"(lo), "+v"(hi));  // opaque: whole bytes, so that each is one v_cvt_f32_ubyte
-                return pack_bf16x2(__builtin_fmaf((float)((lo >> (8 * q)) & 0xffu), m.s, m.z), __builtin_fmaf((float)((hi >> (8 * q)) & 0xffu), m.s, m.z));
+                return pack16<BF16>(__builtin_fmaf((float)((lo >> (8 * q)) & 0xffu), m.s, m.z), __builtin_fmaf((float)((hi >> (8 * q)) & 0xffu), m.s, m.z));
             } else {
                 return dequant_pair<BF16>((__builtin_amdgcn_perm(w, w, 0x0c000c00u | (q << 16) | q) & nat_mask) | nat_magic, m, 1024.0f, 64.0f);
             }
@@ -478,7 +481,7 @@ __device__ __forceinline__ void gemm_tile(const ExpertArgs& a, const ExpertTile&
 
 // Workgroup tile of at most BM rows x BN columns.  A tile with fewer rows than a shorter tile has (an expert's last one)
 // runs as that: 8200 rows on 16 experts of 4096^2, 16-bit, took 329 us when every tile cost as much as a full one.
-template <int FMT, bool BF16, int BM, int BN>
+template <int FMT, bool BF16, bool Z32, int BM, int BN>
 __global__ __launch_bounds__((GemmShape<FMT, BM, BN>::THREADS)) void experts_gemm_kernel(ExpertArgs a, int tiles_n) {
     extern __shared__ __align__(16) unsigned char smem[];
     int ct = 0;
@@ -506,20 +509,20 @@ __global__ __launch_bounds__((GemmShape<FMT, BM, BN>::THREADS)) void experts_gem
     }
     if constexpr (BM >= 256) {
         if (rows > 128) {
-            gemm_tile<FMT, BF16, 256, BN>(a, tile, ct, smem);
+            gemm_tile<FMT, BF16, Z32, 256, BN>(a, tile, ct, smem);
             return;
         }
     }
     if constexpr (BM >= 128) {
         if (rows > 64) {
-            gemm_tile<FMT, BF16, 128, BN>(a, tile, ct, smem);
+            gemm_tile<FMT, BF16, Z32, 128, BN>(a, tile, ct, smem);
             return;
         }
     }
-    gemm_tile<FMT, BF16, 64, BN>(a, tile, ct, smem);
+    gemm_tile<FMT, BF16, Z32, 64, BN>(a, tile, ct, smem);
 }
 
-template <int FMT, bool BF16, int BM, int BN>
+template <int FMT, bool BF16, bool Z32, int BM, int BN>
 int launch_one(const ExpertArgs& a, hipStream_t stream) {
     constexpr int L64 = GemmShape<FMT, 64, BN>::LDS, L128 = BM >= 128 ? GemmShape<FMT, 128, BN>::LDS : 0, L256 = BM >= 256 ? GemmShape<FMT, 256, BN>::LDS : 0;
     constexpr int LA = L64 > L128 ? L64 : L128, LDS = LA > L256 ? LA : L256;
@@ -531,7 +534,7 @@ int launch_one(const ExpertArgs& a, hipStream_t stream) {
         set_error("experts: %lld tiles exceed the grid", (long long)grid);
         return GLA_ERR_INVALID_ARGUMENT;
     }
-    const auto kernel = experts_gemm_kernel<FMT, BF16, BM, BN>;
+    const auto kernel = experts_gemm_kernel<FMT, BF16, Z32, BM, BN>;
     static DeviceOnce once;
     if (once.first()) {
         const int rc = check_hip(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS), "hipFuncSetAttribute");
@@ -545,20 +548,22 @@ int launch_one(const ExpertArgs& a, hipStream_t stream) {
 // two workgroups share a CU and one starts while the other streams (256 tokens, 16 experts of 4096^2, 16-bit: 105 -> 98 us;
 // 64 tokens top 8 of 128, fp8 2048 -> 2 x 768: 64 -> 57 us).  4-bit weights fill LDS less and do better on 256 columns
 // (64 tokens top 2 of 8, 4096 -> 2 x 14336: 160 against 182 us), as do all taller tiles, which read least from LDS that way.
-template <int FMT, bool BF16>
+template <int FMT, bool BF16, bool Z32 = false>
 int launch_bm(const ExpertArgs& a, int bm, hipStream_t stream) {
     if constexpr (FMT != kEW4) {
-        if (bm >= 256) return launch_one<FMT, BF16, 256, 256>(a, stream);
+        if (bm >= 256) return launch_one<FMT, BF16, Z32, 256, 256>(a, stream);
     }
-    if (bm >= 128) return launch_one<FMT, BF16, 128, 256>(a, stream);
-    return launch_one<FMT, BF16, 64, FMT == kEW4 ? 256 : 128>(a, stream);
+    if (bm >= 128) return launch_one<FMT, BF16, Z32, 128, 256>(a, stream);
+    return launch_one<FMT, BF16, Z32, 64, FMT == kEW4 ? 256 : 128>(a, stream);
 }
 
 }  // namespace
 
 int launch_experts_gemm(const ExpertArgs& a, int format, bool bf16, int bm, hipStream_t stream) {
     switch (format) {
-        case kEW4: return bf16 ? launch_bm<kEW4, true>(a, bm, stream) : launch_bm<kEW4, false>(a, bm, stream);
+        case kEW4:
+            if (bf16) return launch_bm<kEW4, true>(a, bm, stream);
+            return a.c2 != 0.0f && a.zeros != nullptr ? launch_bm<kEW4, false, true>(a, bm, stream) : launch_bm<kEW4, false>(a, bm, stream);
         case kEF8: return bf16 ? launch_bm<kEF8, true>(a, bm, stream) : launch_bm<kEF8, false>(a, bm, stream);
         default: return bf16 ? launch_bm<kE16, true>(a, bm, stream) : launch_bm<kE16, false>(a, bm, stream);
     }

@@ -1,0 +1,62 @@
+"""Mixture-of-experts operators on the GPU at the edges of what callers may pass: activations with a mean, values that are not
+finite, offsets that are a slice of longer ones, single rows of odd strides, tall tiles filled to the end.
+
+Plain 64-bit computations and tolerances are those of ``test_gpu_experts`` (derived at its top)."""
+import pytest
+import torch
+
+import gemlite_amd
+from gemlite_amd import DType, ExpertPlan, GemLiteExperts, GemLiteLinear, GemLiteMoE, _ext, experts as experts_module
+from gemlite_amd.helper import A16W4_HQQ_INT
+from test_gpu_experts import DT, FORMATS, _gen, check, make_ids, make_layers, make_x, ref_plan, ref_route, ref_rows, run_case, silu
+
+pytestmark = pytest.mark.gpu
+
+# a tile configuration of every product kernel: streaming kernel (4- and 16-row tiles, with K splits), tiled GEMM
+KERNELS = [4, 16, 2016, 64, 2064, 128, 256]
+
+
+# ---------------------------------------------------------------------------
+# 4-bit weights with a zero point in codes
+# ---------------------------------------------------------------------------
+def shifted_layers(kind, dtype, E, K, N, gs, seed=0):
+    """E layers whose weights are (q - zero) * scale, and these weights [E, K, N] in float64."""
+    g = _gen(seed)
+    dt, gdt = DT[dtype]
+    layers, weights = [], []
+    for _ in range(E):
+        q = torch.randint(0, 16, (N, K), generator=g, dtype=torch.int32).to(torch.uint8)
+        if kind == "channelwise":     # fractional zeros, one scale per output channel
+            s = ((0.5 + torch.rand((N, 1), generator=g)) / (4.6 * K ** 0.5)).to(dt)
+            z = (torch.rand((N, 1), generator=g) * 3 + 6).to(dt)
+            layer = A16W4_HQQ_INT(device="cuda", dtype=dt).from_weights(q.cuda(), s.cuda(), z.cuda())
+            w = (q.double() - z.double()) * s.double()
+        else:                         # one integer zero for all groups
+            s = ((0.5 + torch.rand((N * K // gs, 1), generator=g)) / (4.6 * K ** 0.5)).to(dt)
+            layer = GemLiteLinear(4, gs, K, N, gdt, gdt).pack(q.cuda(), s.cuda(), 7)
+            w = ((q.double() - 7).view(N, K // gs, gs) * s.double().view(N, K // gs, 1)).view(N, K)
+        layers.append(layer)
+        weights.append(w.t())
+    return layers, torch.stack(weights)
+
+
+@pytest.mark.parametrize("kind", ["channelwise", "integer"])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("tile_config", [16, 64, 128])
+def test_shifted_codes_and_activations_with_a_mean(kind, dtype, tile_config):
+    """Every weight is rounded to the activation type at most once: an error of zero * scale, the same for all codes of a
+    group, would add up with the sum of the activations.  The roundings of the weights and the result are independent and
+    uniform, 0.58 u each: 0.82 u in the 2-norm, below u as in ``test_gpu_experts``."""
+    E, R, K, N = 2, 150, 2048, 96
+    layers, W = shifted_layers(kind, dtype, E, K, N, 128)
+    e = GemLiteExperts.from_layers(layers)
+    assert e.meta_args[10] == 3
+    u = torch.finfo(DT[dtype][0]).eps / 2
+    x = (make_x(R, K, "bf16").float() + 1).to(DT[dtype][0])
+    offsets = torch.tensor([0, 70, R], dtype=torch.int32)
+    y, mag = ref_rows("w4", x, W, offsets)
+    s = max(float(layer.scales.data.abs().max()) for layer in layers)
+    off = 128 if dtype == "bf16" else 1024
+    slack = u * mag + K * 2.0 ** -24 * x.double().abs().sum(1, keepdim=True) * ((off + 15) * s + 16 * s)
+    out = gemlite_amd.experts_functional(x.cuda(), None, e.get_tensor_args(), e.get_meta_args(), offsets.cuda(), tile_config=tile_config)
+    check(out, y, slack, u, u)
