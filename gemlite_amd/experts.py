@@ -159,6 +159,8 @@ def _prepare(mode, x, fits, bias, tensor_args, meta_args, offsets, plan, tile_co
         raise ValueError(f"x: rows of {x.shape[1]} values for experts with K={K}")
     if x.dtype not in (torch.float16, torch.bfloat16):
         raise NotImplementedError(f"experts take fp16 or bf16 activations, got {x.dtype}")
+    if nbits == 16 and W_q.dtype != x.dtype:
+        raise NotImplementedError(f"16-bit experts of {W_q.dtype} take activations of that type, got {x.dtype}")
     for name, t in (("W_q", W_q), ("scales", scales), ("zeros", zeros), ("bias", bias)):
         if t is not None and t.numel() > 0 and t.device != x.device:
             raise ValueError(f"{name} is on {t.device}, x on {x.device}")
