@@ -372,7 +372,7 @@ int gla_route_experts(const void* logits, int dtype, int64_t stride, int T, int 
         set_error("route: top_k=%d of %d experts, scoring %d", top_k, E, scoring);
         return GLA_ERR_INVALID_ARGUMENT;
     }
-    if (T > 0 && (logits == nullptr || weights == nullptr || stride < E)) {
+    if (T > 0 && (logits == nullptr || weights == nullptr || (T > 1 && stride < E))) {
         set_error("route: NULL pointer, or rows %lld apart with %d logits", (long long)stride, E);
         return GLA_ERR_INVALID_ARGUMENT;
     }

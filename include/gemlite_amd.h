@@ -321,7 +321,7 @@ int gla_unpack_over_cols(const void* packed, uint8_t* out, int64_t rows, int64_t
 #define GLA_SCORING_SIGMOID 1
 
 /* ids[T, top_k] / weights[T, top_k]: the top_k largest of each row of logits [T, E] (fp32, fp16 or bf16, rows
- * stride_t elements apart), largest first, ties to the lower expert; NaN and -inf are never chosen (id -1, weight 0).
+ * stride_t elements apart, not read for T = 1), largest first, ties to the lower expert; NaN and -inf are never chosen (id -1, weight 0).
  * weights: softmax or sigmoid in fp32, divided by their sum over the chosen ones if `renormalize`, times `scale`.
  * Then the plan of these ids: offsets [E + 1], order [T * top_k], places [T * top_k].  top_k <= 64.
  * workspace: gla_route_workspace_bytes(T, E, top_k) bytes (0 for small calls), 16-byte aligned, contents arbitrary. */

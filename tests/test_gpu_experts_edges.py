@@ -60,3 +60,11 @@ def test_shifted_codes_and_activations_with_a_mean(kind, dtype, tile_config):
     slack = u * mag + K * 2.0 ** -24 * x.double().abs().sum(1, keepdim=True) * ((off + 15) * s + 16 * s)
     out = gemlite_amd.experts_functional(x.cuda(), None, e.get_tensor_args(), e.get_meta_args(), offsets.cuda(), tile_config=tile_config)
     check(out, y, slack, u, u)
+
+
+def test_route_of_one_row_of_any_stride():
+    """A [1, E] row is contiguous whatever its row stride says (a transposed [E, 1] product has 1)."""
+    values = torch.randn(64, generator=_gen(0)).cuda()
+    want = gemlite_amd.route_experts(values[:16].view(1, 16), 4)
+    for row in (values[:16].view(16, 1).t(), values.as_strided((1, 16), (0, 1)), values.as_strided((1, 16), (64, 1))):
+        assert row.stride(0) != 16 and all(torch.equal(a, b) for a, b in zip(gemlite_amd.route_experts(row, 4), want))
