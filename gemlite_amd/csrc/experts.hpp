@@ -167,10 +167,12 @@ __device__ __forceinline__ uint32_t magnitude_max(uint32_t m, uint32_t v) {
 }
 
 // The scale and the reciprocal that a block of 128 activations of amax is quantised with (NaN if it holds one).  (The
-// constant's reciprocal, not a division: the codes of values that lie on a border between two depend on it.)
+// constant's reciprocal, not a division: the codes of values that lie on a border between two depend on it.)  An infinity
+// would be the code of inf * (1 / inf), a NaN, which the clamp to the codes' range loses: the scale is NaN in its place.
 __device__ __forceinline__ void block_scale(float amax, float& s, float& inv) {
     s = amax * (1.0f / 448.0f);
     s = s < 1e-6f ? 1e-6f : s;
+    s = s < __builtin_inff() ? s : __builtin_nanf("");
     inv = 1.0f / s;
 }
 

@@ -68,3 +68,32 @@ def test_route_of_one_row_of_any_stride():
     want = gemlite_amd.route_experts(values[:16].view(1, 16), 4)
     for row in (values[:16].view(16, 1).t(), values.as_strided((1, 16), (0, 1)), values.as_strided((1, 16), (64, 1))):
         assert row.stride(0) != 16 and all(torch.equal(a, b) for a, b in zip(gemlite_amd.route_experts(row, 4), want))
+
+
+# ---------------------------------------------------------------------------
+# values that are not finite
+# ---------------------------------------------------------------------------
+def same_kind(y, ref):
+    """NaN, +inf and -inf in the same places (``ref`` in 64 bits, sums of moderate size otherwise)."""
+    y = y.cpu().double()
+    return torch.equal(torch.isnan(y), torch.isnan(ref)) and torch.equal(torch.isposinf(y), torch.isposinf(ref)) and torch.equal(
+        torch.isneginf(y), torch.isneginf(ref))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("tile_config", KERNELS)
+def test_infinite_activations_of_fp8_experts(dtype, tile_config):
+    """s = inf / 448 = inf, 1 / s = 0, code = e4m3(inf * 0) = NaN: a block with an infinity is NaN by the definition."""
+    E, R, K, N = 2, 40, 512, 64
+    layers, W = make_layers("fp8", dtype, E, K, N)
+    e = GemLiteExperts.from_layers(layers)
+    off = torch.tensor([0, 13, R], dtype=torch.int32, device="cuda")
+    x = make_x(R, K, dtype).cuda()
+    args = (None, e.get_tensor_args(), e.get_meta_args(), off)
+    clean = gemlite_amd.experts_functional(x, *args, tile_config=tile_config)
+    x[3, 200], x[20, 7], x[30, 511], x[30, 0] = float("inf"), float("-inf"), float("inf"), float("-inf")
+    out = gemlite_amd.experts_functional(x, *args, tile_config=tile_config)
+    odd = torch.zeros(R, dtype=torch.bool, device="cuda")
+    odd[[3, 20, 30]] = True
+    assert torch.equal(out[~odd], clean[~odd])
+    assert bool(torch.isnan(out[odd]).all())
