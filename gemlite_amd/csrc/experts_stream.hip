@@ -312,6 +312,49 @@ __global__ __launch_bounds__(NW * 64, 2) void experts_stream_kernel(ExpertArgs a
             unit(ring + at * SLOT, []() __attribute__((always_inline)) {});
             at = at == D - 1 ? 0 : at + 1;
         }
+        if constexpr (FMT == kEW4) {
+            // A sum that is not finite may be so only because of the codes' offset (inf - inf, or an overflow of 128 x): such
+            // sums are taken again from dequantised weights, rounded to 16 bits as in the tiled GEMM.
+            bool odd = false;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) odd = odd || !(__builtin_fabsf(acc[t][r]) < __builtin_inff());
+            if (__any(odd)) {
+                const int col = unit_column_inside<WC>(a.half, a.N, ct, 4 * cg);
+                int row = tile.row0 + cg;
+                if (row > tile.row_end - 1) row = tile.row_end - 1;
+                const unsigned char* x = a.x + source_row(a, row) * a.xsm + kb * 16;
+                float4_t plain[NT];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) plain[t] = zero4;
+                const int k1 = u1 * 128 < a.K ? u1 * 128 : a.K;
+#pragma unroll 1
+                for (int k = u0 * 128; k < k1; k += 32) {
+                    const u32x4 w = *(const u32x4*)(we + ((int64_t)(k / 8 + kb) * a.N + col) * 4);
+                    const int64_t at = ((int64_t)(k / a.group) * a.N + col) * 2;
+                    const u32x2 rs = *(const u32x2*)(se + at), rz = *(const u32x2*)(ze + at);
+                    const u32x4 xa = pairs_of(*(const u32x4*)(x + (int64_t)k * 2));
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        const float sc = t & 1 ? high16<BF16>(rs[t / 2]) : low16<BF16>(rs[t / 2]);
+                        float zp = t & 1 ? high16<BF16>(rz[t / 2]) : low16<BF16>(rz[t / 2]);
+                        zp = a.zeros == nullptr ? 0.0f : zp * __builtin_fmaf(a.c2, sc, a.c1);
+                        u32x4 q;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            q[j] = pack16<BF16>(__builtin_fmaf((float)((w[t] >> (4 * j)) & 15u), sc, zp),
+                                                __builtin_fmaf((float)((w[t] >> (4 * j + 16)) & 15u), sc, zp));
+                        plain[t] = mfma16<BF16>(xa, q, plain[t]);
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (!(__builtin_fabsf(acc[t][r]) < __builtin_inff())) acc[t][r] = plain[t][r];
+            }
+        }
         __syncthreads();  // every ring is done
 
         // ---- the waves' sums.  W4: the lane holds rows 4 kb + r of columns 4 cg + t; else (weights were the row operand)

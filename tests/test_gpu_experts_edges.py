@@ -97,3 +97,43 @@ def test_infinite_activations_of_fp8_experts(dtype, tile_config):
     odd[[3, 20, 30]] = True
     assert torch.equal(out[~odd], clean[~odd])
     assert bool(torch.isnan(out[odd]).all())
+
+
+@pytest.mark.parametrize("fmt", ["w4", "h16"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("tile_config", KERNELS)
+def test_infinite_activations_of_unquantised_rows(fmt, dtype, tile_config):
+    """An infinity times a weight is an infinity of its sign in every kernel, two of opposite sign make NaN."""
+    E, R, K, N = 2, 40, 512, 64
+    layers, W = make_layers(fmt, dtype, E, K, N, 64)
+    e = GemLiteExperts.from_layers(layers)
+    offsets = torch.tensor([0, 13, R], dtype=torch.int32)
+    x = make_x(R, K, dtype)
+    args = (None, e.get_tensor_args(), e.get_meta_args(), offsets.cuda())
+    clean = gemlite_amd.experts_functional(x.cuda(), *args, tile_config=tile_config)
+    x[3, 200], x[20, 7], x[30, 511], x[30, 0], x[39, 100] = float("inf"), float("-inf"), float("inf"), float("-inf"), float("nan")
+    out = gemlite_amd.experts_functional(x.cuda(), *args, tile_config=tile_config)
+    odd = torch.zeros(R, dtype=torch.bool)
+    odd[[3, 20, 30, 39]] = True
+    assert torch.equal(out.cpu()[~odd], clean.cpu()[~odd])
+    assert same_kind(out, ref_rows(fmt, x, W, offsets)[0])
+
+
+@pytest.mark.parametrize("tile_config", KERNELS)
+def test_large_activations_of_4_bit_experts(tile_config):
+    """Values whose product with a code of 128 + q would overflow fp32 while that with the weight does not."""
+    E, R, K, N = 2, 24, 256, 64
+    layers, W = make_layers("w4", "bf16", E, K, N, 64)
+    e = GemLiteExperts.from_layers(layers)
+    offsets = torch.tensor([0, 13, R], dtype=torch.int32)
+    x = make_x(R, K, "bf16")
+    x[5] = 0
+    x[5, 17] = 2.0 ** 124          # 128 of it: 2^131
+    x[20, 3], x[20, 4] = 2.0 ** 122, -(2.0 ** 123)
+    y, mag = ref_rows("w4", x, W, offsets)
+    u = 2.0 ** -8
+    assert float(y.abs().max()) < 2.0 ** 127
+    out = gemlite_amd.experts_functional(x.cuda(), None, e.get_tensor_args(), e.get_meta_args(), offsets.cuda(), tile_config=tile_config).cpu().double()
+    # (one rounding of each weight and one of the result; fp32 sums of these few terms of one size)
+    for r in (5, 20):
+        assert bool(((out[r] - y[r]).abs() <= (2 * u + K * 2.0 ** -24) * mag[r]).all())
