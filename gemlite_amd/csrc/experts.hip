@@ -29,6 +29,7 @@ __global__ __launch_bounds__(256) void experts_finish_kernel(FinishArgs a) {
     const int width = a.half ? a.half : a.N;
     const int c = (blockIdx.y * 256 + threadIdx.x) * 4;
     if (c >= width) return;
+    const int from = a.offsets[0] > 0 ? a.offsets[0] : 0;  // rows outside from .. limit - 1 have no expert
     int limit = a.offsets[a.E];
     if (limit > a.R) limit = a.R;
     const int64_t slab = (int64_t)a.R * a.N;
@@ -42,13 +43,13 @@ __global__ __launch_bounds__(256) void experts_finish_kernel(FinishArgs a) {
     if constexpr (COMBINED) {
         for (int j = 0; j < a.k; ++j) {
             const int p = a.places[row * a.k + j];
-            if (p < 0 || p >= limit) continue;
+            if (p < from || p >= limit) continue;
             const float w = a.weights[row * a.k + j];
             const float4_t y = sum_at(p, c);
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] = __builtin_fmaf(w, y[i], v[i]);
         }
-    } else if (row < limit) {
+    } else if (row >= from && row < limit) {
         v = sum_at(row, c);
         if (a.half) {
             const float4_t up = sum_at(row, c + a.half);

@@ -1,8 +1,8 @@
 // Products grouped by expert: what the streaming kernel (experts_stream.hip), the tiled GEMM (experts_gemm.hip), the
 // finishing kernel and the host side (experts.hip) share.
 //
-// The R rows of a call are sorted by expert: rows offsets[e] .. offsets[e + 1] - 1 meet the weights of expert e, rows from
-// offsets[E] on meet none.  offsets lives on the device, so the host knows only R and E: a launch has as many row tiles
+// The R rows of a call are sorted by expert: rows offsets[e] .. offsets[e + 1] - 1 meet the weights of expert e, rows in front
+// of offsets[0] and from offsets[E] on meet none.  offsets lives on the device, so the host knows only R and E: a launch has as many row tiles
 // as any distribution can need, and a workgroup finds its tile (expert, first row, last row) from offsets itself.
 #pragma once
 
@@ -42,7 +42,7 @@ struct ExpertArgs {
 
 // Sum of the row tiles of all experts for BM-row tiles, at most (host): a experts with rows need a + floor((R - a) / BM).
 inline int64_t max_row_tiles(int64_t R, int E, int BM) {
-    const int64_t a = R < (int64_t)E + 1 ? R : (int64_t)E + 1;  // rows without an expert count as one more
+    const int64_t a = R < (int64_t)E + 2 ? R : (int64_t)E + 2;  // rows without an expert count as two more: in front, behind
     return a + (R - a) / BM;
 }
 
@@ -67,8 +67,9 @@ struct ExpertTile {
 
 // The row tile `pick(total)` of the call's `total` ones, computed by every wave for itself: lane l counts the tiles of
 // experts l C .. l C + C - 1 (C = 1 up to 63 experts), an inclusive sum over the lanes finds the lane, that lane the
-// expert.  Offsets are clamped to 0 .. R and to rising order, so no tile leaves the R rows whatever they hold.  One round
-// trip to memory and about a hundred vector instructions; a table written by the routing kernel would cost the same round
+// expert; the tiles of the rows in front of offsets[0] come last.  Offsets are clamped to 0 .. R and an expert whose end
+// is not behind its begin has no tiles, so no tile leaves the R rows whatever they hold (where they do not rise, rows may have
+// several tiles or none).  One round trip to memory and about a hundred vector instructions; a table written by the routing kernel would cost the same round
 // trip.
 template <int BM, typename Pick>
 __device__ __forceinline__ ExpertTile find_tile(const int32_t* offsets, int E, int R, bool with_rest, Pick pick) {
@@ -93,11 +94,18 @@ __device__ __forceinline__ ExpertTile find_tile(const int32_t* offsets, int E, i
     }
     const int upto = wave_inclusive_sum(mine);
     ExpertTile r;
-    r.total = __builtin_amdgcn_readlane(upto, 63);
+    const int first = with_rest ? __builtin_amdgcn_readfirstlane(at(0)) : 0, of_experts = __builtin_amdgcn_readlane(upto, 63);
+    r.total = of_experts + (first + BM - 1) / BM;
     const int t = pick(r.total);
     if (t < 0 || t >= r.total) {
         r.expert = -1;
         r.row0 = r.row_end = 0;
+        return r;
+    }
+    if (t >= of_experts) {
+        r.expert = E;
+        r.row0 = (t - of_experts) * BM;
+        r.row_end = r.row0 + BM < first ? r.row0 + BM : first;
         return r;
     }
     const int owner = __builtin_ctzll(__ballot(upto > t));

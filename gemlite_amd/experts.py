@@ -250,7 +250,8 @@ def _launch(mode, x, bias, tensor_args, meta_args, offsets, plan, tile_config):
 def experts_functional(x: Tensor, bias: Optional[Tensor], tensor_args: List[Tensor], meta_args: List[int], offsets: Tensor,
                        tile_config: int = -1) -> Tensor:
     """``out[r] = x[r] @ W[e(r)] (+ bias[e(r)])`` for rows [R, K] that are already grouped by expert: rows
-    ``offsets[e] .. offsets[e + 1] - 1`` are expert ``e``'s, rows from ``offsets[E]`` on come out as zeros.
+    ``offsets[e] .. offsets[e + 1] - 1`` are expert ``e``'s, rows from ``offsets[E]`` on and in front of ``offsets[0]`` (above 0
+    in a slice of longer offsets) come out as zeros.
 
     ``tensor_args = [W_q, scales, zeros]`` and ``meta_args`` are those of ``GemLiteLinear`` with a leading axis of experts
     on every tensor; ``bias`` is [E, N] fp32 and is added before the result is rounded.  fp8 experts quantise every row of

@@ -314,7 +314,8 @@ int gla_unpack_over_cols(const void* packed, uint8_t* out, int64_t rows, int64_t
  * A plan sorts the R = T * top_k (token, slot) pairs by expert: order[p] is the flat index token * top_k + slot of
  * sorted row p (within an expert in rising order), places[token * top_k + slot] the sorted row of a pair, and rows
  * offsets[e] .. offsets[e + 1] - 1 belong to expert e.  Pairs without an expert (id < 0 or >= E) come last, from
- * offsets[E] on.  offsets, order and places are device memory; the kernels keep whatever they hold inside the R rows. */
+ * offsets[E] on.  (Offsets made elsewhere may start above 0, as a slice of longer ones does: rows in front of offsets[0]
+ * have no expert either.)  offsets, order and places are device memory; the kernels keep whatever they hold inside the R rows. */
 #define GLA_EXPERTS_MAX 1024
 
 #define GLA_SCORING_SOFTMAX 0

@@ -137,3 +137,54 @@ def test_large_activations_of_4_bit_experts(tile_config):
     # (one rounding of each weight and one of the result; fp32 sums of these few terms of one size)
     for r in (5, 20):
         assert bool(((out[r] - y[r]).abs() <= (2 * u + K * 2.0 ** -24) * mag[r]).all())
+
+
+# ---------------------------------------------------------------------------
+# offsets that do not start at the first row
+# ---------------------------------------------------------------------------
+def poison(*shapes):
+    """Leave memory full of NaN to the allocator, so that rows nobody writes show."""
+    held = [torch.full(s, float("nan"), device="cuda") for s in shapes for _ in range(2)]
+    torch.cuda.synchronize()
+    del held
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("tile_config", KERNELS + [-1])
+def test_offsets_of_a_slice_of_the_experts(fmt, tile_config):
+    """Rows before offsets[0], such as those of another rank's experts, have no expert: zeros, and nothing in a combination."""
+    E, R, K, N = 4, 300, 512, 64
+    layers, _ = make_layers(fmt, "bf16", E, K, N)
+    e = GemLiteExperts.from_layers(layers)
+    x = make_x(R, K, "bf16").cuda()
+    targs, meta = e.get_tensor_args(), e.get_meta_args()
+    for first in (1, 7, 64, 70, 290):
+        off = torch.tensor([first, first, first + 5, first + 5, first + 8], dtype=torch.int32, device="cuda")
+        inner = x[first:first + 8].contiguous()
+        want = gemlite_amd.experts_functional(inner, None, targs, meta, off - first, tile_config=tile_config)
+        poison((R, N), (4, R, N), (R, N // 2), (R, K))
+        out = gemlite_amd.experts_functional(x, None, targs, meta, off, tile_config=tile_config)
+        assert not out[:first].any() and not out[first + 8:].any()
+        if tile_config != -1:     # (-1: the number of rows chooses the kernel)
+            assert torch.equal(out[first:first + 8], want)
+        order = torch.arange(R, dtype=torch.int32, device="cuda")
+        plan = ExpertPlan(torch.ones((R, 1), device="cuda"), order.view(R, 1), off, order, order.view(R, 1))
+        poison((R, N), (4, R, N), (R, N // 2), (R, K))
+        gated = gemlite_amd.experts_gated_functional(x, None, targs, meta, plan, tile_config=tile_config)
+        assert gated[first:first + 8].any() and not gated[:first].any() and not gated[first + 8:].any()
+        poison((R, N), (4, R, N), (R, N // 2), (R, K))
+        combined = gemlite_amd.experts_combined_functional(x, None, targs, meta, plan, tile_config=tile_config)
+        assert not combined[:first].any() and not combined[first + 8:].any()
+        if tile_config != -1:
+            assert torch.equal(combined[first:first + 8], want)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_every_row_in_front_of_the_first_expert(fmt):
+    E, R, K, N = 4, 200, 128, 64
+    layers, _ = make_layers(fmt, "bf16", E, K, N)
+    e = GemLiteExperts.from_layers(layers)
+    off = torch.full((E + 1,), R, dtype=torch.int32, device="cuda")
+    poison((R, N), (4, R, N))
+    assert not e(make_x(R, K, "bf16").cuda(), off).any()
