@@ -93,6 +93,10 @@ int validate(const gla_experts_args* p) {
         set_error("experts: output type %d (fp16 and bf16 are built)", p->output_dtype);
         return GLA_ERR_UNSUPPORTED_DTYPE;
     }
+    if ((gated || combined) && (p->R > 0 || p->T > 0) && (p->top_k <= 0 || (int64_t)p->T * p->top_k != p->R)) {
+        set_error("experts: T=%d tokens of %d slots are not the plan's R=%d rows", p->T, p->top_k, p->R);
+        return GLA_ERR_INVALID_ARGUMENT;
+    }
     const int fmt = format_of(*p);
     if (fmt < 0) {
         set_error("experts: W_nbits=%d elements_per_sample=%d input_dtype=%d output_dtype=%d channel_scale_mode=%d W_group_mode=%d is not built "
@@ -139,12 +143,6 @@ int validate(const gla_experts_args* p) {
         if (p->w_stride_e < expert_bytes) {
             set_error("experts: w_stride_e=%lld bytes is shorter than an expert's %lld", (long long)p->w_stride_e, (long long)expert_bytes);
             return GLA_ERR_INVALID_ARGUMENT;
-        }
-        if (gated || combined) {
-            if (p->top_k <= 0 || (int64_t)p->T * p->top_k != p->R) {
-                set_error("experts: T=%d tokens of %d slots are not the plan's R=%d rows", p->T, p->top_k, p->R);
-                return GLA_ERR_INVALID_ARGUMENT;
-            }
         }
         if (fmt == kEF8 && (!p->scales || p->meta_dtype != GLA_DT_FP32)) {
             set_error("experts: fp8 experts need fp32 block scales");

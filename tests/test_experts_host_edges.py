@@ -41,3 +41,34 @@ def test_unquantised_weights_of_another_type_than_the_activations(launches, dtyp
     with pytest.raises(NotImplementedError):
         gemlite_amd.experts_functional(x, None, [e.W_q.to(other), e.scales, e.zeros], e.get_meta_args(), off)
     assert len(launches) == 1
+
+
+def _args(**kw):
+    """Valid 4-bit arguments; the addresses are never dereferenced on the host."""
+    a = _ext.ExpertsArgs()
+    a.struct_size = ctypes.sizeof(_ext.ExpertsArgs)
+    a.mode, a.R, a.T, a.top_k, a.E, a.N, a.K = 0, 8, 4, 2, 4, 64, 256
+    a.x = a.w = a.out = a.offsets = a.order = a.places = a.weights = a.scales = a.zeros = 4096
+    a.w_stride_e, a.meta_stride_e, a.x_stride_m, a.out_stride_m = 256 * 64 // 2, 2 * 64 * 2, 256, 64
+    a.W_nbits, a.group_size, a.elements_per_sample = 4, 128, 8
+    a.input_dtype = a.output_dtype = a.meta_dtype = a.x_dtype = DType.BF16.value
+    a.W_group_mode, a.tile_config = 4, -1
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def test_tokens_without_slots_are_refused(launches):
+    """Tokens whose plan has no slots have no rows: the combination would return memory that nothing has written."""
+    lib = _ext.load_library()
+    for mode in (1, 2):
+        for top_k in (0, 2, -1):
+            bad = _args(mode=mode, R=0, T=5, top_k=top_k)
+            assert lib.gla_experts_workspace_bytes(ctypes.byref(bad)) == -1 and lib.gla_experts_matmul(ctypes.byref(bad), None) == -1
+        assert lib.gla_experts_matmul(ctypes.byref(_args(mode=mode, R=0, T=0, top_k=2)), None) == 0
+    e = _raw_experts(torch.bfloat16)
+    none = torch.empty(0, dtype=torch.int32)
+    plan = ExpertPlan(torch.empty((5, 0)), none.view(5, 0), torch.zeros(3, dtype=torch.int32), none, none.view(5, 0))
+    with pytest.raises(ValueError):
+        e.forward_combined(torch.empty((0, 64), dtype=torch.bfloat16), plan)
+    assert not launches
