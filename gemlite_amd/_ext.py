@@ -577,6 +577,9 @@ _ROUTE_WORKSPACE = {}  # (T, E, k) -> bytes
 def _route_need(T, E, k):
     need = _ROUTE_WORKSPACE.get((T, E, k))
     if need is None:
+        # (the library takes 32-bit integers, and ctypes wraps what they cannot hold)
+        if not (0 <= T * k < 2 ** 31 and 0 <= T < 2 ** 31 and 1 <= E <= 1024 and 1 <= k <= 64):
+            raise ValueError(f"a plan of {T} tokens with {k} of {E} experts each: at most 2^31 - 1 pairs, 1024 experts and 64 per token")
         need = load_library().gla_route_workspace_bytes(T, E, k)
         if need < 0:
             _check(int(need), "gla_route_workspace_bytes")

@@ -85,7 +85,7 @@ int validate(const gla_experts_args* p) {
         return GLA_ERR_UNSUPPORTED_MODE;
     }
     const bool combined = p->mode == GLA_EXPERTS_COMBINED, gated = p->mode == GLA_EXPERTS_GATED;
-    if (p->R < 0 || p->T < 0 || p->E <= 0 || p->E > GLA_EXPERTS_MAX || p->N <= 0 || p->K <= 0 || p->K > (1 << 20)) {
+    if (p->R < 0 || p->R > GLA_EXPERTS_MAX_ROWS || p->T < 0 || p->E <= 0 || p->E > GLA_EXPERTS_MAX || p->N <= 0 || p->K <= 0 || p->K > (1 << 20)) {
         set_error("experts: R=%d T=%d E=%d (1..%d) N=%d K=%d (at most 2^20)", p->R, p->T, p->E, GLA_EXPERTS_MAX, p->N, p->K);
         return GLA_ERR_INVALID_ARGUMENT;
     }

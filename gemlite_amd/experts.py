@@ -46,6 +46,7 @@ class ExpertPlan(NamedTuple):
 # ---------------------------------------------------------------------------
 def _empty_plan(like, T, k, E):
     """(ids, offsets, order, places), views of one allocation (the kernels address them element by element)."""
+    _ext._route_need(T, E, k)  # (refuses sizes that no plan can have)
     n = T * k
     ints = like.new_empty(3 * n + E + 1, dtype=torch.int32)
     return (ints.as_strided((T, k), (k, 1), 0), ints.as_strided((E + 1,), (1,), 3 * n), ints.as_strided((n,), (1,), n),
@@ -166,6 +167,9 @@ def _prepare(mode, x, fits, bias, tensor_args, meta_args, offsets, plan, tile_co
             raise ValueError(f"{name} is on {t.device}, x on {x.device}")
     device = x.device
 
+    sizes = (E, N, K, x.shape[0]) if plan is None else (E, N, K, x.shape[0], plan.places.numel(), *plan.places.shape)
+    if max(sizes) >= 2 ** 31:
+        raise ValueError(f"sizes {sizes}: the library takes 32-bit integers")
     a = _ext.ExpertsArgs()
     a.mode = mode
     a.E, a.N, a.K = E, N, K

@@ -317,6 +317,7 @@ int gla_unpack_over_cols(const void* packed, uint8_t* out, int64_t rows, int64_t
  * offsets[E] on.  (Offsets made elsewhere may start above 0, as a slice of longer ones does: rows in front of offsets[0]
  * have no expert either.)  offsets, order and places are device memory; the kernels keep whatever they hold inside the R rows. */
 #define GLA_EXPERTS_MAX 1024
+#define GLA_EXPERTS_MAX_ROWS (0x7fffffff - 1023) /* R of a product: a row index plus a tile's height stays an int */
 
 #define GLA_SCORING_SOFTMAX 0
 #define GLA_SCORING_SIGMOID 1

@@ -72,3 +72,24 @@ def test_tokens_without_slots_are_refused(launches):
     with pytest.raises(ValueError):
         e.forward_combined(torch.empty((0, 64), dtype=torch.bfloat16), plan)
     assert not launches
+
+
+def test_sizes_that_32_bits_cannot_hold(launches):
+    """Sizes reach the library as 32-bit integers: larger ones are refused, not wrapped."""
+    for T, E, k in ((2 ** 32 + 10, 8, 1), (2 ** 31, 8, 1), (2 ** 30, 8, 4), (4, 2 ** 32 + 8, 2), (4, 8, 2 ** 32 + 2)):
+        with pytest.raises(ValueError):
+            _ext._route_need(T, E, k)
+    ids, w = torch.zeros((4, 2), dtype=torch.int32), torch.ones((4, 2))
+    for experts in (2 ** 32 + 8, 1025, 0, -5):
+        for rows in (4, 0):
+            with pytest.raises(ValueError):
+                gemlite_amd.plan_experts(ids[:rows], w[:rows], experts)
+    lib = _ext.load_library()
+    for R in (2 ** 31 - 1, 2 ** 31 - 256):   # row + tile height has to stay an int
+        assert lib.gla_experts_workspace_bytes(ctypes.byref(_args(R=R))) == -1
+    with pytest.raises(ValueError):
+        meta = torch.empty((2 ** 32 + 8, 64), dtype=torch.bfloat16, device="meta")
+        e = _raw_experts(torch.bfloat16)
+        t = [v.to("meta") for v in e.get_tensor_args()]
+        gemlite_amd.experts_functional(meta, None, t, e.get_meta_args(), torch.empty(3, dtype=torch.int32, device="meta"))
+    assert not launches
