@@ -296,6 +296,7 @@ int gla_experts_matmul(const gla_experts_args* p, void* stream) {
     a.groups = h.format == kEW4 ? p->K / p->group_size : 0;
     a.group_mul = divide_mul(h.format == kEW4 ? p->group_size / 32 : 1);
     a.top_k_mul = divide_mul(p->top_k);
+    a.top_k_divides = (int64_t)p->R * p->top_k > (int64_t)1 << 32;
     a.chunk = h.chunk;
     a.stream_waves = h.waves;
     a.c1 = p->W_group_mode == GLA_WGM_FMA ? 1.0f : 0.0f;

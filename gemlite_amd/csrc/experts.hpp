@@ -34,6 +34,7 @@ struct ExpertArgs {
     int to_partials;                // raw fp32 sums to `partials` instead of finished rows to `out`
     int group;                      // W4: K-values per group (scales and zeros have the activations' type)
     uint32_t group_mul, top_k_mul;  // n / (group / 32) and n / top_k as the high half of n * this (0: see divide_by)
+    int top_k_divides;              // R * top_k passes 2^32, where top_k_mul is not exact: divide
     int groups;                     // W4: K / group
     int stream_waves;               // streaming kernel: waves of a workgroup, 4 (W4: or 2)
     int chunk;                      // streaming kernel: units of 128 K-values per wave; tiled GEMM: stages per split
@@ -130,8 +131,8 @@ __device__ __forceinline__ ExpertTile find_tile(const int32_t* offsets, int E, i
     return r;
 }
 
-// n / d with mul = ceil(2^32 / d): exact while n d < 2^32 (n below 2^26 for d up to 64).  0 stands for d = 1 (mul would
-// be 2^32).
+// n / d as the high half of n * mul, mul = ceil(2^32 / d): exact while n d < 2^32.  mul = 0 stands for d = 1 (it would be
+// 2^32).
 inline uint32_t divide_mul(uint32_t d) { return d <= 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + d - 1) / d); }
 __device__ __forceinline__ uint32_t divide_by(uint32_t n, uint32_t mul) { return mul == 0 ? n : __umulhi(n, mul); }
 
@@ -140,7 +141,7 @@ __device__ __forceinline__ int64_t source_row(const ExpertArgs& a, int r) {
     if (a.order == nullptr) return r;
     int v = a.order[r];
     v = v < 0 ? 0 : (v > a.R - 1 ? a.R - 1 : v);
-    return a.R <= (1 << 26) ? (int64_t)divide_by((uint32_t)v, a.top_k_mul) : (int64_t)(v / a.top_k);
+    return a.top_k_divides ? (int64_t)(v / a.top_k) : (int64_t)divide_by((uint32_t)v, a.top_k_mul);
 }
 
 // Column of the weights that column c of the W columns of unit u stands for: u W + c, or (gated) W / 2 gate columns

@@ -188,3 +188,28 @@ def test_every_row_in_front_of_the_first_expert(fmt):
     off = torch.full((E + 1,), R, dtype=torch.int32, device="cuda")
     poison((R, N), (4, R, N))
     assert not e(make_x(R, K, "bf16").cuda(), off).any()
+
+
+def test_many_slots_for_a_token():
+    """(token, slot) indices whose product with the number of slots passes 2^32: the token of a row is still exact."""
+    E, T, k, K, N = 2, 512, 4097, 32, 16
+    layers, W = make_layers("h16", "bf16", E, K, N)
+    e = GemLiteExperts.from_layers(layers)
+    x = make_x(T, K, "bf16")
+    R = T * k
+    slot = torch.arange(R, dtype=torch.int64, device="cuda")
+    expert = (slot % k) % E
+    order = torch.sort(expert, stable=True).indices
+    places = torch.empty_like(order)
+    places[order] = slot
+    offsets = torch.tensor([0, int((expert == 0).sum()), R], dtype=torch.int32, device="cuda")
+    plan = ExpertPlan(torch.zeros((T, k), device="cuda"), expert.view(T, k).int(), offsets, order.int(), places.view(T, k).int())
+    h = e.forward_gated(x.cuda(), plan)
+    z = torch.stack([x.double() @ W[i] for i in range(E)], 1)      # [T, E, N]
+    want = (silu(z[..., : N // 2]) * z[..., N // 2:]).cuda()
+    got = h[plan.places.view(-1).long()].view(T, k, N // 2)
+    for i in range(E):
+        mine = got[:, i::E]
+        assert bool((mine == mine[:, :1]).all())                   # every slot of a token with this expert has one result
+        err = (mine[:, 0].double() - want[:, i]).norm() / want[:, i].norm()
+        assert float(err) <= 2.0 ** -8
