@@ -11,6 +11,7 @@ and the row counts stay on the GPU.
 ``GemLiteExperts`` stacks packed ``GemLiteLinear`` layers of one kind; ``GemLiteMoE`` is the three lines above as a module.
 As everywhere in this package the products have no backward pass: outputs carry no gradient.
 """
+import logging
 import threading
 from typing import List, NamedTuple, Optional
 
@@ -20,6 +21,8 @@ from torch import Tensor
 from . import _ext
 from .core import GemLiteLinear
 from .dtypes import DType, DTYPE_TO_TORCH, TORCH_TO_DTYPE
+
+logger = logging.getLogger(__name__)
 
 SCORINGS = {"softmax": 0, "sigmoid": 1}
 _ROWS, _GATED, _COMBINED = 0, 1, 2
@@ -60,7 +63,7 @@ def route_experts(logits: Tensor, top_k: int, scoring: str = "softmax", renormal
     the remaining slots get id -1 and weight 0.  Weights are ``scoring`` ("softmax" or "sigmoid") of the logits in fp32,
     with ``renormalize`` divided by their sum over the chosen ones, times ``scale``.
     """
-    if torch.compiler.is_compiling():
+    if route_experts_op is not None and torch.compiler.is_compiling():
         return ExpertPlan(*route_experts_op(logits, top_k, scoring, renormalize, scale))
     return _route_experts(logits, top_k, scoring, renormalize, scale)
 
@@ -444,37 +447,45 @@ class GemLiteMoE(torch.nn.Module):
 # ---------------------------------------------------------------------------
 # the same calls as custom ops, so that torch.compile holds each as one node (eager calls do not pay the op dispatch)
 # ---------------------------------------------------------------------------
-@torch.library.custom_op("gemlite::route_experts", mutates_args=())
-def route_experts_op(logits: Tensor, top_k: int, scoring: str, renormalize: bool, scale: float) -> List[Tensor]:
-    # (a plan's integers are views of one allocation; the outputs of an op must not share memory)
-    return [t.clone() for t in _route_experts(logits, top_k, scoring, renormalize, scale)]
+def _make_custom_ops():
+    try:
+        @torch.library.custom_op("gemlite::route_experts", mutates_args=())
+        def route_experts_op(logits: Tensor, top_k: int, scoring: str, renormalize: bool, scale: float) -> List[Tensor]:
+            # (a plan's integers are views of one allocation; the outputs of an op must not share memory)
+            return [t.clone() for t in _route_experts(logits, top_k, scoring, renormalize, scale)]
+
+        @route_experts_op.register_fake
+        def _(logits, top_k, scoring, renormalize, scale):
+            T, E = logits.shape
+            ints = dict(dtype=torch.int32, device=logits.device)
+            return [torch.empty((T, top_k), dtype=torch.float32, device=logits.device), torch.empty((T, top_k), **ints),
+                    torch.empty((E + 1,), **ints), torch.empty((T * top_k,), **ints), torch.empty((T, top_k), **ints)]
+
+        @torch.library.custom_op("gemlite::experts", mutates_args=())
+        def experts_op(mode: int, x: Tensor, bias: Optional[Tensor], tensor_args: List[Tensor], meta_args: List[int], offsets: Tensor,
+                       plan: List[Tensor]) -> Tensor:
+            return _launch(mode, x, bias, tensor_args, meta_args, offsets, ExpertPlan(*plan) if plan else None, -1)
+
+        @experts_op.register_fake
+        def _(mode, x, bias, tensor_args, meta_args, offsets, plan):
+            N, rows = tensor_args[0].shape[2], x.shape[0]
+            if mode != _ROWS:
+                T, k = plan[4].shape
+                rows = T if mode == _COMBINED else T * k
+            return torch.empty((rows, N // 2 if mode == _GATED else N), dtype=DTYPE_TO_TORCH[int(meta_args[6])], device=x.device)
+
+        return route_experts_op, experts_op
+    except Exception as exc:  # a name is taken or torch is too old
+        logger.warning("gemlite_amd: torch custom ops gemlite::route_experts and gemlite::experts were not registered (%s); "
+                       "torch.compile will trace into the plain Python calls", exc)
+        return None, None
 
 
-@route_experts_op.register_fake
-def _(logits, top_k, scoring, renormalize, scale):
-    T, E = logits.shape
-    ints = dict(dtype=torch.int32, device=logits.device)
-    return [torch.empty((T, top_k), dtype=torch.float32, device=logits.device), torch.empty((T, top_k), **ints),
-            torch.empty((E + 1,), **ints), torch.empty((T * top_k,), **ints), torch.empty((T, top_k), **ints)]
-
-
-@torch.library.custom_op("gemlite::experts", mutates_args=())
-def experts_op(mode: int, x: Tensor, bias: Optional[Tensor], tensor_args: List[Tensor], meta_args: List[int], offsets: Tensor,
-               plan: List[Tensor]) -> Tensor:
-    return _launch(mode, x, bias, tensor_args, meta_args, offsets, ExpertPlan(*plan) if plan else None, -1)
-
-
-@experts_op.register_fake
-def _(mode, x, bias, tensor_args, meta_args, offsets, plan):
-    N, rows = tensor_args[0].shape[2], x.shape[0]
-    if mode != _ROWS:
-        T, k = plan[4].shape
-        rows = T if mode == _COMBINED else T * k
-    return torch.empty((rows, N // 2 if mode == _GATED else N), dtype=DTYPE_TO_TORCH[int(meta_args[6])], device=x.device)
+route_experts_op, experts_op = _make_custom_ops()
 
 
 def _dispatch(mode, x, bias, tensor_args, meta_args, offsets, plan, tile_config=-1):
-    if torch.compiler.is_compiling():
+    if experts_op is not None and torch.compiler.is_compiling():
         return experts_op(mode, x, bias, tensor_args, meta_args, offsets, [] if plan is None else list(plan))
     return _launch(mode, x, bias, tensor_args, meta_args, offsets, plan, tile_config)
 

@@ -93,3 +93,21 @@ def test_sizes_that_32_bits_cannot_hold(launches):
         t = [v.to("meta") for v in e.get_tensor_args()]
         gemlite_amd.experts_functional(meta, None, t, e.get_meta_args(), torch.empty(3, dtype=torch.int32, device="meta"))
     assert not launches
+
+
+def test_import_without_custom_ops():
+    """A torch without torch.library.custom_op, or a name that is taken, costs the compiled nodes and not the package."""
+    code = ("import torch; del torch.library.custom_op; import gemlite_amd; from gemlite_amd import experts; "
+            "assert experts.experts_op is None and experts.route_experts_op is None; print('imported')")
+    run = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "imported" in run.stdout, run.stderr
+
+
+def test_compiled_calls_without_custom_ops(launches, monkeypatch):
+    e = _raw_experts(torch.bfloat16)
+    monkeypatch.setattr(torch.compiler, "is_compiling", lambda: True)
+    monkeypatch.setattr(experts_module, "experts_op", None)
+    monkeypatch.setattr(experts_module, "route_experts_op", None)
+    monkeypatch.setattr(_ext, "route_experts", lambda *args: None)
+    assert gemlite_amd.route_experts(torch.zeros((4, 2)), 1).places.shape == (4, 1)
+    assert e(torch.zeros((4, 64), dtype=torch.bfloat16), torch.tensor([0, 2, 4], dtype=torch.int32)).shape == (4, 32) and len(launches) == 1
