@@ -463,11 +463,11 @@ def _make_custom_ops():
 
         @torch.library.custom_op("gemlite::experts", mutates_args=())
         def experts_op(mode: int, x: Tensor, bias: Optional[Tensor], tensor_args: List[Tensor], meta_args: List[int], offsets: Tensor,
-                       plan: List[Tensor]) -> Tensor:
-            return _launch(mode, x, bias, tensor_args, meta_args, offsets, ExpertPlan(*plan) if plan else None, -1)
+                       plan: List[Tensor], tile_config: int = -1) -> Tensor:
+            return _launch(mode, x, bias, tensor_args, meta_args, offsets, ExpertPlan(*plan) if plan else None, tile_config)
 
         @experts_op.register_fake
-        def _(mode, x, bias, tensor_args, meta_args, offsets, plan):
+        def _(mode, x, bias, tensor_args, meta_args, offsets, plan, tile_config=-1):
             N, rows = tensor_args[0].shape[2], x.shape[0]
             if mode != _ROWS:
                 T, k = plan[4].shape
@@ -486,7 +486,7 @@ route_experts_op, experts_op = _make_custom_ops()
 
 def _dispatch(mode, x, bias, tensor_args, meta_args, offsets, plan, tile_config=-1):
     if experts_op is not None and torch.compiler.is_compiling():
-        return experts_op(mode, x, bias, tensor_args, meta_args, offsets, [] if plan is None else list(plan))
+        return experts_op(mode, x, bias, tensor_args, meta_args, offsets, [] if plan is None else list(plan), tile_config)
     return _launch(mode, x, bias, tensor_args, meta_args, offsets, plan, tile_config)
 
 

@@ -111,3 +111,16 @@ def test_compiled_calls_without_custom_ops(launches, monkeypatch):
     monkeypatch.setattr(_ext, "route_experts", lambda *args: None)
     assert gemlite_amd.route_experts(torch.zeros((4, 2)), 1).places.shape == (4, 1)
     assert e(torch.zeros((4, 64), dtype=torch.bfloat16), torch.tensor([0, 2, 4], dtype=torch.int32)).shape == (4, 32) and len(launches) == 1
+
+
+def test_compiled_calls_hand_on_the_tile_configuration(launches, monkeypatch):
+    e = _raw_experts(torch.bfloat16)
+    x, off = torch.zeros((4, 64), dtype=torch.bfloat16), torch.tensor([0, 2, 4], dtype=torch.int32)
+    eager = gemlite_amd.experts_functional(x, None, e.get_tensor_args(), e.get_meta_args(), off, tile_config=2064)
+    monkeypatch.setattr(torch.compiler, "is_compiling", lambda: True)
+    compiled = gemlite_amd.experts_functional(x, None, e.get_tensor_args(), e.get_meta_args(), off, tile_config=2064)
+    assert compiled.shape == eager.shape and [args.tile_config for args, _ in launches] == [2064, 2064]
+    with pytest.raises(ValueError):
+        gemlite_amd.experts_functional(x, None, e.get_tensor_args(), e.get_meta_args(), off, tile_config=7)
+    e(x, off)
+    assert launches[-1][0].tile_config == -1
