@@ -124,3 +124,20 @@ def test_compiled_calls_hand_on_the_tile_configuration(launches, monkeypatch):
         gemlite_amd.experts_functional(x, None, e.get_tensor_args(), e.get_meta_args(), off, tile_config=7)
     e(x, off)
     assert launches[-1][0].tile_config == -1
+
+
+def test_compiled_routing_copies_nothing(monkeypatch):
+    """The op returns what the kernel writes, in five allocations of their own (outputs of an op must not share memory)."""
+    written = []
+
+    def record(logits, top_k, scoring, renormalize, scale, *outputs):
+        written.extend(outputs)
+        for t in outputs:
+            t.zero_()
+
+    monkeypatch.setattr(_ext, "_require_cuda", lambda *tensors: None)
+    monkeypatch.setattr(_ext, "route_experts", record)
+    plan = torch.ops.gemlite.route_experts(torch.zeros((5, 3)), 2, "softmax", True, 1.0)
+    assert [t.data_ptr() for t in plan] == [t.data_ptr() for t in written]
+    assert len({t.untyped_storage().data_ptr() for t in plan}) == 5
+    assert [tuple(t.shape) for t in plan] == [(5, 2), (5, 2), (4,), (10,), (5, 2)]
