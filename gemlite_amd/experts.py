@@ -47,10 +47,12 @@ class ExpertPlan(NamedTuple):
 # ---------------------------------------------------------------------------
 # routing
 # ---------------------------------------------------------------------------
-def _empty_plan(like, T, k, E):
-    """(ids, offsets, order, places), views of one allocation (the kernels address them element by element)."""
+def _empty_plan(like, T, k, E, apart=False):
+    """(ids, offsets, order, places): views of one allocation (the kernels address them element by element), or ``apart``."""
     _ext._route_need(T, E, k)  # (refuses sizes that no plan can have)
     n = T * k
+    if apart:
+        return tuple(like.new_empty(shape, dtype=torch.int32) for shape in ((T, k), (E + 1,), (n,), (T, k)))
     ints = like.new_empty(3 * n + E + 1, dtype=torch.int32)
     return (ints.as_strided((T, k), (k, 1), 0), ints.as_strided((E + 1,), (1,), 3 * n), ints.as_strided((n,), (1,), n),
             ints.as_strided((T, k), (k, 1), 2 * n))
@@ -68,7 +70,7 @@ def route_experts(logits: Tensor, top_k: int, scoring: str = "softmax", renormal
     return _route_experts(logits, top_k, scoring, renormalize, scale)
 
 
-def _route_experts(logits, top_k, scoring, renormalize, scale):
+def _route_experts(logits, top_k, scoring, renormalize, scale, apart=False):
     if logits.dim() != 2:
         raise ValueError(f"logits: expected [tokens, experts], got shape {tuple(logits.shape)}")
     if scoring not in SCORINGS:
@@ -80,7 +82,7 @@ def _route_experts(logits, top_k, scoring, renormalize, scale):
     if logits.stride(1) != 1 or (T > 1 and logits.stride(0) < E):
         logits = logits.contiguous()
     weights = logits.new_empty((T, top_k), dtype=torch.float32)
-    ids, offsets, order, places = _empty_plan(logits, T, top_k, E)
+    ids, offsets, order, places = _empty_plan(logits, T, top_k, E, apart)
     _ext.route_experts(logits, top_k, SCORINGS[scoring], renormalize, scale, weights, ids, offsets, order, places)
     return ExpertPlan(weights, ids, offsets, order, places)
 
@@ -451,8 +453,8 @@ def _make_custom_ops():
     try:
         @torch.library.custom_op("gemlite::route_experts", mutates_args=())
         def route_experts_op(logits: Tensor, top_k: int, scoring: str, renormalize: bool, scale: float) -> List[Tensor]:
-            # (a plan's integers are views of one allocation; the outputs of an op must not share memory)
-            return [t.clone() for t in _route_experts(logits, top_k, scoring, renormalize, scale)]
+            # (the outputs of an op must not share memory)
+            return list(_route_experts(logits, top_k, scoring, renormalize, scale, apart=True))
 
         @route_experts_op.register_fake
         def _(logits, top_k, scoring, renormalize, scale):
