@@ -424,20 +424,27 @@ class GemLiteMoE(torch.nn.Module):
     """Router, gated projection and combined projection of a mixture-of-experts block.
 
     ``gate_up``: experts with the gate columns followed by the up columns; ``down``: experts back to the model's width.
-    ``forward(x, logits)``: x [..., hidden], router logits [..., experts].
+    ``forward(x, logits)``: x [..., hidden], router logits [..., experts].  Two empty ``GemLiteExperts`` make a block that
+    ``load_state_dict`` fills.
     """
 
     def __init__(self, gate_up: GemLiteExperts, down: GemLiteExperts, top_k: int, scoring: str = "softmax", renormalize: bool = True,
                  scale: float = 1.0):
         super().__init__()
-        if gate_up.num_experts != down.num_experts or gate_up.out_features != 2 * down.in_features:
-            raise ValueError(f"gate_up ({gate_up.extra_repr()}) and down ({down.extra_repr()}) do not belong together")
         if scoring not in SCORINGS:
             raise ValueError(f"scoring: expected one of {sorted(SCORINGS)}, got {scoring!r}")
         self.gate_up, self.down = gate_up, down
         self.top_k, self.scoring, self.renormalize, self.scale = top_k, scoring, renormalize, scale
+        if gate_up.meta_args is not None or down.meta_args is not None:
+            self._check_pair()
+
+    def _check_pair(self):
+        up, down = self.gate_up, self.down
+        if up.meta_args is None or down.meta_args is None or up.num_experts != down.num_experts or up.out_features != 2 * down.in_features:
+            raise ValueError(f"gate_up ({up.extra_repr()}) and down ({down.extra_repr()}) do not belong together")
 
     def forward(self, x: Tensor, logits: Tensor) -> Tensor:
+        self._check_pair()
         x2d, logits2d = x.reshape(-1, x.shape[-1]), logits.reshape(-1, logits.shape[-1])
         if x2d.shape[0] != logits2d.shape[0] or logits2d.shape[1] != self.gate_up.num_experts:
             raise ValueError(f"x of shape {tuple(x.shape)} and logits of shape {tuple(logits.shape)} for {self.gate_up.num_experts} experts")

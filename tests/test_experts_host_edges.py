@@ -141,3 +141,19 @@ def test_compiled_routing_copies_nothing(monkeypatch):
     assert [t.data_ptr() for t in plan] == [t.data_ptr() for t in written]
     assert len({t.untyped_storage().data_ptr() for t in plan}) == 5
     assert [tuple(t.shape) for t in plan] == [(5, 2), (5, 2), (4,), (10,), (5, 2)]
+
+
+def test_a_block_is_loaded_from_a_checkpoint(launches, monkeypatch):
+    """A block of empty experts takes their shapes from the checkpoint, like the experts alone."""
+    monkeypatch.setattr(_ext, "route_experts", lambda *args: None)
+    block = GemLiteMoE(_raw_experts(torch.bfloat16, N=128), _raw_experts(torch.bfloat16), 2)
+    model, empty = torch.nn.Sequential(block), torch.nn.Sequential(GemLiteMoE(GemLiteExperts(), GemLiteExperts(), 2))
+    x, logits = torch.zeros((3, 64), dtype=torch.bfloat16), torch.zeros((3, 2))
+    with pytest.raises(ValueError, match="belong together"):
+        empty[0](x, logits)
+    empty.load_state_dict(model.state_dict())
+    assert empty[0].gate_up.num_experts == 2 and empty[0](x, logits).shape == (3, 32) and len(launches) == 2
+    other = torch.nn.Sequential(GemLiteMoE(GemLiteExperts(), GemLiteExperts(), 2))
+    other.load_state_dict(torch.nn.Sequential(torch.nn.ModuleDict({"gate_up": _raw_experts(torch.bfloat16), "down": _raw_experts(torch.bfloat16)})).state_dict())
+    with pytest.raises(ValueError, match="belong together"):
+        other[0](x, logits)
