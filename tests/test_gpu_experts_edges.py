@@ -6,9 +6,9 @@ import pytest
 import torch
 
 import gemlite_amd
-from gemlite_amd import DType, ExpertPlan, GemLiteExperts, GemLiteLinear, GemLiteMoE, _ext, experts as experts_module
+from gemlite_amd import ExpertPlan, GemLiteExperts, GemLiteLinear
 from gemlite_amd.helper import A16W4_HQQ_INT
-from test_gpu_experts import DT, FORMATS, _gen, check, make_ids, make_layers, make_x, ref_plan, ref_route, ref_rows, run_case, silu
+from test_gpu_experts import DT, FORMATS, _gen, check, make_layers, make_x, ref_rows, run_case, silu
 
 pytestmark = pytest.mark.gpu
 
@@ -188,6 +188,37 @@ def test_every_row_in_front_of_the_first_expert(fmt):
     off = torch.full((E + 1,), R, dtype=torch.int32, device="cuda")
     poison((R, N), (4, R, N))
     assert not e(make_x(R, K, "bf16").cuda(), off).any()
+
+
+# ---------------------------------------------------------------------------
+# tall tiles, filled
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("tile_config", [128, 256])
+def test_tiles_filled_to_the_last_row(fmt, dtype, tile_config):
+    """Experts of 256 rows and more, some of whose last tile ends one row past a shorter tile."""
+    E, K, N = 5, 320, 272
+    if fmt == "fp8":
+        K = 384
+    layers, W = make_layers(fmt, dtype, E, K, N, 64)
+    e = GemLiteExperts.from_layers(layers)
+    counts = [256, 0, 512 + 129, 256 + 65, 255]
+    offsets = torch.tensor([0] + counts).cumsum(0).to(torch.int32)
+    R = int(offsets[-1])
+    x = make_x(R, K, dtype)
+    u = torch.finfo(DT[dtype][0]).eps / 2
+    y, mag = ref_rows(fmt, x, W, offsets)
+    slack = K * 2.0 ** -24 * mag + (u * mag if fmt == "w4" else 0)
+    out = gemlite_amd.experts_functional(x.cuda(), None, e.get_tensor_args(), e.get_meta_args(), offsets.cuda(), tile_config=tile_config)
+    check(out, y, slack, u, u)
+
+
+@pytest.mark.parametrize("fmt,E,T,K,N", [("h16", 2, 2400, 64, 4096), ("fp8", 2, 700, 256, 272), ("fp8", 4, 9, 4096, 64), ("fp8", 4, 24, 4096, 64),
+                                          ("fp8", 4, 60, 4096, 64), ("fp8", 2, 400, 128, 256), ("w4", 2, 300, 256, 144)])
+def test_heights_the_library_chooses(fmt, E, T, K, N):
+    """256-row tiles of 16-bit and fp8 weights, streamed fp8 weights of long columns, 128-row tiles of 4-bit weights."""
+    run_case(fmt, "bf16", E, T, 1, K, N)
 
 
 def test_many_slots_for_a_token():
