@@ -171,6 +171,7 @@ SYMBOLS = {
         [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_void_p],
     ),
     "gla_route_workspace_bytes": (ctypes.c_int64, [ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    "gla_plan_workspace_bytes": (ctypes.c_int64, [ctypes.c_int, ctypes.c_int, ctypes.c_int]),
     "gla_route_experts": (
         ctypes.c_int,
         [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
@@ -571,7 +572,7 @@ def unpack_over_cols(packed: torch.Tensor, out: torch.Tensor, rows: int, pcols: 
 # ---------------------------------------------------------------------------
 # mixture of experts
 # ---------------------------------------------------------------------------
-_ROUTE_WORKSPACE = {}  # (T, E, k) -> bytes
+_ROUTE_WORKSPACE = {}  # (T, E, k) -> bytes to route, to sort given ids
 
 
 def _route_need(T, E, k):
@@ -580,9 +581,10 @@ def _route_need(T, E, k):
         # (the library takes 32-bit integers, and ctypes wraps what they cannot hold)
         if not (0 <= T * k < 2 ** 31 and 0 <= T < 2 ** 31 and 1 <= E <= 1024 and 1 <= k <= 64):
             raise ValueError(f"a plan of {T} tokens with {k} of {E} experts each: at most 2^31 - 1 pairs, 1024 experts and 64 per token")
-        need = load_library().gla_route_workspace_bytes(T, E, k)
-        if need < 0:
-            _check(int(need), "gla_route_workspace_bytes")
+        lib = load_library()
+        need = lib.gla_route_workspace_bytes(T, E, k), lib.gla_plan_workspace_bytes(T, E, k)
+        if min(need) < 0:
+            _check(int(min(need)), "gla_route_workspace_bytes")
         if len(_ROUTE_WORKSPACE) > 4096:
             _ROUTE_WORKSPACE.clear()
         _ROUTE_WORKSPACE[(T, E, k)] = need
@@ -602,7 +604,7 @@ def route_experts(logits, top_k, scoring, renormalize, scale, weights, ids, offs
     lib = load_library()
     T, E = logits.shape
     dtype = TORCH_TO_DTYPE.get(logits.dtype)
-    need = _route_need(T, E, top_k)
+    need = _route_need(T, E, top_k)[0]
     counts = logits.new_empty(need, dtype=torch.uint8) if need else None
     status = _on_current_device(lambda stream: lib.gla_route_experts(
         logits.data_ptr(), -1 if dtype is None else dtype.value, logits.stride(0), T, E, top_k, scoring, renormalize, scale,
@@ -615,7 +617,7 @@ def route_experts(logits, top_k, scoring, renormalize, scale, weights, ids, offs
 def plan_experts(ids, num_experts, offsets, order, places):
     lib = load_library()
     T, k = ids.shape
-    need = _route_need(T, int(num_experts), k)
+    need = _route_need(T, int(num_experts), k)[1]
     counts = ids.new_empty(need, dtype=torch.uint8) if need else None
     status = _on_current_device(lambda stream: lib.gla_plan_experts(
         ids.data_ptr(), T, int(num_experts), k, offsets.data_ptr(), order.data_ptr(), places.data_ptr(),

@@ -347,11 +347,16 @@ static int check_route(int64_t T, int E, int top_k, const void* ids, const void*
 
 int64_t gla_route_workspace_bytes(int T, int E, int top_k) {
     const int rc = check_route_sizes(T, E, top_k);
-    return rc != GLA_OK ? rc : route_counts(T, E, top_k) * 4;
+    return rc != GLA_OK ? rc : route_counts(T, E, top_k, true) * 4;
 }
 
-static int check_counts(int T, int E, int top_k, const void* workspace, int64_t bytes) {
-    const int64_t need = route_counts(T, E, top_k) * 4;
+int64_t gla_plan_workspace_bytes(int T, int E, int top_k) {
+    const int rc = check_route_sizes(T, E, top_k);
+    return rc != GLA_OK ? rc : route_counts(T, E, top_k, false) * 4;
+}
+
+static int check_counts(int T, int E, int top_k, bool select, const void* workspace, int64_t bytes) {
+    const int64_t need = route_counts(T, E, top_k, select) * 4;
     if (need > 0 && (workspace == nullptr || bytes < need || !aligned(workspace, 16))) {
         set_error("route: a 16-byte aligned workspace of %lld bytes required, %lld given", (long long)need, (long long)bytes);
         return GLA_ERR_WORKSPACE_TOO_SMALL;
@@ -376,7 +381,7 @@ int gla_route_experts(const void* logits, int dtype, int64_t stride, int T, int 
         set_error("route: NULL pointer, or rows %lld apart with %d logits", (long long)stride, E);
         return GLA_ERR_INVALID_ARGUMENT;
     }
-    if ((rc = check_counts(T, E, top_k, workspace, workspace_bytes)) != GLA_OK) return rc;
+    if ((rc = check_counts(T, E, top_k, true, workspace, workspace_bytes)) != GLA_OK) return rc;
     return launch_route(logits, T > 0 ? dtype : GLA_DT_FP32, stride, T, E, top_k, scoring == GLA_SCORING_SIGMOID, renormalize, scale, weights, ids,
                         offsets, order, places, (int32_t*)workspace, (hipStream_t)stream);
 }
@@ -385,7 +390,7 @@ int gla_plan_experts(const int32_t* ids, int T, int E, int top_k, int32_t* offse
                      int64_t workspace_bytes, void* stream) {
     int rc = check_route(T, E, top_k, ids, offsets, order, places);
     if (rc != GLA_OK) return rc;
-    if ((rc = check_counts(T, E, top_k, workspace, workspace_bytes)) != GLA_OK) return rc;
+    if ((rc = check_counts(T, E, top_k, false, workspace, workspace_bytes)) != GLA_OK) return rc;
     return launch_route(nullptr, 0, 0, T, E, top_k, 0, 0, 1.0f, nullptr, const_cast<int32_t*>(ids), offsets, order, places, (int32_t*)workspace,
                         (hipStream_t)stream);
 }

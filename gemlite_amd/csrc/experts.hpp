@@ -209,8 +209,8 @@ int launch_experts_quantise(const void* x, bool bf16, int64_t xsm, int rows, int
 int launch_experts_stream(const ExpertArgs& a, int format, bool bf16, int rows, hipStream_t stream);
 int launch_experts_gemm(const ExpertArgs& a, int format, bool bf16, int bm, hipStream_t stream);
 
-// logits NULL: the ids are given and only sorted.  counts: route_counts() integers of scratch.
-int64_t route_counts(int T, int E, int top_k);
+// logits NULL: the ids are given and only sorted.  counts: route_counts() integers of scratch (select: not for given ids).
+int64_t route_counts(int T, int E, int top_k, bool select);
 int launch_route(const void* logits, int dtype, int64_t stride, int T, int E, int top_k, int sigmoid, int renormalize, float scale,
                  float* weights, int32_t* ids, int32_t* offsets, int32_t* order, int32_t* places, int32_t* counts, hipStream_t stream);
 

@@ -7,8 +7,8 @@
 //              come last.  offsets[e] is where expert e's begin; places is the inverse of order
 //
 // A wave per token (32 tokens and 16 waves to a workgroup): lane l holds logits l, l + 64, ...; each of the k rounds is one
-// wave-wide maximum and, where several lanes have it, one minimum of their indices (DPP, no LDS).  Up to kSmallSlots
-// (token, slot) pairs one workgroup does everything in one launch.  Above, a first launch selects and counts each block's
+// wave-wide maximum and, where several lanes have it, one minimum of their indices (DPP, no LDS).  A small call
+// (small_call()) is done by one workgroup in one launch.  Otherwise a first launch selects and counts each block's
 // slots per expert, and a second one sorts: every block adds up the counts of the blocks in front of it for itself (they
 // are a few kilobytes in L2), so no third launch has to.  Counting by ballots and integer sums only: the result does not
 // depend on the order of execution.
@@ -22,7 +22,8 @@ namespace gla {
 
 namespace {
 
-constexpr int kSmallSlots = 1024;
+constexpr int kSmallSlots = 1024;  // (token, slot) pairs that one workgroup sorts, a thread each
+constexpr int kSmallTokens = 40;   // tokens that one workgroup selects for
 constexpr int kMaxBlocks = 256;
 constexpr int kMinTokens = 32;  // tokens per block, at least
 constexpr int kThreads = 1024;
@@ -188,7 +189,7 @@ __device__ __forceinline__ void scan_classes(int* totals, int classes) {
     }
 }
 
-// Everything in one workgroup: T k <= kSmallSlots.  DT < 0: the ids are given.
+// Everything in one workgroup (small_call()).  DT < 0: the ids are given.
 template <int DT, int V>
 __global__ __launch_bounds__(1024) void route_small_kernel(RouteArgs a, int bits) {
     extern __shared__ int lds[];
@@ -330,10 +331,16 @@ int bits_of(int classes) {
     return b;
 }
 
+// One workgroup in one launch, or two launches over many.  Sorting given ids is faster in one up to the last thread (us, one
+// launch / two: 1024 tokens top 1 of 64 3.5 / 7.0, 128 top 8 of 256 4.2 / 9.4).  Selecting is serial in the 16 waves: top 2 of 8 at
+// 32 / 64 / 512 tokens 4.9 / 6.2, 7.0 / 6.5, 36 / 7.9; top 6 of 64 at 40 / 48 7.5 / 7.8, 8.5 / 8.1; top 8 of 128 at 32 / 40 / 128 8.4 / 9.0,
+// 9.4 / 9.4, 22.9 / 12.6; top 8 of 256 at 40 / 48 10.9 / 11.8, 13.0 / 12.0; top 16 of 1024 at 24 / 40 23.6 / 29.3, 36.8 / 32.1.
+bool small_call(int64_t T, int top_k, bool select) { return T * top_k <= kSmallSlots && (!select || T <= kSmallTokens); }
+
 template <int DT, int V>
 int launch_dt(RouteArgs a, hipStream_t stream) {
     const int classes = a.E + 1, bits = bits_of(classes);
-    if ((int64_t)a.T * a.k <= kSmallSlots) {
+    if (small_call(a.T, a.k, DT >= 0)) {
         const int slots = a.T * a.k;
         int waves = slots > 64 ? (slots + 63) / 64 : 1;
         if (DT >= 0 && waves < a.T) waves = a.T < 16 ? a.T : 16;
@@ -374,7 +381,7 @@ static int route_blocks(int T) {
     return b < 4 ? 4 : (b + 3) / 4 * 4;
 }
 
-int64_t route_counts(int T, int E, int top_k) { return (int64_t)T * top_k <= kSmallSlots ? 0 : (int64_t)(E + 1) * route_blocks(T); }
+int64_t route_counts(int T, int E, int top_k, bool select) { return small_call(T, top_k, select) ? 0 : (int64_t)(E + 1) * route_blocks(T); }
 
 int launch_route(const void* logits, int dtype, int64_t stride, int T, int E, int top_k, int sigmoid, int renormalize, float scale,
                  float* weights, int32_t* ids, int32_t* offsets, int32_t* order, int32_t* places, int32_t* counts, hipStream_t stream) {

@@ -331,7 +331,8 @@ int64_t gla_route_workspace_bytes(int T, int E, int top_k);
 int gla_route_experts(const void* logits, int dtype, int64_t stride_t, int T, int E, int top_k, int scoring, int renormalize, float scale,
                       float* weights, int32_t* ids, int32_t* offsets, int32_t* order, int32_t* places, void* workspace,
                       int64_t workspace_bytes, void* stream);
-/* The plan alone, of ids [T, top_k] that another router chose. */
+/* The plan alone, of ids [T, top_k] that another router chose; its workspace is gla_plan_workspace_bytes() bytes. */
+int64_t gla_plan_workspace_bytes(int T, int E, int top_k);
 int gla_plan_experts(const int32_t* ids, int T, int E, int top_k, int32_t* offsets, int32_t* order, int32_t* places, void* workspace,
                      int64_t workspace_bytes, void* stream);
 

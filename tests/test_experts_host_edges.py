@@ -157,3 +157,16 @@ def test_a_block_is_loaded_from_a_checkpoint(launches, monkeypatch):
     other.load_state_dict(torch.nn.Sequential(torch.nn.ModuleDict({"gate_up": _raw_experts(torch.bfloat16), "down": _raw_experts(torch.bfloat16)})).state_dict())
     with pytest.raises(ValueError, match="belong together"):
         other[0](x, logits)
+
+
+def test_one_workgroup_routes_few_tokens():
+    """One workgroup's 16 waves take the tokens one after the other: above a few per wave the launch over many blocks, which
+    keeps counts, is the faster one at every number of experts."""
+    lib = _ext.load_library()
+    for E, k in ((8, 2), (64, 1), (128, 8), (1024, 16)):
+        assert lib.gla_route_workspace_bytes(40, E, k) == 0 and lib.gla_route_workspace_bytes(41, E, k) > 0
+        assert lib.gla_route_workspace_bytes(128, E, k) > 0
+    assert lib.gla_route_workspace_bytes(17, 1024, 64) > 0   # more (token, slot) pairs than threads
+    # given ids are sorted by a thread each
+    assert lib.gla_plan_workspace_bytes(128, 128, 8) == 0 and lib.gla_plan_workspace_bytes(129, 128, 8) > 0
+    assert lib.gla_plan_workspace_bytes(4, 0, 1) == -1

@@ -8,7 +8,7 @@ import torch
 import gemlite_amd
 from gemlite_amd import ExpertPlan, GemLiteExperts, GemLiteLinear
 from gemlite_amd.helper import A16W4_HQQ_INT
-from test_gpu_experts import DT, FORMATS, _gen, check, make_layers, make_x, ref_rows, run_case, silu
+from test_gpu_experts import DT, FORMATS, _gen, check, make_layers, make_x, ref_plan, ref_route, ref_rows, run_case, silu
 
 pytestmark = pytest.mark.gpu
 
@@ -68,6 +68,20 @@ def test_route_of_one_row_of_any_stride():
     want = gemlite_amd.route_experts(values[:16].view(1, 16), 4)
     for row in (values[:16].view(16, 1).t(), values.as_strided((1, 16), (0, 1)), values.as_strided((1, 16), (64, 1))):
         assert row.stride(0) != 16 and all(torch.equal(a, b) for a, b in zip(gemlite_amd.route_experts(row, 4), want))
+
+
+@pytest.mark.parametrize("T,E,k", [(39, 128, 8), (40, 8, 2), (41, 8, 2), (63, 60, 6), (40, 1024, 16), (41, 512, 8)])
+def test_routes_around_the_single_workgroup(T, E, k):
+    logits = torch.randn((T, E), generator=_gen(T)).half().float()   # ties
+    plan = gemlite_amd.route_experts(logits.cuda(), k)
+    w, ids = ref_route(logits, k, "softmax", True, 1.0)
+    offsets, order, places = ref_plan(ids, E)
+    for got, want in zip(plan[1:], (ids, offsets, order, places)):
+        assert torch.equal(got.cpu().long(), want)
+    # (as in test_gpu_experts: exp of a difference below 32, a sum of up to E of them, one division)
+    assert bool(((plan.weights.cpu().double() - w).abs() <= (2.0 ** -18 + E * 2.0 ** -24) * w).all())
+    again = gemlite_amd.plan_experts(plan.expert_ids, plan.weights, E)
+    assert all(torch.equal(a, b) for a, b in zip(plan, again))
 
 
 # ---------------------------------------------------------------------------
