@@ -179,21 +179,26 @@ struct ExpertPlanHost {
     int64_t partial_bytes, code_bytes, total_bytes;  // of the workspace: fp32 rows, codes, scales
 };
 
-// Rows per tile from the mean rows per expert with any (the distribution itself is on the device).  Times in us, both sides
-// of each threshold, at the sizes named (E experts, k of them per token):
-//  * 4-bit, 4096 -> 2 x 14336, E = 8, k = 2: 16-row streaming tiles against 64-row ones at 8 rows per expert 116 / 170, at 16
-//    168 / 164, at 24 240 / 164; 64 against 128 rows at 32 rows per expert 177 / 201, at 64 236 / 229, at 100 352 / 261.
+// Rows per tile from the mean rows per expert with any (the distribution itself is on the device; rows without an expert count
+// too, so a plan most of whose slots belong to other ranks gets taller tiles than its own rows need).  Times in us, both sides
+// of each threshold, at the sizes named (E experts, k of them per token); up to 24 rows per expert with copies of the weights
+// in turn, 700 MB together, so that each call finds its own in memory:
+//  * 4-bit, 4096 -> 2 x 14336, E = 8, k = 2: 16-row streaming tiles against 64-row ones at 8 rows per expert 112 / 174, at 16
+//    155 / 178, at 24 219 / 178; 64 against 128 rows at 32 rows per expert 177 / 201, at 64 236 / 229, at 100 352 / 261.
 //    256-row tiles leave one workgroup per CU, 128-row ones two: 1091 / 1014 at 512 rows per expert.
-//  * 16-bit, 4096^2, E = 16: 16 against 64 at 6 rows per expert 72 / 88, at 12 113 / 98; 64 against 128 at 28 112 / 116, at 57
-//    125 / 114.  Above, 128- and 256-row tiles cost 1.0 to 1.7 and run in rounds of one per CU: whichever needs less.
-//  * fp8: the streaming kernel quantises in every wave and needs long K ranges: 4096 -> 2 x 2048, E = 32, k = 4: 4 / 16 / 64 rows
-//    at 1 row per expert 57 / 66 / 73, at 4 109 / 93 / 119; 2048 -> 2 x 768, E = 128, k = 8 at 4 91 / 83 / 57; 768 -> 2048 at
-//    1 token 12.0 / 11.9 / 15.0, at 8 tokens 30 / 40 / 26.  64 against 128 at 62 rows per expert 119 / 121, at 125 168 / 147; 128
-//    against 256 at 250 151 / 174 and 232 / 222, at 512 449 / 404.
+//  * 16-bit, 4096^2, E = 16: 4 against 16 at 2 rows per expert 53 / 58, at 3 76 / 58; 16 against 64 at 6 65 / 85, at 12 105 / 93; 64
+//    against 128 at 28 112 / 116, at 57 125 / 114.  Above, 128- and 256-row tiles cost 1.0 to 1.7 and run in rounds of one per
+//    CU: whichever needs less.
+//  * fp8: the streaming kernel quantises in every wave and needs long K ranges.  4 / 16 / 64 rows: K = 4096 (-> 2 x 2048, E = 32,
+//    k = 4) at 1 row per expert 54 / 61 / 83, at 4 94 / 84 / 114, at 8 154 / 110 / 122; 7168 there at 4 161 / 131 / 149, at 8 261 / 173 / 168;
+//    3584 at 2 56 / 65 / 64, at 4 82 / 77 / 80; 2560 at 2 45 / 53 / 50, at 4 65 / 63 / 60, and 2560 -> 2 x 768, E = 128, k = 8 at 2 62 / 68 / 61;
+//    2048 -> 2 x 768, E = 128, k = 8 at 1 41 / 53 / 43, at 2 53 / 61 / 51, at 4 84 / 78 / 64; 768 -> 2048 at 1 token 11.2 / 11.3 / 15.1, at 8 tokens
+//    28 / 39 / 28.  64 against 128 at 62 rows per expert 119 / 121, at 125 168 / 147; 128 against 256 at 250 151 / 174 and 232 / 222,
+//    at 512 449 / 404.
 int choose_rows(int format, int K, int64_t R, int64_t active, int64_t width_of_128) {
     const int64_t per = active > 0 ? R / active : 0;
     if (format == kEF8) {
-        if (K >= 4096 ? per <= 8 : per <= 1 && active * width_of_128 <= 256) return per > 2 ? 16 : 4;
+        if (K >= 4096 ? per <= 8 : K > 2048 ? per <= 2 : per <= 1 && active * width_of_128 <= 256) return per > 2 ? 16 : 4;
         return per <= 64 ? 64 : per <= 300 ? 128 : 256;
     }
     if (format == kE16) {
@@ -230,7 +235,8 @@ ExpertPlanHost plan_of(const gla_experts_args& p) {
     if (p.mode != GLA_EXPERTS_COMBINED && (s < 4 || tiles > 96)) s = 1;
     h.S = want_s > 0 ? want_s : s;
     // 4-bit weights, many workgroups: two waves of twice the K range each, which start half as often (one token, 4096 -> 2 x
-    // 14336, 896 workgroups: 31.8 -> 29.1 us; 16 tokens top 2 of 8: 107 -> 103; 14336 -> 4096, 512 workgroups: 48 -> 64)
+    // 14336, 896 workgroups, weights in memory: 32.2 -> 29.9 us; 16 tokens top 2 of 8: 109 -> 106; 61 tokens top 6 of 64, 2048 ->
+    // 2 x 1408: 49 -> 46; 14336 -> 4096, 512 workgroups: 48 -> 64)
     h.waves = h.format == kEW4 && tiles * h.S >= 768 && steps >= 16 * h.S ? 2 : 4;
     const int unit = stream || h.format == kEF8 ? 128 : 64, parts = stream ? h.waves * h.S : h.S;
     const int n_units = (p.K + unit - 1) / unit;

@@ -170,3 +170,21 @@ def test_one_workgroup_routes_few_tokens():
     # given ids are sorted by a thread each
     assert lib.gla_plan_workspace_bytes(128, 128, 8) == 0 and lib.gla_plan_workspace_bytes(129, 128, 8) > 0
     assert lib.gla_plan_workspace_bytes(4, 0, 1) == -1
+
+
+def _fp8_args(K, R, N=4096, E=4):
+    return _args(mode=0, R=R, T=0, top_k=0, E=E, N=N, K=K, W_nbits=8, group_size=K, elements_per_sample=1, input_dtype=DType.FP8.value, zeros=None,
+                 meta_dtype=DType.FP32.value, channel_scale_mode=5, W_group_mode=0, w_stride_e=K * N, meta_stride_e=K // 128 * N // 128 * 4,
+                 x_stride_m=K, out_stride_m=N)
+
+
+def test_few_rows_of_fp8_experts_are_streamed():
+    """The streaming kernel quantises in registers, the tiled one in a launch that writes to the workspace."""
+    lib = _ext.load_library()
+
+    def streamed(K, R):
+        return lib.gla_experts_workspace_bytes(ctypes.byref(_fp8_args(K, R))) == 0
+
+    assert [streamed(K, 8) for K in (2048, 2176, 2560, 3584, 4096)] == [False, True, True, True, True]
+    assert [streamed(K, 12) for K in (2048, 2560, 3584, 4096)] == [False, False, False, True]
+    assert streamed(4096, 32) and not streamed(4096, 36)

@@ -228,10 +228,10 @@ def test_tiles_filled_to_the_last_row(fmt, dtype, tile_config):
     check(out, y, slack, u, u)
 
 
-@pytest.mark.parametrize("fmt,E,T,K,N", [("h16", 2, 2400, 64, 4096), ("fp8", 2, 700, 256, 272), ("fp8", 4, 9, 4096, 64), ("fp8", 4, 24, 4096, 64),
+@pytest.mark.parametrize("fmt,E,T,K,N", [("h16", 2, 2400, 64, 4096), ("fp8", 2, 700, 256, 272), ("fp8", 4, 9, 4096, 64), ("fp8", 4, 8, 2560, 64), ("fp8", 4, 24, 4096, 64),
                                           ("fp8", 4, 60, 4096, 64), ("fp8", 2, 400, 128, 256), ("w4", 2, 300, 256, 144)])
 def test_heights_the_library_chooses(fmt, E, T, K, N):
-    """256-row tiles of 16-bit and fp8 weights, streamed fp8 weights of long columns, 128-row tiles of 4-bit weights."""
+    """256-row tiles of 16-bit and fp8 weights, streamed fp8 weights, 128-row tiles of 4-bit weights."""
     run_case(fmt, "bf16", E, T, 1, K, N)
 
 
