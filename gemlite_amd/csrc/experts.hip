@@ -176,6 +176,7 @@ struct ExpertPlanHost {
     int S, chunk, waves;
     bool to_partials;
     bool quantise;                       // F8: a launch in front writes codes and scales to the workspace
+    bool sums;                           // W4: a launch in front writes the sums of the groups there
     int64_t partial_bytes, code_bytes, total_bytes;  // of the workspace: fp32 rows, codes, scales
 };
 
@@ -183,9 +184,10 @@ struct ExpertPlanHost {
 // too, so a plan most of whose slots belong to other ranks gets taller tiles than its own rows need).  Times in us, both sides
 // of each threshold, at the sizes named (E experts, k of them per token); up to 24 rows per expert with copies of the weights
 // in turn, 700 MB together, so that each call finds its own in memory:
-//  * 4-bit, 4096 -> 2 x 14336, E = 8, k = 2: 16-row streaming tiles against 64-row ones at 8 rows per expert 112 / 174, at 16
-//    155 / 178, at 24 219 / 178; 64 against 128 rows at 32 rows per expert 177 / 201, at 64 236 / 229, at 100 352 / 261.
-//    256-row tiles leave one workgroup per CU, 128-row ones two: 1091 / 1014 at 512 rows per expert.
+//  * 4-bit, 4096 -> 2 x 14336, E = 8, k = 2, groups of 128 (of 64 and 32 the same sides): 16-row streaming tiles against 64-row
+//    ones at 8 rows per expert 112 / 171, at 16 154 / 175, at 20 192 / 177; 64 against 128 rows at 32 rows per expert 186 / 201, at
+//    48 191 / 208, at 64 231 / 238, at 100 347 / 280; 14336 -> 4096 combined at 64 134 / 128.  (256-row tiles would leave one workgroup per CU,
+//    128-row ones two.)
 //  * 16-bit, 4096^2, E = 16: 4 against 16 at 2 rows per expert 53 / 58, at 3 76 / 58; 16 against 64 at 6 65 / 85, at 12 105 / 93; 64
 //    against 128 at 28 112 / 116, at 57 125 / 114.  Above, 128- and 256-row tiles cost 1.0 to 1.7 and run in rounds of one per
 //    CU: whichever needs less.
@@ -247,7 +249,8 @@ ExpertPlanHost plan_of(const gla_experts_args& p) {
     const int64_t rows = p.mode == GLA_EXPERTS_GATED ? p.T : p.R;
     h.quantise = h.format == kEF8 && h.bm > 16;
     h.code_bytes = h.quantise ? rows * p.K : 0;
-    h.total_bytes = h.partial_bytes + h.code_bytes + (h.quantise ? rows * (p.K / 128) * 4 : 0);
+    h.sums = h.format == kEW4 && h.bm > 16;
+    h.total_bytes = h.partial_bytes + h.code_bytes + (h.quantise ? rows * (p.K / 128) * 4 : 0) + (h.sums ? rows * (p.K / p.group_size) * 16 : 0);
     return h;
 }
 
@@ -316,6 +319,12 @@ int gla_experts_matmul(const gla_experts_args* p, void* stream) {
         a.x = codes;
         a.xsm = p->K;
         a.scales_x = scales_x;
+    }
+    if (h.sums) {
+        unsigned char* sums = (unsigned char*)p->workspace + h.partial_bytes;
+        const int rcs = launch_experts_sums(p->x, bf16, a.xsm, p->mode == GLA_EXPERTS_GATED ? p->T : p->R, p->K, p->group_size, sums, s);
+        if (rcs != GLA_OK) return rcs;
+        a.sums = sums;
     }
     const int rc2 = h.bm > 16 ? launch_experts_gemm(a, h.format, bf16, h.bm, s) : launch_experts_stream(a, h.format, bf16, h.bm, s);
     if (rc2 != GLA_OK || !h.to_partials) return rc2;

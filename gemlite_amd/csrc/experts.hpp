@@ -18,6 +18,7 @@ struct ExpertArgs {
     const unsigned char* w;         // expert 0's weights
     const unsigned char* scales;    // W4: [E][G][N] 16-bit; F8: [E][K/128][ceil(N/128)] fp32
     const unsigned char* zeros;     // W4: as scales, or NULL
+    const unsigned char* sums;      // W4, tiled GEMM: [rows of x][groups] sums of a group's activations, as 16-byte operand pieces
     const float* scales_x;          // F8, tiled GEMM: [rows of x][K/128] (the streaming kernel quantises 16-bit rows itself)
     const float* bias;              // [E][N] fp32 or NULL
     void* out;                      // 16-bit rows (rows / gated)
@@ -202,6 +203,21 @@ __device__ __forceinline__ float high16(uint32_t v) {
     if constexpr (BF16) return __builtin_bit_cast(float, v & 0xffff0000u);
     else return half_bits_to_float((uint16_t)(v >> 16));
 }
+
+// A float as three bf16 values in the high halves of t: 8 bits of its significand each, so that their sum is exact (but for
+// underflow).
+__device__ __forceinline__ void bf16_terms(float v, uint32_t (&t)[3]) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        t[i] = __builtin_bit_cast(uint32_t, v) & 0xffff0000u;
+        v -= __builtin_bit_cast(float, t[i]);
+    }
+}
+__device__ __forceinline__ uint32_t high_halves(uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
+
+// 16-bit rows -> sums of every group of `group` values, in fp32, as the activations' side of eight products of bf16 terms
+// [rows][K / group][8] (experts_quant.hip)
+int launch_experts_sums(const void* x, bool bf16, int64_t xsm, int rows, int K, int group, unsigned char* sums, hipStream_t stream);
 
 // 16-bit rows -> e4m3 codes [rows][K] and scales [rows][K/128] (experts_quant.hip)
 int launch_experts_quantise(const void* x, bool bf16, int64_t xsm, int rows, int K, unsigned char* codes, float* scales, hipStream_t stream);

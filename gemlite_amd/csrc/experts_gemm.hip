@@ -10,13 +10,15 @@
 //    front of it.  The barrier of a stage stands before its last K-step, whose fragments are in registers by then: the
 //    matrix pipe has work while the waves meet and the first fragments of the next stage arrive.
 //  * W4: the packed words lie in LDS as they are in memory (a word = 8 K-values of a column = a lane's share of a
-//    K-step's operand) and are dequantised into the operand registers between the MFMAs, w = s q + z, rounded once to the
-//    activation type, as the dense layers' tiled GEMM does: 2^-8 (bf16) or 2^-11 (fp16) of each weight at most, which makes
-//    the error of a sum 1.4 times that of rounding the result alone.  (Codes with the constants applied to the sums, as in
-//    the streaming kernel, would need a second set of accumulators: 128 rows would no longer fit two workgroups on a CU, and
-//    with one the call below takes 1190 us.)  bf16: in fp32, then converted.  fp16: one packed fma where z is an fp16 value
-//    as it stands; where it is a product zero * s (Z32) in fp32 as for bf16, since that product rounded to fp16 first would be
-//    an error that all codes of a group share and that grows with the sum of the activations.
+//    K-step's operand).  The codes go into the MFMA as they are (bf16 16 + q, fp16 64 + q: a byte select and a masked OR per
+//    pair), so that no weight is rounded.  With w = s q + z on a group,
+//        sum(x w) = s sum(x (off + q)) + (z - off s) sum(x).
+//    First terms: the sums are kept divided by their column's current scale; where a group begins they are multiplied by the
+//    old scale over the new one, which needs no second set of accumulators (128 rows: two workgroups on a CU).  Second
+//    terms: a launch in front (experts_quant.hip) takes every group's sum of x; sum and constant are three bf16 terms
+//    each (24 bits), and eight of the products of two groups fill one MFMA behind the K loop.  Sums that are not finite are
+//    taken again from dequantised weights.  (Weights dequantised and rounded in front of the MFMA: the error of a result 1.7
+//    times that of its own rounding; groups of 128 / 64 / 32 below 1040 / 1040 / 1040 us for 1070 / 1230 / 1530.)
 //  * F8: v_mfma_f32_16x16x128 starts from zero on every 128-block and its result joins the fp32 sum times the block's two
 //    scales.
 //  * gridDim.y splits K where the tiles do not fill the chip (fp32 sums to the workspace, added in order by the
@@ -37,11 +39,13 @@
 
 #include "common.hpp"
 #include "experts.hpp"
-#include "wn_dequant.hpp"
 
 namespace gla {
 
 namespace {
+
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 
 __device__ __align__(16) unsigned char g_zero_chunk[16];  // what activations past the end of K are read from
 
@@ -64,25 +68,25 @@ struct GemmShape {
     static constexpr int WN = BN / WC, WM = BM / (WAVES / WN);     // waves side by side, rows of a wave
     static constexpr int A_BYTES = BM * 128;
     static constexpr int B_BYTES = FMT == kEW4 ? 8 * BN * 4 : BN * 128;
-    // W4: [32-half][scale, zero][column]; F8: rows, columns
-    static constexpr int M_BYTES = FMT == kEW4 ? 8 * BN : (FMT == kEF8 ? (BM + BN) * 4 : 0);
+    // W4: [32-half][column]; F8: rows, columns
+    static constexpr int M_BYTES = FMT == kEW4 ? 4 * BN : (FMT == kEF8 ? (BM + BN) * 4 : 0);
     static constexpr int STAGE = A_BYTES + B_BYTES + M_BYTES;
     static constexpr int RING = FMT == kEW4 ? (BM == 128 ? 3 : 4) : (BM == 256 ? 2 : 3);  // (W4: two workgroups per CU)
     static constexpr int A_JOBS = BM / 8 / WAVES;                  // copies per wave and stage
     static constexpr int B_JOBS = B_BYTES / 1024 / WAVES;
     static constexpr int M_JOBS = FMT == kE16 ? 0 : 1;
     static constexpr int LPS = A_JOBS + B_JOBS + M_JOBS;
-    static constexpr int LDS = RING * STAGE;
+    static constexpr int X_OFF = RING * STAGE;                     // W4: 32 floats per wave, see `spread`
+    static constexpr int LDS = X_OFF + (FMT == kEW4 ? WAVES * 128 : 0);
 };
 
 // One tile of up to BM rows x BN columns.
-template <int FMT, bool BF16, bool Z32, int BM, int BN>
+template <int FMT, bool BF16, int BM, int BN>
 __device__ __forceinline__ void gemm_tile(const ExpertArgs& a, const ExpertTile& tile, int ct, unsigned char* smem) {
     using SH = GemmShape<FMT, BM, BN>;
     constexpr int WAVES = SH::WAVES;
     constexpr int RING = SH::RING, LPS = SH::LPS, WC = SH::WC, WM = SH::WM;
     constexpr bool F8 = FMT == kEF8, W4 = FMT == kEW4;
-    constexpr bool W32 = BF16 || Z32;                  // W4: weights computed in fp32
     constexpr int MT = F8 ? 16 : 32;                   // MFMA tile edge
     constexpr int TI = WM / MT, TJ = WC / MT;
     constexpr int KS = F8 ? 128 : 64;                  // K-values per stage
@@ -127,19 +131,20 @@ __device__ __forceinline__ void gemm_tile(const ExpertArgs& a, const ExpertTile&
             b_off[i] = (uint32_t)unit_column_inside<WC>(a.half, a.N, ct * SH::WN + c / WC, c % WC) * (uint32_t)(a.K * ES);
         }
     }
-    // one 4-byte copy per wave and stage: W4: scales (even waves) / zeros (odd) of 128 columns and one 32-half of the
-    // stage; F8: the activation scales of 64 rows, or the block scale of each of 64 columns
+    // one 4-byte copy per wave and stage: W4: scales of 128 columns for one 32-half of the stage (four jobs, done twice: all
+    // waves have the same number of copies in flight); F8: the activation scales of 64 rows, or the block scale of each of
+    // 64 columns
     uint32_t m_off = 0;
     int64_t m_row = 0;
     int m_dst = 0, m_half = 0, m_step = (a.N + 127) / 128 * 4;
     const unsigned char* m_src = se;
     if constexpr (W4) {
-        const int part = BN == 256 ? (wave >> 1) & 1 : 0, c = part * 128 + 2 * lane;
-        m_half = BN == 256 ? wave >> 2 : wave >> 1;
+        static_assert(BN == 256, "four copies of scales");
+        const int part = wave & 1, c = part * 128 + 2 * lane;
+        m_half = (wave >> 1) & 1;
         // (a pair lies inside the run of 4 it belongs to)
         m_off = (uint32_t)(unit_column_inside<WC>(a.half, a.N, ct * SH::WN + (c & ~3) / WC, (c & ~3) % WC) + (c & 3)) * 2u;
-        m_src = wave & 1 ? ze : se;
-        m_dst = M_OFF + m_half * (BN * 4) + (wave & 1) * (BN * 2) + part * 256;
+        m_dst = M_OFF + m_half * (BN * 2) + part * 256;
     } else if constexpr (F8) {
         constexpr int JOBS = BM / 64 + BN / 64;
         static_assert(JOBS <= WAVES, "one scale copy per wave");
@@ -205,7 +210,7 @@ __device__ __forceinline__ void gemm_tile(const ExpertArgs& a, const ExpertTile&
         for (int j = 0; j < TJ; ++j)
 #pragma unroll
             for (int e = 0; e < AE; ++e) acc[i][j][e] = 0.0f;
-    const int fr = lane & (MT - 1), fk = lane / MT;  // row of a fragment, K part
+    int fr = lane & (MT - 1), fk = lane / MT;        // row of a fragment, K part
     const int swz = (fr >> 1) & 7;                   // (tile offsets are multiples of 16 rows)
     const int a_row = (wm * WM + fr) * 128, b_row = B_OFF + (wn * WC + fr) * 128;
 
@@ -294,6 +299,234 @@ __device__ __forceinline__ void gemm_tile(const ExpertArgs& a, const ExpertTile&
         for (; k + RING < stages; ++k) stage(k, std::true_type{});
 #pragma unroll 1
         for (; k < stages; ++k) stage(k, std::false_type{});
+    } else if constexpr (W4) {
+        static_assert(TJ == 1 && WM == BM, "a wave has 32 columns and every row");
+        constexpr float OFF = BF16 ? 16.0f : 64.0f;                                     // of a code in the MFMA
+        constexpr uint32_t CODE = BF16 ? 0x00780078u : 0x00f000f0u, BASE = BF16 ? 0x41804180u : 0x54005400u;
+        float* const mine = (float*)(smem + SH::X_OFF) + wave * 32;
+        u32x4 fa[TI], fb[2];         // (an activation fragment is read anew behind its one MFMA of a K-step)
+        uint32_t word, scale;        // codes of the next K-step, the lane's column's scale of the 32-half it belongs to
+        uint32_t mask = CODE, offset = BASE;  // 0 where that scale is 0: codes of such a group enter as zeros
+        static_assert(SH::STAGE % 128 == 0, "rows of 128 bytes");
+        uint32_t a_off = (uint32_t)(fr * 128 + (fk ^ swz) * 16);
+        auto read_a = [&](const unsigned char* base, int s, int i) __attribute__((always_inline)) {
+            fa[i] = *(const u32x4*)(base + (a_off ^ (32 * s)) + i * 32 * 128);  // chunk (2 s + fk) ^ swz of the row
+        };
+        auto read_word = [&](const unsigned char* base, int s) __attribute__((always_inline)) {
+            word = *(const uint32_t*)(base + B_OFF + (2 * s + fk) * (BN * 4) + (wn * WC + fr) * 4);
+        };
+        auto read_scale = [&](const unsigned char* base, int h) __attribute__((always_inline)) {
+            scale = *(const uint16_t*)(base + M_OFF + h * (BN * 2) + (wn * WC + fr) * 2);
+        };
+        // register q of the operand: OFF + codes 2q, 2q + 1, a shift each for the word and a byte select and a masked OR here
+        auto convert = [&](int q) __attribute__((always_inline)) -> uint32_t {
+            const uint32_t lo = BF16 ? word << 3 : word << 4, hi = BF16 ? word >> 1 : word;
+            return (__builtin_amdgcn_perm(hi, lo, 0x0c000c00u | ((4 + q) << 16) | q) & mask) | offset;
+        };
+        auto choose = [&]() __attribute__((always_inline)) {
+            const bool none = (scale & 0x7fffu) == 0;
+            mask = none ? 0u : CODE;
+            offset = none ? 0u : BASE;
+        };
+        auto mfma = [&](const u32x4& b, const u32x4& x, float16_t c) __attribute__((always_inline)) {
+            if constexpr (BF16)
+                return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, b), __builtin_bit_cast(bf16x8_t, x), c, 0, 0, 0);
+            else
+                return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, b), __builtin_bit_cast(half8_t, x), c, 0, 0, 0);
+        };
+        // a factor of the lane's column, to the lanes that hold the column's sums: through LDS (one wave: in order)
+        auto put = [&](float v) __attribute__((always_inline)) {
+            mine[fr] = v;
+            __builtin_amdgcn_wave_barrier();
+        };
+        auto times = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float4_t f = *(const float4_t*)(mine + 8 * g + 4 * fk);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][0][4 * g + e] *= f[e];
+            }
+        };
+        const int halves = a.group / 32;
+        int left = halves - (2 * k_first) % halves;  // 32-halves to the next group
+        bool enters = false;
+        float unit = 1.0f;                           // the scale the column's sums are divided by
+        auto enter_group = [&]() __attribute__((always_inline)) {
+            const float s = low16<BF16>(scale);
+            float r = 1.0f;
+            if (s != 0.0f) {
+                r = unit / s;
+                const float m = __builtin_fabsf(r);
+                if (!(m < 0x1p64f && m > 0x1p-64f)) r = __builtin_nanf("");  // (taken again below)
+                unit = s;
+            }
+            put(r);
+        };
+
+        const unsigned char* base = smem;
+#pragma unroll
+        for (int i = 0; i < TI; ++i) read_a(base, 0, i);
+        read_scale(base, 0);
+        read_word(base, 0);
+        choose();
+        if (low16<BF16>(scale) != 0.0f) unit = low16<BF16>(scale);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) fb[0][q] = convert(q);
+        int slot = 0;
+        auto stage = [&](int k, auto refill_tag) __attribute__((always_inline)) {
+            constexpr bool REFILL = decltype(refill_tag)::value;
+            const int next_slot = slot == RING - 1 ? 0 : slot + 1;
+            const unsigned char* next = smem + next_slot * SH::STAGE;
+            asm volatile("" : "+v"(a_off));  // or one address per K-step stays in registers, which the sums need
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const int cur = s & 1, nxt = cur ^ 1;
+                if (s == 3) {  // as for 16-bit weights
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    wait_vmcnt_e<REFILL ? (RING - 2) * LPS : 0>();
+                    bare_barrier();
+                }
+                const unsigned char* from = s == 3 ? next : base;
+                const int s1 = (s + 1) & 3;
+                if (s % 2 == 0 && enters) {
+#pragma unroll
+                    for (int i = 0; i < TI; ++i) times(i);
+                }
+                read_word(from, s1);
+                if (s == 1) read_scale(base, 1);
+                if (s == 3) read_scale(next, 0);
+                // slices of one MFMA each, with the scheduler fenced between them
+#pragma unroll
+                for (int i = 0; i < TI; ++i) {
+                    acc[i][0] = mfma(fb[cur], fa[i], acc[i][0]);
+                    read_a(from, s1, i);
+                    if (s % 2 == 1 && i == 0) choose();
+#pragma unroll
+                    for (int q = i * 4 / TI; q < (i + 1) * 4 / TI; ++q) fb[nxt][q] = convert(q);
+                    if (s % 2 == 1 && i == TI - 1) {  // does the next 32-half begin a group?
+                        enters = --left == 0 && (s == 1 || k + 1 < stages);
+                        if (enters) {
+                            enter_group();
+                            left = halves;
+                        }
+                    }
+                    if constexpr (REFILL) {
+                        if (s == 3) {
+#pragma unroll
+                            for (int c = i * LPS / TI; c < (i + 1) * LPS / TI; ++c) issue_one(k + RING, slot, c);
+                        }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            slot = next_slot;
+            base = next;
+        };
+        int k = 0;
+#pragma unroll 1
+        for (; k + RING < stages; ++k) stage(k, std::true_type{});
+#pragma unroll 1
+        for (; k < stages; ++k) stage(k, std::false_type{});
+        // (the lane's number anew: nothing but the sums, the unit and wave-uniform values stays in registers behind the loop)
+        int fresh = 0;
+        asm volatile("" : "+s"(fresh));
+        fresh = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, (uint32_t)fresh));
+        put(unit);
+        fr = fresh & 31;
+        fk = fresh >> 5;
+#pragma unroll
+        for (int i = 0; i < TI; ++i) times(i);
+
+        // ---- the groups' constants times their sums of activations, two groups to an MFMA: the groups that begin in this split
+        const int k0 = k_first * 64, k1 = k0 + stages * 64 < a.K ? k0 + stages * 64 : a.K;
+        const int g0 = (k0 + a.group - 1) / a.group, g1 = (k1 + a.group - 1) / a.group;
+        const int col = unit_column_inside<WC>(a.half, a.N, ct * SH::WN + wn, fr & ~3) + (fr & 3);
+        constexpr int AT_ONCE = 16, PIECES = BM * AT_ONCE / SH::THREADS, STEPS = AT_ONCE / 2;  // groups, pieces per thread, MFMAs
+        static_assert(BM * AT_ONCE * 16 <= SH::X_OFF, "sums of a chunk of groups fit the ring");
+        const int piece = wave * 64 + (fk * 32 + fr);
+        uint32_t x_off = (uint32_t)(fr * (AT_ONCE * 16) + (fk ^ (fr & (AT_ONCE - 1))) * 16);  // piece 2 j + fk of a row: ^ 32 j
+        const unsigned char* from[PIECES];
+        u32x4 held[PIECES];
+#pragma unroll
+        for (int q = 0; q < PIECES; ++q) {
+            int r = tile.row0 + (piece + q * SH::THREADS) / AT_ONCE;
+            if (r > tile.row_end - 1) r = tile.row_end - 1;
+            from[q] = a.sums + (source_row(a, r) * groups + piece % AT_ONCE) * 16;
+        }
+        auto hold = [&](int gc) __attribute__((always_inline)) {
+#pragma unroll
+            for (int q = 0; q < PIECES; ++q) {
+                held[q] = u32x4{0, 0, 0, 0};
+                if (gc + piece % AT_ONCE < g1) held[q] = *(const u32x4*)(from[q] + (int64_t)gc * 16);
+            }
+        };
+#pragma unroll 1
+        for (int gc = g0; gc < g1; gc += AT_ONCE) {
+            hold(gc);
+            uint32_t sb[STEPS], zb[STEPS];  // (all in flight together)
+#pragma unroll
+            for (int j = 0; j < STEPS; ++j) {
+                const int g = gc + 2 * j + fk;
+                const int64_t at = ((int64_t)(g < g1 ? g : g1 - 1) * a.N + col) * 2;
+                sb[j] = *(const uint16_t*)(se + at);
+                zb[j] = *(const uint16_t*)(ze + at);
+            }
+            __syncthreads();  // the ring (the chunk in front) has been read
+#pragma unroll
+            for (int q = 0; q < PIECES; ++q) {
+                const int row = (piece + q * SH::THREADS) / AT_ONCE;
+                *(u32x4*)(smem + row * (AT_ONCE * 16) + (((piece % AT_ONCE) ^ (row & (AT_ONCE - 1))) * 16)) = held[q];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < STEPS; ++j) {
+                if (gc + 2 * j >= g1) break;
+                asm volatile("" : "+v"(x_off));  // (no address per step in registers)
+                const float sc = low16<BF16>(sb[j]);
+                float z = a.zeros == nullptr ? 0.0f : low16<BF16>(zb[j]) * __builtin_fmaf(a.c2, sc, a.c1);
+                z = gc + 2 * j + fk < g1 ? __builtin_fmaf(-OFF, sc, z) : 0.0f;
+                uint32_t t[3];
+                bf16_terms(z, t);
+                const u32x4 b = u32x4{high_halves(t[0], t[0]), high_halves(t[0], t[1]), high_halves(t[1], t[1]), high_halves(t[2], t[2])};
+#pragma unroll
+                for (int i = 0; i < TI; ++i) {
+                    const u32x4 x = *(const u32x4*)(smem + (x_off ^ (32 * j)) + i * 32 * (AT_ONCE * 16));
+                    acc[i][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, b), __builtin_bit_cast(bf16x8_t, x), acc[i][0], 0, 0, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);  // (or the fragments of all steps are read first, which takes the sums' registers)
+            }
+        }
+
+        // ---- sums that are not finite, perhaps only because of the codes' offset (inf - inf, or an overflow of OFF x) or of scales
+        // that are 2^64 apart: again from dequantised weights, rounded to 16 bits
+#pragma unroll
+        for (int i = 0; i < TI; ++i) {
+            bool odd = false;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) odd = odd || !(__builtin_fabsf(acc[i][0][e]) < __builtin_inff());
+            if (!__any(odd)) continue;
+            int r = tile.row0 + i * 32 + fr;
+            if (r > tile.row_end - 1) r = tile.row_end - 1;
+            const unsigned char* x = a.x + source_row(a, r) * a.xsm + fk * 16;
+            float16_t plain;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) plain[e] = 0.0f;
+#pragma unroll 1
+            for (int k = k0; k < k1; k += 16) {
+                const uint32_t w = *(const uint32_t*)(we + ((int64_t)(k / 8 + fk) * a.N + col) * 4);
+                const int64_t at = ((int64_t)(k / a.group) * a.N + col) * 2;
+                const float sc = low16<BF16>(*(const uint16_t*)(se + at));
+                const float z = a.zeros == nullptr ? 0.0f : low16<BF16>(*(const uint16_t*)(ze + at)) * __builtin_fmaf(a.c2, sc, a.c1);
+                u32x4 b;
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    b[q] = pack16<BF16>(__builtin_fmaf((float)((w >> (8 * q)) & 15u), sc, z), __builtin_fmaf((float)((w >> (8 * q + 4)) & 15u), sc, z));
+                plain = mfma(b, *(const u32x4*)(x + (int64_t)k * 2), plain);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if (!(__builtin_fabsf(acc[i][0][e]) < __builtin_inff())) acc[i][0][e] = plain[e];
+        }
     } else {
         u32x4 fa[2][TI], fb[2][TJ];
         auto read_a = [&](const unsigned char* base, int s, int buf, int i) __attribute__((always_inline)) {
@@ -308,45 +541,6 @@ __device__ __forceinline__ void gemm_tile(const ExpertArgs& a, const ExpertTile&
             else
                 acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, b), __builtin_bit_cast(half8_t, fa[buf][i]), acc[i][j], 0, 0, 0);
         };
-        // W4: words of the K-step at hand and the next one, constants of the stage's two 32-halves
-        uint32_t words[2][TJ];
-        ColMeta<W32> meta[2][TJ];
-        uint32_t raw_s[2][TJ], raw_z[2][TJ];
-        auto read_words = [&](const unsigned char* base, int s, int buf) __attribute__((always_inline)) {
-#pragma unroll
-            for (int j = 0; j < TJ; ++j) words[buf][j] = *(const uint32_t*)(base + B_OFF + (2 * s + fk) * (BN * 4) + (wn * WC + j * 32 + fr) * 4);
-        };
-        auto read_meta = [&](const unsigned char* base) __attribute__((always_inline)) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int j = 0; j < TJ; ++j) {
-                    raw_s[h][j] = *(const uint16_t*)(base + M_OFF + h * (BN * 4) + (wn * WC + j * 32 + fr) * 2);
-                    raw_z[h][j] = *(const uint16_t*)(base + M_OFF + h * (BN * 4) + BN * 2 + (wn * WC + j * 32 + fr) * 2);
-                }
-        };
-        auto convert_meta = [&](int h) __attribute__((always_inline)) {
-#pragma unroll
-            for (int j = 0; j < TJ; ++j) {
-                const float s = low16<BF16>(raw_s[h][j]);
-                float z = low16<BF16>(raw_z[h][j]);
-                z = a.zeros == nullptr ? 0.0f : z * __builtin_fmaf(a.c2, s, a.c1);
-                meta[h][j] = make_meta<W32, 0>(s, z);
-            }
-        };
-        uint32_t nat_mask = 0x00F0000Fu, nat_magic = 0x54006400u;
-        asm volatile("" : "+s"(nat_mask), "+v"(nat_magic));
-        // register q (codes 2q, 2q + 1) of the operand of column set j
-        auto dequant = [&](uint32_t w, const ColMeta<W32>& m, int q) __attribute__((always_inline)) -> uint32_t {
-            if constexpr (W32) {
-                uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
-                asm("" : "+v"(lo), "+v"(hi));  // opaque: whole bytes, so that each is one v_cvt_f32_ubyte
-                return pack16<BF16>(__builtin_fmaf((float)((lo >> (8 * q)) & 0xffu), m.s, m.z), __builtin_fmaf((float)((hi >> (8 * q)) & 0xffu), m.s, m.z));
-            } else {
-                return dequant_pair<BF16>((__builtin_amdgcn_perm(w, w, 0x0c000c00u | (q << 16) | q) & nat_mask) | nat_magic, m, 1024.0f, 64.0f);
-            }
-        };
-
         // the copies of the last K-step's slice q (the slot is free behind the stage's barrier)
         auto refill_slice = [&](int k, int slot, int q, bool on) __attribute__((always_inline)) {
             if (!on) return;
@@ -358,17 +552,8 @@ __device__ __forceinline__ void gemm_tile(const ExpertArgs& a, const ExpertTile&
         const unsigned char* base = smem;
 #pragma unroll
         for (int i = 0; i < TI; ++i) read_a(base, 0, 0, i);
-        if constexpr (W4) {
-            read_meta(base);
-            read_words(base, 0, 0);
-            convert_meta(0);
-            convert_meta(1);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) fb[0][0][q] = dequant(words[0][0], meta[0][0], q);
-        } else {
-#pragma unroll
-            for (int j = 0; j < TJ; ++j) read_b(base, 0, 0, j);
-        }
+        for (int j = 0; j < TJ; ++j) read_b(base, 0, 0, j);
         int slot = 0;
         auto stage = [&](int k, auto refill_tag) __attribute__((always_inline)) {
             constexpr bool REFILL = decltype(refill_tag)::value;
@@ -388,39 +573,14 @@ __device__ __forceinline__ void gemm_tile(const ExpertArgs& a, const ExpertTile&
                 const int s1 = (s + 1) & 3;
                 // slices of one MFMA each, with the scheduler fenced between them (left alone it reads every fragment
                 // right in front of its MFMA)
-                if constexpr (W4) {
-                    read_words(from, s1, nxt);
-                    if (s == 3) read_meta(next);
-                    // MFMAs of column set 0 with the dequantisation of set 1, then set 1 with set 0 of the next K-step
 #pragma unroll
-                    for (int j = 0; j < TJ; ++j) {
-#pragma unroll
-                        for (int i = 0; i < TI; ++i) {
-                            mfma(i, j, cur, fb[0][j]);
-                            if (j == 0) read_a(from, s1, nxt, i);
-                            if (i == 0 && j == TJ - 1 && s == 3) convert_meta(0);
-#pragma unroll
-                            for (int q = i * 4 / TI; q < (i + 1) * 4 / TI; ++q) {
-                                if (j + 1 < TJ) fb[0][j + 1][q] = dequant(words[cur][j + 1], meta[s / 2][j + 1], q);
-                                // (one column set: its registers for the next K-step are the other buffer)
-                                else fb[TJ > 1 ? 0 : 1][0][q] = dequant(words[nxt][0], meta[s == 3 ? 0 : s1 / 2][0], q);
-                            }
-                            if (s == 3) refill_slice(k, slot, j * TI + i, REFILL);
-                            __builtin_amdgcn_sched_barrier(0);
-                        }
-                    }
-                    if constexpr (TJ == 1) fb[0][0] = fb[1][0];
-                    if (s == 3) convert_meta(1);
-                } else {
-#pragma unroll
-                    for (int q = 0; q < TI * TJ; ++q) {
-                        const int i = q / TJ, j = q % TJ;
-                        mfma(i, j, cur, fb[cur][j]);
-                        if (q < TJ) read_b(from, s1, nxt, q);
-                        if (j == 0) read_a(from, s1, nxt, i);
-                        if (s == 3) refill_slice(k, slot, q, REFILL);
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
+                for (int q = 0; q < TI * TJ; ++q) {
+                    const int i = q / TJ, j = q % TJ;
+                    mfma(i, j, cur, fb[cur][j]);
+                    if (q < TJ) read_b(from, s1, nxt, q);
+                    if (j == 0) read_a(from, s1, nxt, i);
+                    if (s == 3) refill_slice(k, slot, q, REFILL);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
             slot = next_slot;
@@ -481,8 +641,8 @@ __device__ __forceinline__ void gemm_tile(const ExpertArgs& a, const ExpertTile&
 
 // Workgroup tile of at most BM rows x BN columns.  A tile with fewer rows than a shorter tile has (an expert's last one)
 // runs as that: 8200 rows on 16 experts of 4096^2, 16-bit, took 329 us when every tile cost as much as a full one.
-template <int FMT, bool BF16, bool Z32, int BM, int BN>
-__global__ __launch_bounds__((GemmShape<FMT, BM, BN>::THREADS)) void experts_gemm_kernel(ExpertArgs a, int tiles_n) {
+template <int FMT, bool BF16, int BM, int BN>
+__global__ __launch_bounds__((GemmShape<FMT, BM, BN>::THREADS), (FMT == kEW4 ? 4 : 1)) void experts_gemm_kernel(ExpertArgs a, int tiles_n) {
     extern __shared__ __align__(16) unsigned char smem[];
     int ct = 0;
     const ExpertTile tile = find_tile<BM>(a.offsets, a.E, a.R, !a.to_partials, [&](int total_m) {
@@ -509,20 +669,20 @@ __global__ __launch_bounds__((GemmShape<FMT, BM, BN>::THREADS)) void experts_gem
     }
     if constexpr (BM >= 256) {
         if (rows > 128) {
-            gemm_tile<FMT, BF16, Z32, 256, BN>(a, tile, ct, smem);
+            gemm_tile<FMT, BF16, 256, BN>(a, tile, ct, smem);
             return;
         }
     }
     if constexpr (BM >= 128) {
         if (rows > 64) {
-            gemm_tile<FMT, BF16, Z32, 128, BN>(a, tile, ct, smem);
+            gemm_tile<FMT, BF16, 128, BN>(a, tile, ct, smem);
             return;
         }
     }
-    gemm_tile<FMT, BF16, Z32, 64, BN>(a, tile, ct, smem);
+    gemm_tile<FMT, BF16, 64, BN>(a, tile, ct, smem);
 }
 
-template <int FMT, bool BF16, bool Z32, int BM, int BN>
+template <int FMT, bool BF16, int BM, int BN>
 int launch_one(const ExpertArgs& a, hipStream_t stream) {
     constexpr int L64 = GemmShape<FMT, 64, BN>::LDS, L128 = BM >= 128 ? GemmShape<FMT, 128, BN>::LDS : 0, L256 = BM >= 256 ? GemmShape<FMT, 256, BN>::LDS : 0;
     constexpr int LA = L64 > L128 ? L64 : L128, LDS = LA > L256 ? LA : L256;
@@ -534,7 +694,7 @@ int launch_one(const ExpertArgs& a, hipStream_t stream) {
         set_error("experts: %lld tiles exceed the grid", (long long)grid);
         return GLA_ERR_INVALID_ARGUMENT;
     }
-    const auto kernel = experts_gemm_kernel<FMT, BF16, Z32, BM, BN>;
+    const auto kernel = experts_gemm_kernel<FMT, BF16, BM, BN>;
     static DeviceOnce once;
     if (once.first()) {
         const int rc = check_hip(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS), "hipFuncSetAttribute");
@@ -548,22 +708,20 @@ int launch_one(const ExpertArgs& a, hipStream_t stream) {
 // two workgroups share a CU and one starts while the other streams (256 tokens, 16 experts of 4096^2, 16-bit: 105 -> 98 us;
 // 64 tokens top 8 of 128, fp8 2048 -> 2 x 768: 64 -> 57 us).  4-bit weights fill LDS less and do better on 256 columns
 // (64 tokens top 2 of 8, 4096 -> 2 x 14336: 160 against 182 us), as do all taller tiles, which read least from LDS that way.
-template <int FMT, bool BF16, bool Z32 = false>
+template <int FMT, bool BF16>
 int launch_bm(const ExpertArgs& a, int bm, hipStream_t stream) {
     if constexpr (FMT != kEW4) {
-        if (bm >= 256) return launch_one<FMT, BF16, Z32, 256, 256>(a, stream);
+        if (bm >= 256) return launch_one<FMT, BF16, 256, 256>(a, stream);
     }
-    if (bm >= 128) return launch_one<FMT, BF16, Z32, 128, 256>(a, stream);
-    return launch_one<FMT, BF16, Z32, 64, FMT == kEW4 ? 256 : 128>(a, stream);
+    if (bm >= 128) return launch_one<FMT, BF16, 128, 256>(a, stream);
+    return launch_one<FMT, BF16, 64, FMT == kEW4 ? 256 : 128>(a, stream);
 }
 
 }  // namespace
 
 int launch_experts_gemm(const ExpertArgs& a, int format, bool bf16, int bm, hipStream_t stream) {
     switch (format) {
-        case kEW4:
-            if (bf16) return launch_bm<kEW4, true>(a, bm, stream);
-            return a.c2 != 0.0f && a.zeros != nullptr ? launch_bm<kEW4, false, true>(a, bm, stream) : launch_bm<kEW4, false>(a, bm, stream);
+        case kEW4: return bf16 ? launch_bm<kEW4, true>(a, bm, stream) : launch_bm<kEW4, false>(a, bm, stream);
         case kEF8: return bf16 ? launch_bm<kEF8, true>(a, bm, stream) : launch_bm<kEF8, false>(a, bm, stream);
         default: return bf16 ? launch_bm<kE16, true>(a, bm, stream) : launch_bm<kE16, false>(a, bm, stream);
     }

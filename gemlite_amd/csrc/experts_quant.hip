@@ -40,7 +40,43 @@ __global__ __launch_bounds__(256) void experts_quantise_kernel(const unsigned ch
     if (lane == 0) scales[b] = s;
 }
 
+// Sums of the groups of a row, for the tiled GEMM of 4-bit experts: L lanes to a group, 8 values of a lane at a time, in a
+// fixed order.  Bound by the bytes it reads.
+template <bool BF16, int L>
+__global__ __launch_bounds__(256) void experts_sums_kernel(const unsigned char* x, int64_t xsm, int64_t count, int groups, int group, unsigned char* sums) {
+    const int lane = threadIdx.x & (L - 1);
+    const int64_t q = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+    if (q >= count) return;  // whole sets of L lanes
+    const int64_t row = q / groups;
+    const unsigned char* p = x + row * xsm + (q - row * groups) * group * 2;
+    float s = 0.0f;
+    for (int k = lane * 8; k < group; k += L * 8) {
+        const u32x4 v = *(const u32x4*)(p + (int64_t)k * 2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s += low16<BF16>(v[i]) + high16<BF16>(v[i]);
+    }
+#pragma unroll
+    for (int m = 1; m < L; m <<= 1) s += wave_xor(s, m);
+    uint32_t t[3];
+    bf16_terms(s, t);
+    if (lane == 0) *(u32x4*)(sums + q * 16) = u32x4{high_halves(t[0], t[1]), high_halves(t[2], t[0]), high_halves(t[1], t[2]), high_halves(t[0], t[1])};
+}
+
+template <bool BF16, int L>
+void launch_sums(const void* x, int64_t xsm, int64_t count, int groups, int group, unsigned char* sums, hipStream_t stream) {
+    experts_sums_kernel<BF16, L><<<(unsigned)((count * L + 255) / 256), 256, 0, stream>>>((const unsigned char*)x, xsm, count, groups, group, sums);
+}
+
 }  // namespace
+
+int launch_experts_sums(const void* x, bool bf16, int64_t xsm, int rows, int K, int group, unsigned char* sums, hipStream_t stream) {
+    const int groups = K / group;
+    const int64_t count = (int64_t)rows * groups;
+    // (long groups: a wave each, or few groups would leave the chip empty)
+    if (group >= 1024) bf16 ? launch_sums<true, 64>(x, xsm, count, groups, group, sums, stream) : launch_sums<false, 64>(x, xsm, count, groups, group, sums, stream);
+    else bf16 ? launch_sums<true, 4>(x, xsm, count, groups, group, sums, stream) : launch_sums<false, 4>(x, xsm, count, groups, group, sums, stream);
+    return check_hip(hipGetLastError(), "experts_sums");
+}
 
 int launch_experts_quantise(const void* x, bool bf16, int64_t xsm, int rows, int K, unsigned char* codes, float* scales, hipStream_t stream) {
     const int64_t blocks = (int64_t)rows * (K / 128);

@@ -205,6 +205,83 @@ def test_every_row_in_front_of_the_first_expert(fmt):
 
 
 # ---------------------------------------------------------------------------
+# 4-bit codes are multiplied as they are: no weight is rounded
+# ---------------------------------------------------------------------------
+def raw_w4(dtype, E, K, N, gs, mode, scales, zeros, seed=0):
+    """Random codes with these group scales / zeros [E, K / gs, N] (float64 values of the type): tensors, meta, weights."""
+    dt, gdt = DT[dtype]
+    W = torch.randint(-2 ** 31, 2 ** 31, (E, K // 8, N), generator=_gen(seed), dtype=torch.int64).to(torch.int32)
+    q = torch.stack([(W >> (4 * i)) & 15 for i in range(8)], 2).reshape(E, K, N).double()
+    s, z = scales.to(dt), zeros.to(dt)
+    full = lambda t: t.double().repeat_interleave(gs, 1)   # noqa: E731
+    w = {2: q * full(s), 3: (q - full(z)) * full(s), 4: q * full(s) + full(z)}[mode]
+    zt = torch.empty(0, dtype=torch.int32) if mode == 2 else z
+    return [W.cuda(), s.cuda(), zt.cuda()], [0, 4, gs, 15, 8, gdt.value, gdt.value, 0, gdt.value, 0, mode, 1], w
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("mode", [2, 3, 4])
+@pytest.mark.parametrize("gs", [32, 64, 96, 128, 192, 1152])
+@pytest.mark.parametrize("tile_config", [16, 2016, 64, 3064, 128])
+def test_4_bit_products_are_rounded_once(dtype, mode, gs, tile_config):
+    """The one rounding of the result: uniform over a step, so an rms of u / sqrt(3) of each value or less (rounding every
+    weight as well would come to more than that)."""
+    E, R, K, N = 2, 150, 1152, 96
+    g = _gen(3)
+    s = (0.5 + torch.rand((E, K // gs, N), generator=g, dtype=torch.float64)) / (4.6 * K ** 0.5)
+    s *= torch.where(torch.rand(s.shape, generator=g) < 0.3, -1.0, 1.0)
+    z = 6 + 3 * torch.rand(s.shape, generator=g, dtype=torch.float64)
+    targs, meta, W = raw_w4(dtype, E, K, N, gs, mode, s, z if mode == 3 else -s * z)
+    x = (make_x(R, K, "bf16").float() + 0.25).to(DT[dtype][0])
+    offsets = torch.tensor([0, 70, R], dtype=torch.int32)
+    u = torch.finfo(DT[dtype][0]).eps / 2
+    y, mag = ref_rows("w4", x, W, offsets)
+    out = gemlite_amd.experts_functional(x.cuda(), None, targs, meta, offsets.cuda(), tile_config=tile_config)
+    off = 128 if dtype == "bf16" else 1024
+    slack = K * 2.0 ** -24 * (mag + x.double().abs().sum(1, keepdim=True) * (off + 15) * float(s.abs().max()))
+    check(out, y, slack, u, u / 3 ** 0.5)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("gs", [32, 64, 128])
+@pytest.mark.parametrize("tile_config", [16, 64, 2064, 128])
+def test_4_bit_groups_of_any_scale(dtype, gs, tile_config):
+    """Scales of 0 (a group of constants, or of nothing) and scales of one column that lie far apart."""
+    E, R, K, N = 1, 40, 512, 64
+    G, g = K // gs, _gen(5)
+    s = (0.5 + torch.rand((E, G, N), generator=g, dtype=torch.float64)) / 64
+    z = torch.randn((E, G, N), generator=g, dtype=torch.float64) / 16
+    s[:, torch.rand(G, generator=g) < 0.5, 8:16] = 0
+    s[:, 0, 16:24] = 0
+    s[:, :, 24:32] = 0
+    s[:, :, 32:40], z[:, :, 32:40] = 0, 0
+    s[:, ::2, 40:48] *= 2.0 ** -9
+    if dtype == "bf16":   # as far apart as only this type can
+        s[:, ::2, 48:56] *= 2.0 ** -90
+        z[:, ::2, 48:56] *= 2.0 ** -90
+    targs, meta, W = raw_w4(dtype, E, K, N, gs, 4, s, z)
+    x = make_x(R, K, dtype)
+    offsets = torch.tensor([0, R], dtype=torch.int32)
+    u = torch.finfo(DT[dtype][0]).eps / 2
+    y, mag = ref_rows("w4", x, W, offsets)
+    out = gemlite_amd.experts_functional(x.cuda(), None, targs, meta, offsets.cuda(), tile_config=tile_config)
+    off = 128 if dtype == "bf16" else 1024
+    scale = targs[1].cpu().double().abs().amax(1)
+    slack = K * 2.0 ** -24 * (mag + x.double().abs().sum(1, keepdim=True) * (off + 15) * scale)
+    slack[:, 48:56] += u * mag[:, 48:56]    # (scales 2^64 apart: from weights rounded to 16 bits)
+    check(out, y, slack, u, u)
+    assert not out[:, 32:40].any()
+
+
+@pytest.mark.parametrize("mode", ["gated", "combined"])
+@pytest.mark.parametrize("K,gs", [(4608, 32), (4352, 128), (2144, 32)])
+def test_many_groups_of_4_bit_experts(mode, K, gs):
+    """More groups than are joined at a time, an odd number of them, K that ends inside a stage."""
+    run_case("w4", "bf16", 3, 90, 2, K, 80, gs, drop=0.1, modes=(mode,))
+    run_case("w4", "fp16", 3, 90, 2, K, 80, gs, tile_config=5064, modes=(mode,))
+
+
+# ---------------------------------------------------------------------------
 # tall tiles, filled
 # ---------------------------------------------------------------------------
 @pytest.mark.parametrize("fmt", FORMATS)
