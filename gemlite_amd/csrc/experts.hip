@@ -7,8 +7,6 @@ namespace gla {
 
 namespace {
 
-typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
-
 struct FinishArgs {
     const float* partials;   // [S][R][N]
     const int32_t* offsets;

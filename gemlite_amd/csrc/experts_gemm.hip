@@ -1,7 +1,7 @@
 // Products grouped by expert, many rows per expert: a tiled MFMA GEMM over ragged row blocks.
 //
 //  * Workgroup tile BM rows of one expert x 256 (BM = 64: 128) columns, 8 (4) waves; pipeline stage of 128 bytes of K per
-//    activation row (64 16-bit values or 128 e4m3 codes).  Operand tiles, scales and zeros are copied global -> LDS by the load unit
+//    activation row (64 16-bit values or 128 e4m3 codes).  Operand tiles and scales are copied global -> LDS by the load unit
 //    (global_load_lds) into a ring of stages, all of them in flight; gated calls gather their activation rows on the
 //    way.  16-byte chunk c of a 128-byte row r lies at position c ^ ((r >> 1) & 7), chosen on the global side of the copy,
 //    so that the 16 lanes of an LDS read phase hit 16 different bank groups.
@@ -18,7 +18,8 @@
 //    terms: a launch in front (experts_quant.hip) takes every group's sum of x; sum and constant are three bf16 terms
 //    each (24 bits), and eight of the products of two groups fill one MFMA behind the K loop.  Sums that are not finite are
 //    taken again from dequantised weights.  (Weights dequantised and rounded in front of the MFMA: the error of a result 1.7
-//    times that of its own rounding; groups of 128 / 64 / 32 below 1040 / 1040 / 1040 us for 1070 / 1230 / 1530.)
+//    times that of its own rounding; the bf16 call below 1010 us whatever the groups, where this takes 1070 for groups of
+//    128, 1200 for 64 and 1550 for 32.)
 //  * F8: v_mfma_f32_16x16x128 starts from zero on every 128-block and its result joins the fp32 sum times the block's two
 //    scales.
 //  * gridDim.y splits K where the tiles do not fill the chip (fp32 sums to the workspace, added in order by the
@@ -27,14 +28,19 @@
 //    contiguous bands, and a band is walked in groups of 8 row tiles x all columns, so that the L2 of an XCD keeps a
 //    weight panel for all row tiles of the group.
 //
-// Measured: 4-bit, E = 8, top 2, 4096 -> 2 x 14336, 2048 tokens 1020 us (940 TFLOP/s); fp8, E = 32, top 4, 4096 -> 2 x 2048, 4096
-// tokens 383 us (1430 TFLOP/s); 16-bit, 16 experts of 4096^2, 8200 rows 320 us (860; 930 at 16000 rows).  Bound by the copies
-// into LDS beside the reads from it: reads and writes together keep the LDS port busy for as many clocks as the MFMAs
-// take (256 rows, 64 K-values: 192 KB read, 64 KB written, 2048 clocks either way).  Without the copies of the K loop the
-// three calls take 890, 324 and (16000 rows) 444 us instead of 1029, 412 and 576; the fold of the fp8 scales costs nothing.
+// Measured (calls in a row): 4-bit, E = 8, top 2, 4096 -> 2 x 14336, groups of 128, 2048 tokens 1070 us (900 TFLOP/s; fp16 1180); fp8,
+// E = 32, top 4, 4096 -> 2 x 2048, 4096 tokens 420 us (1310 TFLOP/s); 16-bit, 16 experts of 4096^2, 8200 rows 325 us (850; 1070 at 16000
+// rows in 256-row tiles).  What the counters show on random operands, and on zeros, where the power limit does not lower the clock:
+//  * 16-bit, 16000 rows: MFMA busy in 63 % of the clocks at 1.50 GHz (zeros: 54 % at 2.28 GHz, 422 for 502 us); LDS reads in 24 %,
+//    no bank conflicts; waves spend 47 % of their time at a wait.  Power first, then the waits of a ring of two stages with one
+//    workgroup per CU (the dense 16-bit kernel, four stages of half the K: 71 % at 1.55 GHz, 16384 rows in 469 us).
+//  * fp8, 16384 rows: MFMA busy 39 % at 2.02 GHz (zeros 37 % at 2.33): not power; LDS reads in 33 %, two fifths of that conflicts.
+//  * 4-bit: MFMA busy 52 %, vector instructions 63 % at 1.79 GHz (zeros 53 % and 64 % at 2.25, 870 for 1056 us).
+// Without the copies of the K loop, and so without their waits, LDS writes and power, fp8 takes 324 us instead of 412 and 16-bit (16000
+// rows) 444 instead of 576; the fold of the fp8 scales costs nothing.
 // Measured and not kept: four waves with 128 x 128 wave tiles (a third less read from LDS, one wave per SIMD: 635 against 576
-// us at 16000 rows, 4-bit 1222 against 1009), 256 x 128 tiles on four waves with two workgroups per CU (667), stages of 64
-// bytes of K in a ring of four (600; 128 rows 733 against 598).
+// us at 16000 rows), 256 x 128 tiles on four waves with two workgroups per CU (667), stages of 64 bytes of K in a ring of four
+// (600; 128 rows 733 against 598).
 #include <type_traits>
 
 #include "common.hpp"
@@ -44,16 +50,7 @@ namespace gla {
 
 namespace {
 
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
-
 __device__ __align__(16) unsigned char g_zero_chunk[16];  // what activations past the end of K are read from
-
-template <int N>
-__device__ __forceinline__ void wait_vmcnt_e() {
-    static_assert(N >= 0 && N < 64, "vmcnt is a 6-bit counter");
-    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
-}
 
 __device__ __forceinline__ void bare_barrier() {
     asm volatile("" ::: "memory");
@@ -220,8 +217,8 @@ __device__ __forceinline__ void gemm_tile(const ExpertArgs& a, const ExpertTile&
 #pragma unroll
             for (int c = 0; c < LPS; ++c) issue_one(u, u, c);
         }
-    if (stages >= RING) wait_vmcnt_e<(RING - 1) * LPS>();
-    else wait_vmcnt_e<0>();
+    if (stages >= RING) wait_vmcnt<(RING - 1) * LPS>();
+    else wait_vmcnt<0>();
     bare_barrier();
 
     if constexpr (F8) {
@@ -270,7 +267,7 @@ __device__ __forceinline__ void gemm_tile(const ExpertArgs& a, const ExpertTile&
                 const int i = q / TJ, j = q % TJ;
                 if (q == (TI - 1) * TJ) {
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                    wait_vmcnt_e<REFILL ? (RING - 2) * LPS : 0>();
+                    wait_vmcnt<REFILL ? (RING - 2) * LPS : 0>();
                     bare_barrier();
                 }
                 d[q % 4] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j].v, fa[i & 1].v, zero4, 0, 0, 0, 127, 0, 127);
@@ -383,7 +380,7 @@ __device__ __forceinline__ void gemm_tile(const ExpertArgs& a, const ExpertTile&
                 const int cur = s & 1, nxt = cur ^ 1;
                 if (s == 3) {  // as for 16-bit weights
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                    wait_vmcnt_e<REFILL ? (RING - 2) * LPS : 0>();
+                    wait_vmcnt<REFILL ? (RING - 2) * LPS : 0>();
                     bare_barrier();
                 }
                 const unsigned char* from = s == 3 ? next : base;
@@ -566,7 +563,7 @@ __device__ __forceinline__ void gemm_tile(const ExpertArgs& a, const ExpertTile&
                     // the fragments of this K-step are in registers; the next stage's copies have landed, here and (behind the
                     // barrier) everywhere, and nobody reads this stage's slot any more
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                    wait_vmcnt_e<REFILL ? (RING - 2) * LPS : 0>();
+                    wait_vmcnt<REFILL ? (RING - 2) * LPS : 0>();
                     bare_barrier();
                 }
                 const unsigned char* from = s == 3 ? next : base;

@@ -10,9 +10,6 @@ namespace gla {
 
 namespace {
 
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
-
 template <bool BF16>
 __global__ __launch_bounds__(256) void experts_quantise_kernel(const unsigned char* x, int64_t xsm, int64_t blocks, int per_row, int K,
                                                                unsigned char* codes, float* scales) {

@@ -19,10 +19,11 @@
 //    go into one v_mfma_f32_16x16x128 that starts from zero, and its result joins the fp32 sum times the two scales.
 //  * 16-bit weights: plain MFMAs.
 //
-// Measured (all weights from memory): 4-bit, E = 8, top 2, 4096 -> 2 x 14336, one token 27 us for 117 MB; 14336 -> 4096, 16
-// tokens 45 us for 247 MB (5.5 TB/s); E = 64, top 6, 2048 -> 2 x 1408, 61 tokens 51 us for 208 MB (a workgroup's K range is
-// 4 to 8 units there and its start weighs as much as its stream); 16-bit, 16 experts of 2048 x 1000, 129 rows 13 us for 66 MB;
-// fp8, E = 128, top 8, 768 -> 2048, one token 7 us.
+// Measured (calls in a captured graph, copies of the weights in turn that make 700 MB together / the same weights again, which the
+// 256 MB cache keeps in part): 4-bit, E = 8, top 2, 4096 -> 2 x 14336, one token 29.5 / 28.4 us for 117 MB; 14336 -> 4096, 16 tokens 48 / 48 us
+// with the finishing kernel's 4 for 247 MB (5.5 TB/s); E = 64, top 6, 2048 -> 2 x 1408, 61 tokens 50 / 51 us for 208 MB (a workgroup's K
+// range is 4 to 8 units there and its start weighs as much as its stream); 16-bit, 16 experts of 2048 x 1000, 129 rows 14.1 / 12.6 us
+// for 66 MB; fp8, E = 128, top 8, 768 -> 2048, one token 11.1 / 10.0 us with the finishing kernel's 4.
 #include <type_traits>
 
 #include "common.hpp"
@@ -32,15 +33,11 @@ namespace gla {
 
 namespace {
 
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
-
 __device__ __align__(16) unsigned char g_zero_piece[16];  // what activations past the end of K are read from
 
 template <int N>
-__device__ __forceinline__ void wait_vmcnt_s() {
-    static_assert(N >= 0 && N < 64, "vmcnt is a 6-bit counter");
-    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+__device__ __forceinline__ void wait_copies() {
+    wait_vmcnt<N>();
     asm volatile("" ::: "memory");
 }
 
@@ -295,7 +292,7 @@ __global__ __launch_bounds__(NW * 64, 2) void experts_stream_kernel(ExpertArgs a
         int u = u0, at = 0;
 #pragma unroll 1
         for (; u + D < u1; ++u) {
-            wait_vmcnt_s<(D - 1) * OPS>();
+            wait_copies<(D - 1) * OPS>();
             unsigned char* slot = ring + at * SLOT;
             unit(slot, [&]() __attribute__((always_inline)) {
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot has been read
@@ -306,9 +303,9 @@ __global__ __launch_bounds__(NW * 64, 2) void experts_stream_kernel(ExpertArgs a
 #pragma unroll 1
         for (; u < u1; ++u) {
             // (the last D units: the counter cannot tell them apart by one constant)
-            if (D > 2 && u + 2 < u1) wait_vmcnt_s<(D - 1) * OPS>();
-            else if (u + 1 < u1) wait_vmcnt_s<OPS>();
-            else wait_vmcnt_s<0>();
+            if (D > 2 && u + 2 < u1) wait_copies<(D - 1) * OPS>();
+            else if (u + 1 < u1) wait_copies<OPS>();
+            else wait_copies<0>();
             unit(ring + at * SLOT, []() __attribute__((always_inline)) {});
             at = at == D - 1 ? 0 : at + 1;
         }

@@ -222,7 +222,7 @@ def raw_w4(dtype, E, K, N, gs, mode, scales, zeros, seed=0):
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("mode", [2, 3, 4])
 @pytest.mark.parametrize("gs", [32, 64, 96, 128, 192, 1152])
-@pytest.mark.parametrize("tile_config", [16, 2016, 64, 3064, 128])
+@pytest.mark.parametrize("tile_config", [16, 2016, 64, 2064, 3064, 128])
 def test_4_bit_products_are_rounded_once(dtype, mode, gs, tile_config):
     """The one rounding of the result: uniform over a step, so an rms of u / sqrt(3) of each value or less (rounding every
     weight as well would come to more than that)."""
