@@ -311,7 +311,7 @@ __global__ __launch_bounds__(NW * 64, 2) void experts_stream_kernel(ExpertArgs a
         }
         if constexpr (FMT == kEW4) {
             // A sum that is not finite may be so only because of the codes' offset (inf - inf, or an overflow of 128 x): such
-            // sums are taken again from dequantised weights, rounded to 16 bits as in the tiled GEMM.
+            // sums are taken again from dequantised weights, rounded to 16 bits.
             bool odd = false;
 #pragma unroll
             for (int t = 0; t < NT; ++t)

@@ -31,7 +31,7 @@ _ROWS, _GATED, _COMBINED = 0, 1, 2
 class ExpertPlan(NamedTuple):
     """Which experts every token goes to, and the (token, slot) pairs sorted by expert.
 
-    ``weights`` [T, k] fp32 and ``expert_ids`` [T, k] int32 (-1: no expert); ``offsets`` [E + 1] int32: rows
+    ``weights`` [T, k] fp32 and ``expert_ids`` [T, k] int32 (-1 or another id outside ``0 .. E - 1``: no expert); ``offsets`` [E + 1] int32: rows
     ``offsets[e] .. offsets[e + 1] - 1`` of the sorted rows are expert ``e``'s, rows from ``offsets[E]`` on have none;
     ``order`` [T k] int32: flat index ``token * k + slot`` of every sorted row; ``places`` [T, k] int32: sorted row of
     every pair.
