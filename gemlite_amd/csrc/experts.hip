@@ -1,5 +1,7 @@
 // C entry points of the mixture-of-experts operators: argument checks, the choice between the streaming kernel and the
 // tiled GEMM, and the finishing kernel that joins K splits and the experts of a token.
+#include <numeric>
+
 #include "common.hpp"
 #include "experts.hpp"
 
@@ -241,6 +243,11 @@ ExpertPlanHost plan_of(const gla_experts_args& p) {
     const int unit = stream || h.format == kEF8 ? 128 : 64, parts = stream ? h.waves * h.S : h.S;
     const int n_units = (p.K + unit - 1) / unit;
     h.chunk = (n_units + parts - 1) / parts;
+    if (!stream && h.format == kEW4) {
+        // splits begin where groups do: a group's second term and all of its first belong to one of them
+        const int m = p.group_size / std::gcd(p.group_size, unit);
+        h.chunk = (h.chunk + m - 1) / m * m;
+    }
     if (!stream) h.S = (n_units + h.chunk - 1) / h.chunk;  // every split has a stage
     h.to_partials = p.mode == GLA_EXPERTS_COMBINED || h.S > 1;
     h.partial_bytes = h.to_partials ? (int64_t)h.S * p.R * p.N * 4 : 0;

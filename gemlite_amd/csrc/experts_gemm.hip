@@ -345,7 +345,7 @@ __device__ __forceinline__ void gemm_tile(const ExpertArgs& a, const ExpertTile&
             }
         };
         const int halves = a.group / 32;
-        int left = halves - (2 * k_first) % halves;  // 32-halves to the next group
+        int left = halves;  // 32-halves to the next group (a split begins where a group does)
         bool enters = false;
         float unit = 1.0f;                           // the scale the column's sums are divided by
         auto enter_group = [&]() __attribute__((always_inline)) {
@@ -434,9 +434,9 @@ __device__ __forceinline__ void gemm_tile(const ExpertArgs& a, const ExpertTile&
 #pragma unroll
         for (int i = 0; i < TI; ++i) times(i);
 
-        // ---- the groups' constants times their sums of activations, two groups to an MFMA: the groups that begin in this split
+        // ---- the groups' constants times their sums of activations, two groups to an MFMA
         const int k0 = k_first * 64, k1 = k0 + stages * 64 < a.K ? k0 + stages * 64 : a.K;
-        const int g0 = (k0 + a.group - 1) / a.group, g1 = (k1 + a.group - 1) / a.group;
+        const int g0 = k0 / a.group, g1 = (k1 + a.group - 1) / a.group;
         const int col = unit_column_inside<WC>(a.half, a.N, ct * SH::WN + wn, fr & ~3) + (fr & 3);
         constexpr int AT_ONCE = 16, PIECES = BM * AT_ONCE / SH::THREADS, STEPS = AT_ONCE / 2;  // groups, pieces per thread, MFMAs
         static_assert(BM * AT_ONCE * 16 <= SH::X_OFF, "sums of a chunk of groups fit the ring");

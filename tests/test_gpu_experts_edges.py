@@ -281,6 +281,25 @@ def test_many_groups_of_4_bit_experts(mode, K, gs):
     run_case("w4", "fp16", 3, 90, 2, K, 80, gs, tile_config=5064, modes=(mode,))
 
 
+@pytest.mark.parametrize("gs", [96, 128, 192, 1152])
+@pytest.mark.parametrize("tile_config", [2016, 2064, 3064, 5064])
+def test_one_group_of_another_scale_and_k_splits(gs, tile_config):
+    """A column that one split takes from rounded weights (scales far apart) and the others do not; groups at the splits' ends."""
+    E, R, K, N = 1, 40, 1152, 64
+    G, g = K // gs, _gen(6)
+    s = (0.5 + torch.rand((E, G, N), generator=g, dtype=torch.float64)) / 64
+    z = torch.randn((E, G, N), generator=g, dtype=torch.float64) / 16
+    s[:, min(1, G - 1), ::2] *= 2.0 ** -90
+    targs, meta, W = raw_w4("bf16", E, K, N, gs, 4, s, z)
+    x = (make_x(R, K, "bf16").float() + 1).bfloat16()
+    offsets = torch.tensor([0, R], dtype=torch.int32)
+    y, mag = ref_rows("w4", x, W, offsets)
+    out = gemlite_amd.experts_functional(x.cuda(), None, targs, meta, offsets.cuda(), tile_config=tile_config)
+    u = 2.0 ** -8
+    slack = u * mag + K * 2.0 ** -24 * (mag + x.double().abs().sum(1, keepdim=True) * (128 + 15) * float(s.max()))
+    check(out, y, slack, u, 1.5 * u)
+
+
 # ---------------------------------------------------------------------------
 # tall tiles, filled
 # ---------------------------------------------------------------------------
