@@ -348,13 +348,18 @@ __device__ __forceinline__ void gemm_tile(const ExpertArgs& a, const ExpertTile&
         int left = halves;  // 32-halves to the next group (a split begins where a group does)
         bool enters = false;
         float unit = 1.0f;                           // the scale the column's sums are divided by
+        // exponent of the column's first scale that is not 0 (-1: none yet): the others have to be within 2^60 of it, so that no
+        // sum in their units leaves fp32's range
+        int reference = -1;
+        auto exponent = [](float s) __attribute__((always_inline)) { return (int)(__builtin_bit_cast(uint32_t, s) >> 23 & 255u); };
         auto enter_group = [&]() __attribute__((always_inline)) {
             const float s = low16<BF16>(scale);
             float r = 1.0f;
             if (s != 0.0f) {
-                r = unit / s;
-                const float m = __builtin_fabsf(r);
-                if (!(m < 0x1p64f && m > 0x1p-64f)) r = __builtin_nanf("");  // (taken again below)
+                if (reference < 0) reference = exponent(s);  // (the sums are 0)
+                else r = unit / s;
+                const int off = exponent(s) - reference;
+                if (off > 60 || off < -60) r = __builtin_nanf("");  // (taken again below)
                 unit = s;
             }
             put(r);
@@ -366,7 +371,10 @@ __device__ __forceinline__ void gemm_tile(const ExpertArgs& a, const ExpertTile&
         read_scale(base, 0);
         read_word(base, 0);
         choose();
-        if (low16<BF16>(scale) != 0.0f) unit = low16<BF16>(scale);
+        if (low16<BF16>(scale) != 0.0f) {
+            unit = low16<BF16>(scale);
+            reference = exponent(unit);
+        }
 #pragma unroll
         for (int q = 0; q < 4; ++q) fb[0][q] = convert(q);
         int slot = 0;
@@ -495,7 +503,7 @@ __device__ __forceinline__ void gemm_tile(const ExpertArgs& a, const ExpertTile&
         }
 
         // ---- sums that are not finite, perhaps only because of the codes' offset (inf - inf, or an overflow of OFF x) or of scales
-        // that are 2^64 apart: again from dequantised weights, rounded to 16 bits
+        // that are 2^60 apart: again from dequantised weights, rounded to 16 bits
 #pragma unroll
         for (int i = 0; i < TI; ++i) {
             bool odd = false;

@@ -268,7 +268,7 @@ def test_4_bit_groups_of_any_scale(dtype, gs, tile_config):
     off = 128 if dtype == "bf16" else 1024
     scale = targs[1].cpu().double().abs().amax(1)
     slack = K * 2.0 ** -24 * (mag + x.double().abs().sum(1, keepdim=True) * (off + 15) * scale)
-    slack[:, 48:56] += u * mag[:, 48:56]    # (scales 2^64 apart: from weights rounded to 16 bits)
+    slack[:, 48:56] += u * mag[:, 48:56]    # (scales 2^60 apart: from weights rounded to 16 bits)
     check(out, y, slack, u, u)
     assert not out[:, 32:40].any()
 
@@ -298,6 +298,25 @@ def test_one_group_of_another_scale_and_k_splits(gs, tile_config):
     u = 2.0 ** -8
     slack = u * mag + K * 2.0 ** -24 * (mag + x.double().abs().sum(1, keepdim=True) * (128 + 15) * float(s.max()))
     check(out, y, slack, u, 1.5 * u)
+
+
+@pytest.mark.parametrize("order", [1, -1])
+@pytest.mark.parametrize("tile_config", [16, 64, 128])
+def test_scales_that_climb_far(order, tile_config):
+    """Steps that are each in range and leave the range together; only the group of the least scale has activations."""
+    E, R, K, N = 1, 24, 512, 64
+    steps = torch.tensor([-100, -40, 20, 80], dtype=torch.float64)
+    s = (2.0 ** steps.flip(0) if order < 0 else 2.0 ** steps).view(1, 4, 1).expand(1, 4, N).clone()
+    targs, meta, W = raw_w4("bf16", E, K, N, 128, 2, s, s)
+    x = make_x(R, K, "bf16")
+    x[:, 128:] = 0
+    if order < 0:
+        x = x.flip(1).contiguous()
+    offsets = torch.tensor([0, R], dtype=torch.int32)
+    y, mag = ref_rows("w4", x, W, offsets)
+    out = gemlite_amd.experts_functional(x.cuda(), None, targs, meta, offsets.cuda(), tile_config=tile_config)
+    u = 2.0 ** -8
+    check(out, y, u * mag + K * 2.0 ** -24 * (mag + x.double().abs().sum(1, keepdim=True) * (128 + 15) * 2.0 ** -100), u, 1.5 * u)
 
 
 # ---------------------------------------------------------------------------
