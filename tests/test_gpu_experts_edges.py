@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import gemlite_amd
-from gemlite_amd import ExpertPlan, GemLiteExperts, GemLiteLinear
+from gemlite_amd import ExpertPlan, GemLiteExperts, GemLiteLinear, GemLiteMoE
 from gemlite_amd.helper import A16W4_HQQ_INT
 from test_gpu_experts import DT, FORMATS, _gen, check, make_layers, make_x, ref_plan, ref_route, ref_rows, run_case, silu
 
@@ -348,6 +348,27 @@ def test_tiles_filled_to_the_last_row(fmt, dtype, tile_config):
 def test_heights_the_library_chooses(fmt, E, T, K, N):
     """256-row tiles of 16-bit and fp8 weights, streamed fp8 weights, 128-row tiles of 4-bit weights."""
     run_case(fmt, "bf16", E, T, 1, K, N)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_replayed_blocks_of_many_tokens(fmt):
+    """Launches in front of the tiled kernels (quantiser, sums of groups) in a captured graph, against eager calls."""
+    E, k, hidden, inter, T = 4, 2, 256, 128, 300
+    gate_up = GemLiteExperts.from_layers(make_layers(fmt, "bf16", E, hidden, 2 * inter, 64, 0)[0])
+    down = GemLiteExperts.from_layers(make_layers(fmt, "bf16", E, inter, hidden, 64, 50)[0])
+    moe = GemLiteMoE(gate_up, down, k)
+    x, logits = make_x(T, hidden, "bf16").cuda(), torch.randn((T, E), generator=_gen(1)).cuda()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = moe(x, logits)
+    for i in range(4):
+        x.copy_(make_x(T, hidden, "bf16", 20 + i).cuda())
+        logits.copy_(torch.randn((T, E), generator=_gen(30 + i)).cuda())
+        want = moe(x, logits)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
 
 
 def test_many_slots_for_a_token():
