@@ -28,7 +28,8 @@
 //    contiguous bands, and a band is walked in groups of 8 row tiles x all columns, so that the L2 of an XCD keeps a
 //    weight panel for all row tiles of the group.
 //
-// Measured (calls in a row): 4-bit, E = 8, top 2, 4096 -> 2 x 14336, groups of 128, 2048 tokens 1070 us (900 TFLOP/s; fp16 1180); fp8,
+// Measured (calls in a row): 4-bit, E = 8, top 2, 4096 -> 2 x 14336, groups of 128, 2048 tokens 1060 to 1140 us
+// by card (840 to 910 TFLOP/s; fp16 1180); fp8,
 // E = 32, top 4, 4096 -> 2 x 2048, 4096 tokens 420 us (1310 TFLOP/s); 16-bit, 16 experts of 4096^2, 8200 rows 325 us (850; 1070 at 16000
 // rows in 256-row tiles).  What the counters show on random operands, and on zeros, where the power limit does not lower the clock:
 //  * 16-bit, 16000 rows: MFMA busy in 63 % of the clocks at 1.50 GHz (zeros: 54 % at 2.28 GHz, 422 for 502 us); LDS reads in 24 %,
